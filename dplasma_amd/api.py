@@ -111,13 +111,13 @@ def _prec_checked(prec, fn):
     return wrapper
 
 
-def register_op(name, fn):
-    """Register a generic op and its s/d/c/z aliases (+ _Destruct for _New ops)."""
+def register_op(name, fn, precs="sdcz"):
+    """Register a generic op and its aliases, s/d/c/z by default (+ _Destruct for _New ops)."""
     _register(name, fn)
     if name.endswith("_New"):
         base = name[:-4]
         _register(base + "_Destruct", _destruct)
-    for p in "sdcz":
+    for p in precs:
         alias = p + name
         _register(alias, _prec_checked(p, fn))
         if name.endswith("_New"):
@@ -290,3 +290,9 @@ def getrs_incpiv(ctx, trans, A, L, IPIV, B):
 for _n, _f in (("potrf_rec", potrf_rec), ("geqrf_rec", geqrf_rec), ("poinv_sync", poinv_sync),
                ("getrs_incpiv", getrs_incpiv), ("hbrdt", _eig.hbrdt)):
     register_op(_n, _f)
+
+# Products whose matrix depends on the column: low-rank adapters beside a projection, mixtures of experts
+from .models import indexed as _indexed  # noqa: E402
+for _n in ("gemm_lora", "gemm_lora_grad", "moe"):
+    register_op(_n, getattr(_indexed, _n), precs="sdhb")
+    register_op(_n + "_New", getattr(_indexed, _n + "_New"), precs="sdhb")

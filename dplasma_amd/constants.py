@@ -128,6 +128,9 @@ PREC_DTYPE = {
     "z": torch.complex128,
 }
 DTYPE_PREC = {v: k for k, v in PREC_DTYPE.items()}
+# half precisions: descriptors and the products of models/indexed.py only (no kernel code in DTYPE_CODE)
+HALF_DTYPE = {"h": torch.float16, "b": torch.bfloat16}
+DTYPE_PREC.update({v: k for k, v in HALF_DTYPE.items()})
 DTYPE_CODE = {
     torch.float32: dplasmaRealFloat,
     torch.float64: dplasmaRealDouble,

@@ -134,9 +134,17 @@ _SIGS = {
     "dpl_rows_xord": [c_vp, c_vp, c_vp, c_int, c_int, c_vp, c_int, c_int, c_int, c_int, c_vp, c_vp, c_vp],
     # prec, pack, tmp, ldb, W, xo, cnt, maxcnt, bufs, ldx, stream
     "dpl_rows_xcopy": [c_int, c_int, c_vp, c_int, c_int, c_vp, c_vp, c_int, c_vp, c_int, c_vp],
+    # products whose matrix depends on the column (lora.hip, moe.hip): argument record, [gradient,] stream
+    "dpl_lora": [c_vp, c_vp],
+    "dpl_lora_grad": [c_vp, c_vp],
+    "dpl_lora_ws_bytes": [c_vp, c_int],
+    "dpl_lora_args_bytes": [],
+    "dpl_moe": [c_vp, c_vp],
+    "dpl_moe_ws_bytes": [c_vp],
+    "dpl_moe_args_bytes": [],
 }
 _OPTIONAL = set()
-_RESTYPE = {"dpl_dtr_field": c_ll}
+_RESTYPE = {"dpl_dtr_field": c_ll, "dpl_lora_ws_bytes": c_ll, "dpl_moe_ws_bytes": c_ll}
 
 
 def lib_path() -> Path:

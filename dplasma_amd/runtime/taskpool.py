@@ -2,7 +2,8 @@
 
 An algorithm is compiled at ``_New`` time into a list of *tasks*; each task
 is a coarse unit (one batched kernel launch, one panel kernel, one
-collective) bound to a stream class (``panel``/``update``/``aux``) with
+collective) bound to a stream class (``panel``/``update``/``aux``, or ``caller``:
+the stream the taskpool is run from, for every task of it) with
 explicit dependencies on earlier tasks.  Execution enqueues every task in
 program order on its stream, inserting HIP event waits only for
 cross-stream edges, so the whole factorisation is queued asynchronously and
@@ -157,10 +158,13 @@ class Taskpool:
     def _run_gpu_py(self, ctx):
         from ..parallel import comm
         from ..utils import trace
+        used = {t.stream for t in self.tasks}
+        if used == {"caller"}:
+            self._run_caller(ctx)
+            return
         cur = torch.cuda.current_stream(ctx.device)
         start = torch.cuda.Event()
         start.record(cur)
-        used = {t.stream for t in self.tasks}
         for s in used:
             ctx.streams[s].wait_event(start)
         events = {}
@@ -181,6 +185,17 @@ class Taskpool:
             ev = torch.cuda.Event()
             ev.record(ctx.streams[s])
             cur.wait_event(ev)
+
+    def _run_caller(self, ctx):
+        """Tasks bound to the ``caller`` stream class: the stream that is current on the context's device when
+        the taskpool runs, in issue order -- no events, so a short product costs its launch only, and a graph
+        capture on that stream takes it in."""
+        from ..utils import trace
+        with torch.cuda.device(ctx.device):
+            for ti in self.issue_order(ctx):
+                t = self.tasks[ti]
+                with trace.span(ctx, t.name, "task"):
+                    t.fn()
 
     def complete(self, ctx=None):
         ctx = ctx or self.ctx
