@@ -1,0 +1,81 @@
+// Launchers and shared pieces of gemm_lora's kernels (lora*.hip).
+#pragma once
+#include "indexed.h"
+
+// 16 bytes per lane from memory to LDS (lane i to lds + 16 i; lds is the same for the whole wave).  The buffer form reads
+// base[off + soff ..], zeros where that is past `bytes`.
+__device__ inline void dma_buffer(const void* base, int bytes, void* lds, unsigned off, int soff) {
+#ifdef __HIP_DEVICE_COMPILE__
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void*)base, 0, bytes, 0x00020000),
+                                           (__attribute__((address_space(3))) void*)lds, 16, off, soff, 0, 0);
+#endif
+}
+__device__ inline void dma_global(const void* p, void* lds) {
+#ifdef __HIP_DEVICE_COMPILE__
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p,
+                                   (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+#endif
+}
+
+// T <= 64, forward (lora_few.hip)
+size_t lora_few_ws(const LoraArgs& g);
+int lora_few(const LoraArgs& g, hipStream_t st);
+
+// Low-rank vectors of every token as the operand of the next product (Mid<T>::elem, hi and lo parts).
+//   by token:    hi[t * rp + j], zeros for j in r .. rp (rp: r in whole matrix steps)
+//   by adapter:  thi[j * tp + pos[t]], the tokens of an adapter next to each other (the gradients of its factors)
+// Nothing is written for a token without an adapter, and nothing of it is used.
+struct LowOut {
+  void *hi, *lo;    // null: not asked for
+  void *thi, *tlo;  // null: not asked for
+  const int* pos;
+  long long tp;
+  int rp;
+};
+
+template <typename T> __device__ inline void put_low(const LowOut& o, int t, int j, typename Num<T>::acc v) {
+  typedef typename Mid<T>::elem M;
+  M h, l;
+  Mid<T>::put(&h, &l, v);
+  if (o.hi) {
+    ((M*)o.hi)[(long long)t * o.rp + j] = h;
+    if (Mid<T>::PARTS == 2) ((M*)o.lo)[(long long)t * o.rp + j] = l;
+  }
+  if (o.thi) {
+    const long long at = j * o.tp + o.pos[t];
+    ((M*)o.thi)[at] = h;
+    if (Mid<T>::PARTS == 2) ((M*)o.tlo)[at] = l;
+  }
+}
+
+static inline int low_pitch(int prec, int r) {
+  const int ks = prec == DPL_D ? 8 : prec == DPL_S ? 16 : 32;
+  return cdiv(r, ks) * ks;
+}
+static inline size_t mid_bytes(int prec) { return prec == DPL_D ? 8 : prec == DPL_S ? 4 : 2; }
+
+// out(t, j) = s_l sum_c x[t*ldx + c] F[(l*r + j)*ldf + c],  l = ids[t]
+struct LowArgs {
+  const void *x, *F, *scale;
+  const int* ids;
+  long long ldx, ldf;
+  int prec, nt, C, r, L;
+  LowOut out;
+};
+int lora_low(const LowArgs& a, hipStream_t st);
+
+// y[t*ldy + n] = alpha (sum_c x[t*ldx + c] W(n, c) + sum_j low(t, j) F[(l*N + n)*ldf + j]) + beta y[t*ldy + n];
+// nt: W(n, c) = W[n*ldw + c], else W[c*ldw + n] (h and b only)
+struct TileArgs {
+  const void *x, *W, *F, *hi, *lo;
+  const int* ids;
+  void* y;
+  long long ldx, ldw, ldf, ldy;
+  double alpha, beta;
+  int prec, T, C, N, r, rp, L;
+};
+int lora_tile(const TileArgs& a, bool nt, hipStream_t st);
+
+// Gradient in h and b (lora_grad.hip).
+size_t lora_grad_ws(const LoraArgs& g);
+int lora_grad_half(const LoraArgs& g, hipStream_t st);

@@ -6,11 +6,14 @@
 //
 // Layouts (element offsets): W[n*ldw + k], X[t*ldx + k], Y[t*ldy + n], A_l[(l*r + j)*lda + k], B_l[(l*N + n)*ldb + j].
 //
+// Here: the entry points, and the gradient in s and d.  The forward product of few tokens is in lora_few.hip, that of many
+// and the low-rank vectors in lora_tile.hip, the gradient in h and b in lora_grad.hip.
+//
 // Steps: the low-rank vectors S = s_l A_l^T x (and P = s_l B_l dy) of every token into the workspace, then the shared
 // product with the adapter's part added to the same accumulators.  Nothing of one adapter ever meets another's token:
 // where the rows of a tile use several adapters, each adapter's part is formed apart and kept by a select, so an
 // infinity or NaN in one adapter stays with its own tokens.
-#include "indexed.h"
+#include "lora.h"
 
 namespace {
 
@@ -69,15 +72,14 @@ __global__ __launch_bounds__(256) void k_lora_low(const T* __restrict__ x, long 
   }
 }
 
-// y[t*ldy + n] = alpha (sum_c x[t*ldx + c] W(n, c) + sum_j low[t*r + j] F_l(n, j)) + beta y[t*ldy + n]
-// NT (forward): W(n, c) = W[n*ldw + c], F_l(n, j) = F[(l*N + n)*ldf + j];  else (gradient) W[c*ldw + n], F[(l*r + j)*ldf + n].
-template <typename T, bool NT>
+// dx[t*ldy + n] = alpha (sum_c x[t*ldx + c] W[c*ldw + n] + sum_j low[t*r + j] F[(l*r + j)*ldf + n]),  x: dy, F: A
+template <typename T>
 __global__ __launch_bounds__(256) void k_lora_apply(const T* __restrict__ x, long long ldx, const T* __restrict__ W,
                                                     long long ldw, const T* __restrict__ F, long long ldf,
                                                     const int* __restrict__ ids,
                                                     const typename Num<T>::acc* __restrict__ low, int nt, int C, int N,
-                                                    int r, int L, typename Num<T>::acc alpha,
-                                                    typename Num<T>::acc beta, T* __restrict__ y, long long ldy) {
+                                                    int r, int L, typename Num<T>::acc alpha, T* __restrict__ y,
+                                                    long long ldy) {
   typedef typename Num<T>::acc R;
   __shared__ TileLds<R> s;
   __shared__ int sid[64];
@@ -86,21 +88,17 @@ __global__ __launch_bounds__(256) void k_lora_apply(const T* __restrict__ x, lon
   unsigned long long todo = tile_ids(sid, &sfirst, ids, t0, nt, L);
   TileAcc<R> acc, part;
   acc.zero();
-  tile_product<true, NT>(
+  tile_product<true, false>(
       s, acc, C, [&](int i, int c) { return t0 + i < nt ? widen(x[(long long)(t0 + i) * ldx + c]) : R(0); },
-      [&](int n, int c) {
-        return n0 + n < N ? widen(NT ? W[(long long)(n0 + n) * ldw + c] : W[(long long)c * ldw + n0 + n]) : R(0);
-      });
+      [&](int n, int c) { return n0 + n < N ? widen(W[(long long)c * ldw + n0 + n]) : R(0); });
   for (; todo; todo &= todo - 1) {
     const int l = sid[__builtin_ctzll(todo)];
     part.zero();
-    const T* f = F + (long long)l * (NT ? N : r) * ldf;
-    tile_product<true, NT>(
+    const T* f = F + (long long)l * r * ldf;
+    tile_product<true, false>(
         s, part, r,
         [&](int i, int c) { return t0 + i < nt && sid[i] == l ? low[(long long)(t0 + i) * r + c] : R(0); },
-        [&](int n, int c) {
-          return n0 + n < N ? widen(NT ? f[(long long)(n0 + n) * ldf + c] : f[(long long)c * ldf + n0 + n]) : R(0);
-        });
+        [&](int n, int c) { return n0 + n < N ? widen(f[(long long)c * ldf + n0 + n]) : R(0); });
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -113,12 +111,7 @@ __global__ __launch_bounds__(256) void k_lora_apply(const T* __restrict__ x, lon
         }
   }
   acc.each([&](int i, int n, R& v) {
-    if (t0 + i < nt && n0 + n < N) {
-      T* p = &y[(long long)(t0 + i) * ldy + n0 + n];
-      R o = alpha == R(0) ? R(0) : alpha * v;
-      if (beta != R(0)) o += beta * widen(*p);
-      *p = (T)o;
-    }
+    if (t0 + i < nt && n0 + n < N) y[(long long)(t0 + i) * ldy + n0 + n] = (T)(alpha == R(0) ? R(0) : alpha * v);
   });
 }
 
@@ -181,37 +174,23 @@ __global__ __launch_bounds__(256) void k_lora_outer(const T* __restrict__ z, lon
   });
 }
 
-template <typename T> struct LoraWs {
+template <typename T> struct PlainWs {
   typename Num<T>::acc *S, *P;
   int *off, *perm;
   size_t bytes;
-  LoraWs(const LoraArgs& g, void* ws, bool grad) {
+  PlainWs(const LoraArgs& g, void* ws) {
     Carve c{(char*)ws};
     S = c.take<typename Num<T>::acc>((size_t)g.T * g.r);
-    P = grad ? c.take<typename Num<T>::acc>((size_t)g.T * g.r) : nullptr;
-    off = grad ? c.take<int>(g.L + 1) : nullptr;
-    perm = grad ? c.take<int>(g.T) : nullptr;
+    P = c.take<typename Num<T>::acc>((size_t)g.T * g.r);
+    off = c.take<int>(g.L + 1);
+    perm = c.take<int>(g.T);
     bytes = c.used;
   }
 };
 
-template <typename T> int run_forward(const LoraArgs& g, hipStream_t st) {
-  typedef typename Num<T>::acc R;
-  LoraWs<T> w(g, g.ws, false);
-  if ((size_t)g.ws_bytes < w.bytes) return -2;
-  const int tt = cdiv(g.T, 64);
-  const T *X = (const T*)g.X, *A = (const T*)g.A, *B = (const T*)g.B, *W = (const T*)g.W;
-  const int* ids = (const int*)g.ids;
-  if (g.L > 0)
-    k_lora_low<T, true><<<dim3(tt, cdiv(g.r, 64)), 256, 0, st>>>(X, g.ldx, A, g.lda, ids, (const R*)g.scale, g.T, g.K, g.r, g.L, w.S);
-  k_lora_apply<T, true><<<dim3(cdiv(g.N, 64), tt), 256, 0, st>>>(X, g.ldx, W, g.ldw, B, g.ldb, ids, w.S, g.T, g.K, g.N, g.r, g.L,
-                                                                 (R)g.alpha, (R)g.beta, (T*)g.Y, g.ldy);
-  return (int)hipGetLastError();
-}
-
 template <typename T> int run_grad(const LoraArgs& g, hipStream_t st) {
   typedef typename Num<T>::acc R;
-  LoraWs<T> w(g, g.ws, true);
+  PlainWs<T> w(g, g.ws);
   if ((size_t)g.ws_bytes < w.bytes) return -2;
   const int tt = cdiv(g.T, 64), rt = cdiv(g.r, 64);
   const T *X = (const T*)g.X, *A = (const T*)g.A, *B = (const T*)g.B, *W = (const T*)g.W, *dY = (const T*)g.dY;
@@ -219,8 +198,8 @@ template <typename T> int run_grad(const LoraArgs& g, hipStream_t st) {
   const R* scale = (const R*)g.scale;
   if (g.L > 0 && g.T > 0) k_lora_low<T, false><<<dim3(tt, rt), 256, 0, st>>>(dY, g.ldy, B, g.ldb, ids, scale, g.T, g.N, g.r, g.L, w.P);
   if (g.dX && g.T > 0 && g.K > 0)
-    k_lora_apply<T, false><<<dim3(cdiv(g.K, 64), tt), 256, 0, st>>>(dY, g.ldy, W, g.ldw, A, g.lda, ids, w.P, g.T, g.N, g.K, g.r, g.L,
-                                                                    (R)g.alpha, R(0), (T*)g.dX, g.lddx);
+    k_lora_apply<T><<<dim3(cdiv(g.K, 64), tt), 256, 0, st>>>(dY, g.ldy, W, g.ldw, A, g.lda, ids, w.P, g.T, g.N, g.K, g.r, g.L,
+                                                             (R)g.alpha, (T*)g.dX, g.lddx);
   if ((g.dA || g.dB) && g.L > 0) {
     k_lora_sort<<<g.L, 256, 0, st>>>(ids, g.T, g.L, w.off, w.perm);
     if (g.dA && g.K > 0)
@@ -233,31 +212,45 @@ template <typename T> int run_grad(const LoraArgs& g, hipStream_t st) {
   return (int)hipGetLastError();
 }
 
+// T > 64: the low-rank vectors, then the shared product that adds the adapters' parts
+size_t forward_ws(const LoraArgs& g) {
+  return g.T <= 64 ? lora_few_ws(g) : ((size_t)g.T * low_pitch(g.prec, g.r) * mid_bytes(g.prec) + 255 & ~(size_t)255) * 2;
+}
+
+int forward(const LoraArgs& g, hipStream_t st) {
+  if ((size_t)g.ws_bytes < forward_ws(g)) return -2;
+  if (g.T <= 64) return lora_few(g, st);
+  const int rp = low_pitch(g.prec, g.r);
+  const int* ids = (const int*)g.ids;
+  char *hi = (char*)g.ws, *lo = hi + forward_ws(g) / 2;
+  if (g.L > 0) {
+    const int rc = lora_low({g.X, g.A, g.scale, ids, g.ldx, g.lda, g.prec, g.T, g.K, g.r, g.L, {hi, lo, nullptr, nullptr, nullptr, 0, rp}}, st);
+    if (rc) return rc;
+  }
+  return lora_tile({g.X, g.W, g.B, hi, lo, ids, g.Y, g.ldx, g.ldw, g.ldb, g.ldy, g.alpha, g.beta, g.prec, g.T, g.K, g.N, g.r, rp, g.L}, true, st);
+}
+
 }  // namespace
 
 DPL_API int dpl_lora_args_bytes() { return (int)sizeof(LoraArgs); }
 
 DPL_API long long dpl_lora_ws_bytes(const LoraArgs* g, int grad) {
-  return (long long)(g->prec == DPL_D ? LoraWs<double>(*g, nullptr, grad).bytes : LoraWs<float>(*g, nullptr, grad).bytes);
+  if (!grad) return (long long)forward_ws(*g);
+  switch (g->prec) {
+    case DPL_S: return (long long)PlainWs<float>(*g, nullptr).bytes;
+    case DPL_D: return (long long)PlainWs<double>(*g, nullptr).bytes;
+  }
+  return (long long)lora_grad_ws(*g);
 }
 
-DPL_API int dpl_lora(const LoraArgs* g, hipStream_t st) {
-  if (g->T == 0 || g->N == 0) return 0;
-  switch (g->prec) {
-    case DPL_S: return run_forward<float>(*g, st);
-    case DPL_D: return run_forward<double>(*g, st);
-    case DPL_H: return run_forward<_Float16>(*g, st);
-    case DPL_B: return run_forward<__bf16>(*g, st);
-  }
-  return -1;
-}
+DPL_API int dpl_lora(const LoraArgs* g, hipStream_t st) { return g->T == 0 || g->N == 0 ? 0 : forward(*g, st); }
 
 DPL_API int dpl_lora_grad(const LoraArgs* g, hipStream_t st) {
   switch (g->prec) {
     case DPL_S: return run_grad<float>(*g, st);
     case DPL_D: return run_grad<double>(*g, st);
-    case DPL_H: return run_grad<_Float16>(*g, st);
-    case DPL_B: return run_grad<__bf16>(*g, st);
+    case DPL_H:
+    case DPL_B: return lora_grad_half(*g, st);
   }
   return -1;
 }

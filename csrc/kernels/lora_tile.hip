@@ -1,0 +1,434 @@
+// The shared product of many tokens with the adapters' parts added to the same accumulators, and the low-rank vectors
+// that those parts start from.
+#include "lora.h"
+
+namespace {
+
+// ---------------------------------------------------------------- low-rank vectors
+// One wave per (token, j): for few tokens, where the tokens of a workgroup's rows would mostly have adapters of their own.
+template <typename T> __global__ __launch_bounds__(256) void k_low_dot(LowArgs a) {
+  typedef typename Num<T>::acc R;
+  constexpr int E = Op<T>::E;
+  const int t = blockIdx.x, j = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int l = a.ids[t];
+  if (j >= a.out.rp || (unsigned)l >= (unsigned)a.L) return;
+  R s = 0;
+  if (j < a.r) {
+    const T* f = (const T*)a.F + ((long long)l * a.r + j) * a.ldf;
+    const T* p = (const T*)a.x + (long long)t * a.ldx;
+#pragma unroll 4
+    for (int c = lane * E; c < a.C; c += 64 * E) {
+      const typename Op<T>::vec u = load_part(f + c, a.C - c), v = load_part(p + c, a.C - c);
+#pragma unroll
+      for (int i = 0; i < E; ++i) s = fma((R)u[i], (R)v[i], s);
+    }
+    for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
+    s *= a.scale ? ((const R*)a.scale)[l] : R(1);
+  }
+  if (lane == 0) {
+    LowOut o = a.out;
+    if (j >= a.r) o.thi = nullptr;
+    put_low<T>(o, t, j, s);
+  }
+}
+
+// 16 TF tokens and 16 JF rows of the factors per workgroup, the contraction split over 8 waves and joined in LDS, one
+// adapter of these tokens at a time.
+template <typename T, int JF, int TF> __global__ __launch_bounds__(512) void k_low_tile(LowArgs a) {
+  typedef typename Num<T>::acc R;
+  typedef typename Op<T>::vec V;
+  constexpr int E = Op<T>::E, KS = Op<T>::KS, U = 2;
+  __shared__ R red[8][16 * JF][16 * TF + 1];
+  __shared__ int sid[16 * TF];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, q = lane >> 4, c = lane & 15;
+  const int t0 = blockIdx.x * 16 * TF, j0 = blockIdx.y * 16 * JF;
+  int mine = -1;
+  if (lane < 16 * TF && t0 + lane < a.nt) mine = a.ids[t0 + lane];
+  if ((unsigned)mine >= (unsigned)a.L) mine = -1;
+  if (tid < 16 * TF) sid[tid] = mine;
+  const T* px[TF];
+#pragma unroll
+  for (int f = 0; f < TF; ++f) px[f] = (const T*)a.x + (long long)min(t0 + 16 * f + c, a.nt - 1) * a.ldx + q * E;
+  const int steps = (a.C + KS - 1) / KS, each = (steps + 7) / 8;
+  const int s0 = min(steps, w * each), s1 = min(steps, s0 + each), whole = min(s1, a.C / KS);
+  unsigned long long todo = __ballot(mine >= 0);
+  while (todo) {
+    const int l = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
+    todo &= ~__ballot(mine == l);
+    const T* pf[JF];
+#pragma unroll
+    for (int f = 0; f < JF; ++f)
+      pf[f] = (const T*)a.F + ((long long)l * a.r + min(j0 + 16 * f + c, a.r - 1)) * a.ldf + q * E;
+    typename Op<T>::out acc[JF][TF];
+#pragma unroll
+    for (int i = 0; i < JF; ++i)
+#pragma unroll
+      for (int f = 0; f < TF; ++f) acc[i][f] = typename Op<T>::out{R(0), R(0), R(0), R(0)};
+    int s = s0;
+    for (; s + U <= whole; s += U) {
+      V x[U][TF], f[U][JF];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int i = 0; i < TF; ++i) x[u][i] = load_vec(px[i] + (long long)(s + u) * KS);
+#pragma unroll
+        for (int i = 0; i < JF; ++i) f[u][i] = load_vec(pf[i] + (long long)(s + u) * KS);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < JF; ++i)
+#pragma unroll
+          for (int k = 0; k < TF; ++k) acc[i][k] = Op<T>::mma(f[u][i], x[u][k], acc[i][k]);
+    }
+    for (; s < s1; ++s) {
+      const int left = a.C - s * KS - q * E;
+      V x[TF];
+#pragma unroll
+      for (int k = 0; k < TF; ++k) x[k] = load_part(px[k] + (long long)s * KS, left);
+#pragma unroll
+      for (int i = 0; i < JF; ++i) {
+        const V f = load_part(pf[i] + (long long)s * KS, left);
+#pragma unroll
+        for (int k = 0; k < TF; ++k) acc[i][k] = Op<T>::mma(f, x[k], acc[i][k]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < JF; ++i)
+#pragma unroll
+      for (int k = 0; k < TF; ++k)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) red[w][16 * i + out_row<T>(lane, v)][16 * k + c] = acc[i][k][v];
+    __syncthreads();
+    const R sc = a.scale ? ((const R*)a.scale)[l] : R(1);
+    for (int p = tid; p < 256 * JF * TF; p += 512) {
+      const int j = p % (16 * JF), t = p / (16 * JF);
+      if (sid[t] != l || j0 + j >= a.out.rp) continue;
+      R v = 0;
+      if (j0 + j < a.r) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v += red[k][j][t];
+        put_low<T>(a.out, t0 + t, j0 + j, sc * v);
+      } else {
+        LowOut o = a.out;
+        o.thi = nullptr;
+        put_low<T>(o, t0 + t, j0 + j, v);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+template <typename T> int run_low(const LowArgs& a, hipStream_t st) {
+  if (a.nt <= 256) {
+    k_low_dot<T><<<dim3(a.nt, cdiv(a.out.rp, 4)), 256, 0, st>>>(a);
+    return (int)hipGetLastError();
+  }
+  const int jf = a.r <= 16 ? 1 : a.r <= 32 ? 2 : 4;
+  const int rows = max(a.r, a.out.rp);  // the zeros up to rp are written here too
+  if constexpr (sizeof(T) == 2)
+    if (a.nt >= 4096) {
+      const int tt = cdiv(a.nt, 32);
+      if (jf == 1) k_low_tile<T, 1, 2><<<dim3(tt, cdiv(rows, 16)), 512, 0, st>>>(a);
+      else if (jf == 2) k_low_tile<T, 2, 2><<<dim3(tt, cdiv(rows, 32)), 512, 0, st>>>(a);
+      else k_low_tile<T, 4, 2><<<dim3(tt, cdiv(rows, 64)), 512, 0, st>>>(a);
+      return (int)hipGetLastError();
+    }
+  const int tt = cdiv(a.nt, 16);
+  if (jf == 1) k_low_tile<T, 1, 1><<<dim3(tt, cdiv(rows, 16)), 512, 0, st>>>(a);
+  else if (jf == 2) k_low_tile<T, 2, 1><<<dim3(tt, cdiv(rows, 32)), 512, 0, st>>>(a);
+  else k_low_tile<T, 4, 1><<<dim3(tt, cdiv(rows, 64)), 512, 0, st>>>(a);
+  return (int)hipGetLastError();
+}
+
+// ---------------------------------------------------------------- shared product
+// A workgroup owns BT tokens x BN features, WT x WN waves of (BT / WT) x (BN / WN).  The contraction goes in steps of 128
+// bytes of a row through two LDS buffers: while a step is multiplied the next one is on its way.
+//   DMA: rows begin at multiples of 16 bytes and the tile's rows lie within 2^31 bytes: memory to LDS directly.
+//        A chunk past the rows' end is fetched from past the buffer descriptor's end, which reads as zero.
+//   else: through registers, 16 bytes from any address, with zeros past the rows' end.
+// LDS rows are 8 chunks of 16 bytes; chunk c of row i lies at c ^ (i & 7), so that the 16 rows that a fragment read takes
+// the same chunk of lie in different banks.  W stored with its features contiguous (NT false) is kept as it comes,
+// [step][features], and read through the transposing LDS read: a group of 16 lanes takes 4 steps x 16 features; the
+// 32-byte pair of such a read is displaced by the step's place in the instruction (16 steps of one instruction: 8 pairs).
+// The result has the tokens in its columns: a lane holds one token and 4 neighbouring features.
+template <typename T, int BT, int BN, int WT, int WN, bool NT, bool DMA>
+__global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
+  typedef typename Num<T>::acc R;
+  typedef typename Op<T>::vec V;
+  constexpr int THREADS = 64 * WT * WN, E = Op<T>::E, BK = 8 * E;
+  constexpr int FT = BT / WT / 16, FN = BN / WN / 16;
+  constexpr int JX = BT * 8 / THREADS, JW = BN * 8 / THREADS, CH = BN / E;  // CH: chunks of a [step][features] row
+  static_assert(NT || sizeof(T) == 2, "the transposing LDS read is for 16-bit elements");
+  __shared__ __attribute__((aligned(1024))) char sm[2][(BT + BN) * 128];
+  const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, c16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wt = wave / WN, wn = wave % WN;
+  // tiles of one XCD's workgroups: 8 tile rows of tokens at a time, tokens fastest, so that they share W's rows in its L2
+  const int tt = (a.T + BT - 1) / BT, tn = (a.N + BN - 1) / BN;
+  const int id = xcd_remap(blockIdx.x, tt * tn);
+  const int group = id / (8 * tn), in = id % (8 * tn), gs = min(8, tt - group * 8);
+  const int t0 = (group * 8 + in % gs) * BT, n0 = in / gs * BN;
+  const T* x = (const T*)a.x + (long long)t0 * a.ldx;
+  const T* W = (const T*)a.W + (NT ? (long long)n0 * a.ldw : n0);
+  const int rt = min(BT, a.T - t0), rn = min(BN, a.N - n0);
+
+  // staging: chunk id tid + j * THREADS of either operand
+  const int xr = tid >> 3, xc = (tid & 7) ^ (xr & 7);
+  const int wr = NT ? xr : tid / CH;
+  const int wmask = CH / 2 - 1;
+  auto turn = [&](int step) { return ((step & 3) + 4 * ((step >> 3) & 1)) & wmask; };
+  auto wchunk = [&](int row, int pc) { return 2 * ((pc >> 1) ^ turn(row)) + (pc & 1); };
+  V gx[DMA ? 1 : JX], gw[DMA ? 1 : JW];
+  unsigned ox[DMA ? JX : 1], ow[DMA ? JW : 1];
+  constexpr unsigned NOWHERE = 0x80000000u;
+  if constexpr (DMA) {
+#pragma unroll
+    for (int j = 0; j < JX; ++j) ox[j] = (unsigned)(min(xr + j * (THREADS / 8), rt - 1) * (int)a.ldx + xc * E) * sizeof(T);
+#pragma unroll
+    for (int j = 0; j < JW; ++j) {
+      if (NT) {
+        ow[j] = (unsigned)(min(wr + j * (THREADS / 8), rn - 1) * (int)a.ldw + xc * E) * sizeof(T);
+      } else {
+        const int row = wr + j * (THREADS / CH);
+        ow[j] = (unsigned)(row * (int)a.ldw + wchunk(row, tid % CH) * E) * sizeof(T);
+      }
+    }
+  }
+  const int xbytes = DMA ? (int)(((rt - 1) * a.ldx + a.C) * (long long)sizeof(T)) : 0;
+  const int wbytes = DMA && NT ? (int)(((rn - 1) * a.ldw + a.C) * (long long)sizeof(T)) : 0;
+  auto stage_dma = [&](int b, int k0) {
+    const bool in = k0 + xc * E < a.C;
+    char* sx = &sm[b][wave * 1024];
+#pragma unroll
+    for (int j = 0; j < JX; ++j) dma_buffer(x, xbytes, sx + j * THREADS * 16, in ? ox[j] : NOWHERE, k0 * (int)sizeof(T));
+    char* sw = sx + BT * 128;
+    if (NT) {
+#pragma unroll
+      for (int j = 0; j < JW; ++j) dma_buffer(W, wbytes, sw + j * THREADS * 16, in ? ow[j] : NOWHERE, k0 * (int)sizeof(T));
+    } else {
+      // the descriptor ends with W's last row: steps past it read as zero
+      const int rows = min(BK, a.C - k0), bytes = (int)(((rows - 1) * a.ldw + rn) * (long long)sizeof(T));
+#pragma unroll
+      for (int j = 0; j < JW; ++j) dma_buffer(W + (long long)k0 * a.ldw, bytes, sw + j * THREADS * 16, ow[j], 0);
+    }
+  };
+  auto fetch = [&](int k0) {
+    const int left = a.C - k0 - xc * E;
+#pragma unroll
+    for (int j = 0; j < JX; ++j) gx[j] = load_part(x + (long long)min(xr + j * (THREADS / 8), rt - 1) * a.ldx + k0 + xc * E, left);
+#pragma unroll
+    for (int j = 0; j < JW; ++j) {
+      if (NT) {
+        gw[j] = load_part(W + (long long)min(wr + j * (THREADS / 8), rn - 1) * a.ldw + k0 + xc * E, left);
+      } else {
+        const int row = wr + j * (THREADS / CH), n = wchunk(row, tid % CH) * E;
+        gw[j] = load_part(W + (long long)(k0 + row) * a.ldw + n, k0 + row < a.C ? rn - n : 0);
+      }
+    }
+  };
+  auto put = [&](int b) {
+#pragma unroll
+    for (int j = 0; j < JX; ++j) *(V*)&sm[b][(tid + j * THREADS) * 16] = gx[j];
+#pragma unroll
+    for (int j = 0; j < JW; ++j) *(V*)&sm[b][BT * 128 + (tid + j * THREADS) * 16] = gw[j];
+  };
+
+  typename Op<T>::out acc[FN][FT];
+#pragma unroll
+  for (int i = 0; i < FN; ++i)
+#pragma unroll
+    for (int f = 0; f < FT; ++f) acc[i][f] = typename Op<T>::out{R(0), R(0), R(0), R(0)};
+  const int fx = (wt * FT * 16 + c16) * 128 + ((q ^ (c16 & 7)) << 4);              // ^ 64: the second half of the step
+  const int fw = BT * 128 + (wn * FN * 16 + c16) * 128 + ((q ^ (c16 & 7)) << 4);
+  const int ftr = BT * 128 + (8 * q + (c16 >> 2)) * (BN * 2) + (c16 & 3) * 8;      // + pair * 32
+  const int tw = ((c16 >> 2) + 4 * (q & 1)) & wmask;
+  auto multiply = [&](int b) {
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      V vx[FT], vw[FN];
+#pragma unroll
+      for (int i = 0; i < FN; ++i) {
+        if constexpr (NT) {
+          vw[i] = *(const V*)&sm[b][(fw ^ (kk * 64)) + i * 2048];
+        } else {
+          typedef short s4_t __attribute__((ext_vector_type(4)));
+          const char* p = &sm[b][ftr + (((wn * FN + i) ^ tw) << 5) + kk * 32 * BN * 2];
+          typedef __attribute__((address_space(3))) s4_t* lp;
+          const s4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p));
+          const s4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p + 4 * BN * 2));
+          typedef short s8_t __attribute__((ext_vector_type(8)));
+          const s8_t both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+          vw[i] = __builtin_bit_cast(V, both);
+        }
+      }
+#pragma unroll
+      for (int f = 0; f < FT; ++f) vx[f] = *(const V*)&sm[b][(fx ^ (kk * 64)) + f * 2048];
+#pragma unroll
+      for (int f = 0; f < FT; ++f)
+#pragma unroll
+        for (int i = 0; i < FN; ++i) acc[i][f] = Op<T>::mma(vw[i], vx[f], acc[i][f]);
+    }
+  };
+  // everything asked for has arrived and every wave is past its reads of the buffer that is filled next
+  auto meet = [&]() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  const int steps = (a.C + BK - 1) / BK;
+  if constexpr (DMA) {
+    if (steps > 0) stage_dma(0, 0);
+    for (int s = 0; s < steps; ++s) {
+      meet();
+      if (s + 1 < steps) stage_dma((s + 1) & 1, (s + 1) * BK);
+      multiply(s & 1);
+    }
+  } else {
+    if (steps > 0) fetch(0);
+    for (int s = 0; s < steps; ++s) {
+      put(s & 1);
+      __syncthreads();
+      if (s + 1 < steps) fetch((s + 1) * BK);
+      multiply(s & 1);
+    }
+  }
+
+  // the adapters' parts: one adapter of this wave's tokens at a time, fragments straight from memory (r is short).  The
+  // product is formed apart and added by a select: what it holds for tokens of other adapters may be anything.
+  int lid[FT];
+#pragma unroll
+  for (int f = 0; f < FT; ++f) {
+    const int t = t0 + (wt * FT + f) * 16 + c16;
+    int l = a.L > 0 && t < a.T ? a.ids[t] : -1;
+    if ((unsigned)l >= (unsigned)a.L) l = -1;
+    lid[f] = l;
+  }
+  typedef typename Mid<T>::elem M;
+  typedef typename Op<M>::vec MV;
+  constexpr int NONE = 0x7fffffff;
+  auto after = [&](int l) {  // the next larger adapter of this wave's tokens
+    int next = NONE;
+#pragma unroll
+    for (int f = 0; f < FT; ++f) next = lid[f] > l ? min(next, lid[f]) : next;
+#pragma unroll
+    for (int o = 8; o; o >>= 1) next = min(next, __shfl_xor(next, o));
+    return __builtin_amdgcn_readfirstlane(next);
+  };
+  // (one loop over adapters and steps of r together: two nested ones cost a second copy of the accumulators)
+  int l = after(-1), j0 = 0;
+  while (l != NONE) {
+    {
+      const int j = j0 + q * E;
+      MidOp<T> F[FN];
+#pragma unroll
+      for (int i = 0; i < FN; ++i) {
+        const int n = min(n0 + (wn * FN + i) * 16 + c16, a.N - 1);
+        F[i].set(load_part((const T*)a.F + ((long long)l * a.N + n) * a.ldf + j, a.r - j));
+      }
+#pragma unroll
+      for (int f = 0; f < FT; ++f) {
+        const unsigned long long m = __ballot(lid[f] == l);
+        __builtin_amdgcn_sched_barrier(0);
+        if (m == 0) continue;
+        const long long at = (long long)min(t0 + (wt * FT + f) * 16 + c16, a.T - 1) * a.rp + j;
+        const MV hi = load_vec((const M*)a.hi + at), lo = Mid<T>::PARTS == 2 ? load_vec((const M*)a.lo + at) : hi;
+#pragma unroll
+        for (int i = 0; i < FN; ++i) {
+          const typename Op<T>::out d = F[i].mma(hi, lo, typename Op<T>::out{R(0), R(0), R(0), R(0)});
+          const typename Op<T>::out none = {R(0), R(0), R(0), R(0)};
+          acc[i][f] += lid[f] == l ? d : none;
+        }
+      }
+    }
+    j0 += Op<T>::KS;
+    if (j0 >= a.r) {
+      l = after(l);
+      j0 = 0;
+    }
+  }
+
+  const R alpha = (R)a.alpha, beta = (R)a.beta;
+#pragma unroll
+  for (int f = 0; f < FT; ++f) {
+    const int t = t0 + (wt * FT + f) * 16 + c16;
+    __builtin_amdgcn_sched_barrier(0);  // one column of fragments at a time: their addresses together would spill
+    if (t >= a.T) continue;
+    T* row = (T*)a.y + (long long)t * a.ldy;
+#pragma unroll
+    for (int i = 0; i < FN; ++i) {
+      const int nb = n0 + (wn * FN + i) * 16;
+      typedef T T4 __attribute__((ext_vector_type(4)));
+      if (sizeof(T) != 8 && nb + 4 * q + 4 <= a.N) {
+        T* p = row + nb + 4 * q;
+        T4 o;
+        if (beta != R(0)) __builtin_memcpy(&o, p, sizeof(o));
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          R u = alpha == R(0) ? R(0) : alpha * acc[i][f][v];
+          if (beta != R(0)) u += beta * (R)o[v];
+          o[v] = (T)u;
+        }
+        __builtin_memcpy(p, &o, sizeof(o));
+      } else {
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const int n = nb + out_row<T>(lane, v);
+          if (n >= a.N) continue;
+          R u = alpha == R(0) ? R(0) : alpha * acc[i][f][v];
+          if (beta != R(0)) u += beta * widen(row[n]);
+          row[n] = (T)u;
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int BT, int BN, int WT, int WN, bool NT, bool DMA> void launch(const TileArgs& a, hipStream_t st) {
+  k_tile<T, BT, BN, WT, WN, NT, DMA><<<cdiv(a.T, BT) * cdiv(a.N, BN), 64 * WT * WN, 0, st>>>(a);
+}
+
+template <typename T, bool NT> int run_tile(const TileArgs& a, hipStream_t st) {
+  const long long size = sizeof(T), span = 1ll << 30;
+  auto wide = [&](const void* p, long long ld, int rows) {
+    return ((uintptr_t)p | (uintptr_t)(ld * size)) % 16 == 0 && ld * size * rows < span;
+  };
+  // W with its features contiguous also needs whole chunks of them within a row
+  const bool dma = wide(a.x, a.ldx, 256) && wide(a.W, a.ldw, 256) && a.C % Op<T>::E == 0 && (NT || a.N % 8 == 0);
+  auto tiles = [&](int b) { return (long long)cdiv(a.T, b) * cdiv(a.N, b); };
+  if constexpr (sizeof(T) == 2)
+    if (dma && tiles(256) >= 160) {
+      launch<T, 256, 256, 2, 4, NT, true>(a, st);
+      return (int)hipGetLastError();
+    }
+  if (tiles(128) >= 160 || sizeof(T) == 8) {
+    if (dma) launch<T, 128, 128, 2, 2, NT, true>(a, st);
+    else launch<T, 128, 128, 2, 2, NT, false>(a, st);
+  } else {
+    if (dma) launch<T, 64, 64, 2, 2, NT, true>(a, st);
+    else launch<T, 64, 64, 2, 2, NT, false>(a, st);
+  }
+  return (int)hipGetLastError();
+}
+
+}  // namespace
+
+int lora_low(const LowArgs& a, hipStream_t st) {
+  switch (a.prec) {
+    case DPL_S: return run_low<float>(a, st);
+    case DPL_D: return run_low<double>(a, st);
+    case DPL_H: return run_low<_Float16>(a, st);
+    case DPL_B: return run_low<__bf16>(a, st);
+  }
+  return -1;
+}
+
+int lora_tile(const TileArgs& a, bool nt, hipStream_t st) {
+  switch (a.prec) {
+    case DPL_S: return nt ? run_tile<float, true>(a, st) : -1;
+    case DPL_D: return nt ? run_tile<double, true>(a, st) : -1;
+    case DPL_H: return nt ? run_tile<_Float16, true>(a, st) : run_tile<_Float16, false>(a, st);
+    case DPL_B: return nt ? run_tile<__bf16, true>(a, st) : run_tile<__bf16, false>(a, st);
+  }
+  return -1;
+}
