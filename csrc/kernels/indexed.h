@@ -140,9 +140,14 @@ template <typename T> struct MidOp {
 template <> struct MidOp<_Float16> {
   typedef b8_t vec;
   vec f, g;
+  // 11 bits: the upper 8 by truncation, the rest exactly in the second number (none beside an infinity)
   __device__ inline void set(h8_t v) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) Mid<_Float16>::put((__bf16*)&f + i, (__bf16*)&g + i, (float)v[i]);
+    for (int i = 0; i < 8; ++i) {
+      const float x = (float)v[i], h = __uint_as_float(__float_as_uint(x) & 0xffff0000u), rest = x - h;
+      f[i] = (__bf16)h;
+      g[i] = (__bf16)(rest == rest ? rest : 0.f);
+    }
   }
   __device__ inline f4_t mma(vec hi, vec lo, f4_t c) const {
     c = Op<__bf16>::mma(f, hi, c);

@@ -27,7 +27,7 @@ from ..constants import DTYPE_PREC, STORAGE_LAPACK
 from ..ops import indexed_ops as ops
 from ..runtime import Taskpool
 
-_LIMIT = 4194240      # tokens: 65535 tiles of 64 along one grid axis
+_LIMIT = 4194240      # tokens or features: 65535 tiles of 64 along one grid axis
 _FAMILY = 65535       # adapters: one grid axis
 
 
@@ -121,9 +121,9 @@ def _lora_checks(op, ctx, W, X, A, B, ids, scale, N, outputs, others):
     if N and _family(op, "B", B, N) != L:
         raise ValueError(f"{op}: A holds {L} adapters, B {B.n // N}")
     _matrix(op, ctx, "B", B, r, L * N, dtype)
-    if T > _LIMIT or L > _FAMILY:
-        raise ValueError(f"{op}: at most {_LIMIT} tokens and {_FAMILY} adapters, got {T} and {L}")
-    _extent(op, K=K, N=N, **{"L r": L * r})
+    if max(T, K, N, r) > _LIMIT or L > _FAMILY:
+        raise ValueError(f"{op}: at most {_LIMIT} tokens or features and {_FAMILY} adapters, got T = {T}, K = {K}, "
+                         f"N = {N}, r = {r}, L = {L}")
     _vector(op, ctx, "ids", ids, T, torch.int32)
     if scale is not None:
         _vector(op, ctx, "scale", scale, L, torch.float64 if dtype is torch.float64 else torch.float32)
@@ -210,15 +210,15 @@ def moe_New(ctx, topk, norm, G, W1, W2, alpha, X, beta, Y) -> Taskpool:
     most = 4096  # a token's logits stay in LDS
     if not 1 <= E <= most:
         raise ValueError(f"{op}: 1 to {most} experts, got {E}")
-    if not 1 <= topk <= E or int(topk) != topk:
-        raise ValueError(f"{op}: topk = {topk} of {E} experts")
+    if not 1 <= topk <= min(E, 256) or int(topk) != topk:
+        raise ValueError(f"{op}: topk = {topk} of {E} experts (at most 256)")
     if H and (_family(op, "W2", W2, H) != E or width and _family(op, "W1", W1, 2 * width) != E):
         raise ValueError(f"{op}: G has {E} experts, W1 {W1.n} columns and W2 {W2.n}")
     _matrix(op, ctx, "W1", W1, H, E * 2 * width, dtype)
     _matrix(op, ctx, "W2", W2, width, E * H, dtype)
     if T > 65535:
         raise ValueError(f"{op}: at most 65535 tokens, got {T}")
-    _extent(op, **{"T topk I": T * topk * width, "T topk H": T * topk * H, "2 I": 2 * width})
+    _extent(op, H=H, I=2 * width, E=E * 2 * width)
     _disjoint(op, [("Y", Y)], [("G", G), ("W1", W1), ("W2", W2), ("X", X)])
     return _pool(ctx, op, lambda: ops.moe_call(ctx.device, int(topk), bool(norm), G, W1, W2, float(alpha), X,
                                                float(beta), Y),

@@ -42,10 +42,12 @@ def pointer(M):
 class _Call:
     """A kernel call with its argument record and workspace; ``__call__`` enqueues it on the current stream."""
 
-    def __init__(self, device, name, args, ws_bytes, keep):
+    def __init__(self, device, name, args, ws_bytes, keep, zero=0):
+        """zero: bytes at the workspace's beginning that start as zeros (every run leaves them so)."""
         self.name, self.args, self.device = name, args, device
         self.keep = keep  # tensors whose addresses the record holds
         self.ws = torch.empty(max(256, ws_bytes), dtype=torch.uint8, device=device)
+        self.ws[:zero].zero_()
         self.home = torch.cuda.current_stream(device).cuda_stream
         if not torch.cuda.is_current_stream_capturing():
             # the allocator may have handed out memory that work queued on this stream still uses; the taskpool may
@@ -89,7 +91,7 @@ def moe_call(device, topk, norm, G, W1, W2, alpha, X, beta, Y):
     a = MoeArgs(G=pointer(G), W1=pointer(W1), W2=pointer(W2), X=pointer(X), Y=pointer(Y), ldg=G.ld, ld1=W1.ld,
                 ld2=W2.ld, ldx=X.ld, ldy=Y.ld, alpha=alpha, beta=beta, prec=CODE[X.dtype], T=X.n, H=X.m, I=W2.m,
                 E=G.n, topk=topk, norm=int(norm))
-    return _Call(device, "dpl_moe", a, lib.dpl_moe_ws_bytes(ctypes.byref(a)), [G, W1, W2, X, Y])
+    return _Call(device, "dpl_moe", a, lib.dpl_moe_ws_bytes(ctypes.byref(a)), [G, W1, W2, X, Y], 4 * X.n)
 
 
 # ----------------------------------------------------------------------------- CPU path
