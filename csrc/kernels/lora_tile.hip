@@ -143,12 +143,15 @@ template <typename T> int run_low(const LowArgs& a, hipStream_t st) {
 
 // ---------------------------------------------------------------- shared product
 // A workgroup owns BT tokens x BN features, WT x WN waves of (BT / WT) x (BN / WN).  The contraction goes in steps of 128
-// bytes of a row through two LDS buffers: while a step is multiplied the next one is on its way.
-//   DMA: rows begin at multiples of 16 bytes and the tile's rows lie within 2^31 bytes: memory to LDS directly.
+// bytes of a row (whole cache lines: with 64-byte steps the same lines were asked for twice, 1.12 against 1.13 PFLOP/s at
+// 16384 x 4096 x 16384, and 1.26 against 1.38 where all of it lies in the L2) through two LDS buffers, each step in two halves of one fragment.  While a half is multiplied
+// from registers the fragments of the next one are read from LDS; when a step's second half is in registers its buffer
+// takes the step after next.  So neither latency is waited for, and a step has one barrier.
+//   DMA: rows begin at multiples of 16 bytes and the tile's rows lie within 2^30 bytes: memory to LDS directly.
 //        A chunk past the rows' end is fetched from past the buffer descriptor's end, which reads as zero.
 //   else: through registers, 16 bytes from any address, with zeros past the rows' end.
-// LDS rows are 8 chunks of 16 bytes; chunk c of row i lies at c ^ (i & 7), so that the 16 rows that a fragment read takes
-// the same chunk of lie in different banks.  W stored with its features contiguous (NT false) is kept as it comes,
+// LDS rows are 8 chunks of 16 bytes; chunk c of row i lies at c ^ (i & 7), so that the rows that a fragment read takes
+// the same chunk of lie in different banks (no conflicts by the counter).  W stored with its features contiguous (NT false) is kept as it comes,
 // [step][features], and read through the transposing LDS read: a group of 16 lanes takes 4 steps x 16 features; the
 // 32-byte pair of such a read is displaced by the step's place in the instruction (16 steps of one instruction: 8 pairs).
 // The result has the tokens in its columns: a lane holds one token and 4 neighbouring features.
@@ -156,18 +159,19 @@ template <typename T, int BT, int BN, int WT, int WN, bool NT, bool DMA>
 __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
   typedef typename Num<T>::acc R;
   typedef typename Op<T>::vec V;
-  constexpr int THREADS = 64 * WT * WN, E = Op<T>::E, BK = 8 * E;
+  constexpr int THREADS = 64 * WT * WN, E = Op<T>::E, BK = 2 * Op<T>::KS, STAGE = (BT + BN) * 128;
   constexpr int FT = BT / WT / 16, FN = BN / WN / 16;
   constexpr int JX = BT * 8 / THREADS, JW = BN * 8 / THREADS, CH = BN / E;  // CH: chunks of a [step][features] row
   static_assert(NT || sizeof(T) == 2, "the transposing LDS read is for 16-bit elements");
-  __shared__ __attribute__((aligned(1024))) char sm[2][(BT + BN) * 128];
+  __shared__ __attribute__((aligned(1024))) char sm[2 * STAGE];
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, c16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wt = wave / WN, wn = wave % WN;
-  // tiles of one XCD's workgroups: 8 tile rows of tokens at a time, tokens fastest, so that they share W's rows in its L2
+  // tiles of one XCD's workgroups: 4 tile rows of tokens at a time, tokens fastest, so that they share rows in its L2
+  // (4 / 8 / 16 rows: 1.12 / 1.03 / 1.04 PFLOP/s at 16384 x 4096 x 16384)
   const int tt = (a.T + BT - 1) / BT, tn = (a.N + BN - 1) / BN;
   const int id = xcd_remap(blockIdx.x, tt * tn);
-  const int group = id / (8 * tn), in = id % (8 * tn), gs = min(8, tt - group * 8);
-  const int t0 = (group * 8 + in % gs) * BT, n0 = in / gs * BN;
+  const int group = id / (4 * tn), in = id % (4 * tn), gs = min(4, tt - group * 4);
+  const int t0 = (group * 4 + in % gs) * BT, n0 = in / gs * BN;
   const T* x = (const T*)a.x + (long long)t0 * a.ldx;
   const T* W = (const T*)a.W + (NT ? (long long)n0 * a.ldw : n0);
   const int rt = min(BT, a.T - t0), rn = min(BN, a.N - n0);
@@ -196,9 +200,15 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
   }
   const int xbytes = DMA ? (int)(((rt - 1) * a.ldx + a.C) * (long long)sizeof(T)) : 0;
   const int wbytes = DMA && NT ? (int)(((rn - 1) * a.ldw + a.C) * (long long)sizeof(T)) : 0;
-  auto stage_dma = [&](int b, int k0) {
+  const int steps = (a.C + BK - 1) / BK;
+  // each XCD begins at another eighth of the contraction: beginning together they all ask for the same rows of W at
+  // once (1.13 -> 1.20 PFLOP/s at 16384 x 4096 x 16384, 1.26 -> 1.35 at 8192^3)
+  const int turned = steps / 8 * (blockIdx.x & 7);
+  auto place = [&](int s) { return (s >= steps ? s : s + turned >= steps ? s + turned - steps : s + turned) * BK; };
+  auto stage_dma = [&](int s) {  // steps past the last one read as zero too
+    const int k0 = place(s);
     const bool in = k0 + xc * E < a.C;
-    char* sx = &sm[b][wave * 1024];
+    char* sx = &sm[(s & 1) * STAGE + wave * 1024];
 #pragma unroll
     for (int j = 0; j < JX; ++j) dma_buffer(x, xbytes, sx + j * THREADS * 16, in ? ox[j] : NOWHERE, k0 * (int)sizeof(T));
     char* sw = sx + BT * 128;
@@ -206,14 +216,15 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
 #pragma unroll
       for (int j = 0; j < JW; ++j) dma_buffer(W, wbytes, sw + j * THREADS * 16, in ? ow[j] : NOWHERE, k0 * (int)sizeof(T));
     } else {
-      // the descriptor ends with W's last row: steps past it read as zero
-      const int rows = min(BK, a.C - k0), bytes = (int)(((rows - 1) * a.ldw + rn) * (long long)sizeof(T));
+      // the descriptor ends with W's last row
+      const int pitch = (int)a.ldw * (int)sizeof(T);
+      const int bytes = __builtin_amdgcn_readfirstlane(max(0, max(0, min(BK, a.C - k0)) * pitch - (pitch - rn * (int)sizeof(T))));
 #pragma unroll
       for (int j = 0; j < JW; ++j) dma_buffer(W + (long long)k0 * a.ldw, bytes, sw + j * THREADS * 16, ow[j], 0);
     }
   };
-  auto fetch = [&](int k0) {
-    const int left = a.C - k0 - xc * E;
+  auto fetch = [&](int s) {
+    const int k0 = place(s), left = a.C - k0 - xc * E;
 #pragma unroll
     for (int j = 0; j < JX; ++j) gx[j] = load_part(x + (long long)min(xr + j * (THREADS / 8), rt - 1) * a.ldx + k0 + xc * E, left);
 #pragma unroll
@@ -226,11 +237,12 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
       }
     }
   };
-  auto put = [&](int b) {
+  auto put = [&](int s) {
+    char* b = &sm[(s & 1) * STAGE + tid * 16];
 #pragma unroll
-    for (int j = 0; j < JX; ++j) *(V*)&sm[b][(tid + j * THREADS) * 16] = gx[j];
+    for (int j = 0; j < JX; ++j) *(V*)(b + j * THREADS * 16) = gx[j];
 #pragma unroll
-    for (int j = 0; j < JW; ++j) *(V*)&sm[b][BT * 128 + (tid + j * THREADS) * 16] = gw[j];
+    for (int j = 0; j < JW; ++j) *(V*)(b + BT * 128 + j * THREADS * 16) = gw[j];
   };
 
   typename Op<T>::out acc[FN][FT];
@@ -238,60 +250,99 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
   for (int i = 0; i < FN; ++i)
 #pragma unroll
     for (int f = 0; f < FT; ++f) acc[i][f] = typename Op<T>::out{R(0), R(0), R(0), R(0)};
-  const int fx = (wt * FT * 16 + c16) * 128 + ((q ^ (c16 & 7)) << 4);              // ^ 64: the second half of the step
+  const int fx = (wt * FT * 16 + c16) * 128 + ((q ^ (c16 & 7)) << 4);  // ^ 64: the second half of the step
   const int fw = BT * 128 + (wn * FN * 16 + c16) * 128 + ((q ^ (c16 & 7)) << 4);
-  const int ftr = BT * 128 + (8 * q + (c16 >> 2)) * (BN * 2) + (c16 & 3) * 8;      // + pair * 32
+  const int ftr = BT * 128 + (8 * q + (c16 >> 2)) * (BN * 2) + (c16 & 3) * 8;  // + pair * 32
   const int tw = ((c16 >> 2) + 4 * (q & 1)) & wmask;
-  auto multiply = [&](int b) {
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      V vx[FT], vw[FN];
-#pragma unroll
-      for (int i = 0; i < FN; ++i) {
-        if constexpr (NT) {
-          vw[i] = *(const V*)&sm[b][(fw ^ (kk * 64)) + i * 2048];
-        } else {
-          typedef short s4_t __attribute__((ext_vector_type(4)));
-          const char* p = &sm[b][ftr + (((wn * FN + i) ^ tw) << 5) + kk * 32 * BN * 2];
-          typedef __attribute__((address_space(3))) s4_t* lp;
-          const s4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p));
-          const s4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p + 4 * BN * 2));
-          typedef short s8_t __attribute__((ext_vector_type(8)));
-          const s8_t both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-          vw[i] = __builtin_bit_cast(V, both);
-        }
-      }
-#pragma unroll
-      for (int f = 0; f < FT; ++f) vx[f] = *(const V*)&sm[b][(fx ^ (kk * 64)) + f * 2048];
-#pragma unroll
-      for (int f = 0; f < FT; ++f)
-#pragma unroll
-        for (int i = 0; i < FN; ++i) acc[i][f] = Op<T>::mma(vw[i], vx[f], acc[i][f]);
-    }
+  struct Frag {
+    V x[FT], w[FN];
   };
-  // everything asked for has arrived and every wave is past its reads of the buffer that is filled next
+  auto read = [&](Frag& r, int s, int half) {
+    const char* b = &sm[(s & 1) * STAGE];
+#pragma unroll
+    for (int i = 0; i < FN; ++i) {
+      if constexpr (NT) {
+        r.w[i] = *(const V*)(b + (fw ^ (64 * half)) + i * 2048);
+      } else {
+        typedef short s4_t __attribute__((ext_vector_type(4)));
+        typedef short s8_t __attribute__((ext_vector_type(8)));
+        typedef __attribute__((address_space(3))) s4_t* lp;
+        const char* p = b + ftr + (((wn * FN + i) ^ tw) << 5) + half * 32 * BN * 2;
+        const s4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p));
+        const s4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p + 4 * BN * 2));
+        const s8_t both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        r.w[i] = __builtin_bit_cast(V, both);
+      }
+    }
+#pragma unroll
+    for (int f = 0; f < FT; ++f) r.x[f] = *(const V*)(b + (fx ^ (64 * half)) + f * 2048);
+  };
+  auto multiply = [&](const Frag& r) {
+#pragma unroll
+    for (int f = 0; f < FT; ++f)
+#pragma unroll
+      for (int i = 0; i < FN; ++i) acc[i][f] = Op<T>::mma(r.w[i], r.x[f], acc[i][f]);
+  };
   auto meet = [&]() {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
-  const int steps = (a.C + BK - 1) / BK;
-  if constexpr (DMA) {
-    if (steps > 0) stage_dma(0, 0);
+  constexpr int LOADS = JX + JW, READS = FT + (NT ? FN : 2 * FN), PRODUCTS = FT * FN, EARLY = READS / 2;
+  auto pace = [&](int loads) {
+    // the reads early among the products, then the loads: left alone, the compiler puts the reads where the next half
+    // waits for them
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int k = 0; k < EARLY; ++k) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS / 2 / EARLY, 0);
+      }
+      if (loads) {
+#pragma unroll
+        for (int k = 0; k < LOADS; ++k) {
+          __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS / 2 / LOADS, 0);
+        }
+      }
+    }
+  };
+  if (steps > 0) {
+    Frag one, two;
+    if constexpr (DMA) {
+      stage_dma(0);
+      stage_dma(1);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
+    } else {
+      fetch(0);
+      put(0);
+      fetch(1);
+      put(1);
+      fetch(2);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    meet();
+    read(one, 0, 0);
     for (int s = 0; s < steps; ++s) {
+      read(two, s, 1);
+      multiply(one);
+      pace(0);
+      // step s + 1 has arrived, and this step is in registers: its buffer is free
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       meet();
-      if (s + 1 < steps) stage_dma((s + 1) & 1, (s + 1) * BK);
-      multiply(s & 1);
+      read(one, s + 1, 0);
+      if constexpr (DMA) {
+        stage_dma(s + 2);
+      } else {
+        put(s + 2);
+        fetch(s + 3);
+      }
+      multiply(two);
+      pace(1);
     }
-  } else {
-    if (steps > 0) fetch(0);
-    for (int s = 0; s < steps; ++s) {
-      put(s & 1);
-      __syncthreads();
-      if (s + 1 < steps) fetch((s + 1) * BK);
-      multiply(s & 1);
-    }
+    // nothing is on its way to LDS when the workgroup ends
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   }
 
   // the adapters' parts: one adapter of this wave's tokens at a time, fragments straight from memory (r is short).  The
@@ -348,37 +399,49 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
     }
   }
 
+  // Out through LDS, 16 tokens of a wave at a time, so that memory gets whole rows of the wave's features (from the
+  // accumulators a store would write 32 bytes of each of 16 rows)
   const R alpha = (R)a.alpha, beta = (R)a.beta;
+  constexpr int ROW = FN * 16, PITCH = ROW + 16 / sizeof(R), OW = 16 / sizeof(T), LANES = ROW / OW;  // lanes of a row
+  static_assert(WT * WN * 16 * PITCH * sizeof(R) <= 2 * STAGE && 64 % LANES == 0, "staging");
+  __syncthreads();
+  R* mine = (R*)sm + wave * 16 * PITCH;
+  const int col = lane % LANES * OW, n = n0 + wn * ROW + col;
 #pragma unroll
   for (int f = 0; f < FT; ++f) {
-    const int t = t0 + (wt * FT + f) * 16 + c16;
-    __builtin_amdgcn_sched_barrier(0);  // one column of fragments at a time: their addresses together would spill
-    if (t >= a.T) continue;
-    T* row = (T*)a.y + (long long)t * a.ldy;
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int i = 0; i < FN; ++i) {
-      const int nb = n0 + (wn * FN + i) * 16;
-      typedef T T4 __attribute__((ext_vector_type(4)));
-      if (sizeof(T) != 8 && nb + 4 * q + 4 <= a.N) {
-        T* p = row + nb + 4 * q;
-        T4 o;
-        if (beta != R(0)) __builtin_memcpy(&o, p, sizeof(o));
+      if constexpr (sizeof(T) == 8) {
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          R u = alpha == R(0) ? R(0) : alpha * acc[i][f][v];
-          if (beta != R(0)) u += beta * (R)o[v];
-          o[v] = (T)u;
+        for (int v = 0; v < 4; ++v) mine[c16 * PITCH + i * 16 + out_row<T>(lane, v)] = acc[i][f][v];
+      } else {
+        *(typename Op<T>::out*)&mine[c16 * PITCH + i * 16 + 4 * q] = acc[i][f];
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int r0 = 0; r0 < 16; r0 += 64 / LANES) {
+      const int r = r0 + lane / LANES, t = t0 + (wt * FT + f) * 16 + r;
+      if (r >= 16 || t >= a.T || n >= a.N) continue;
+      T* p = (T*)a.y + (long long)t * a.ldy + n;
+      R u[OW];
+#pragma unroll
+      for (int v = 0; v < OW; ++v) u[v] = alpha == R(0) ? R(0) : alpha * mine[r * PITCH + col + v];
+      if (n + OW <= a.N) {
+        V o;
+        if (beta != R(0)) {
+          o = load_vec(p);
+#pragma unroll
+          for (int v = 0; v < OW; ++v) u[v] += beta * (R)o[v];
         }
-        __builtin_memcpy(p, &o, sizeof(o));
+#pragma unroll
+        for (int v = 0; v < OW; ++v) o[v] = (T)u[v];
+        __builtin_memcpy(p, &o, 16);
       } else {
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const int n = nb + out_row<T>(lane, v);
-          if (n >= a.N) continue;
-          R u = alpha == R(0) ? R(0) : alpha * acc[i][f][v];
-          if (beta != R(0)) u += beta * widen(row[n]);
-          row[n] = (T)u;
-        }
+        for (int v = 0; v < OW; ++v)
+          if (n + v < a.N) p[v] = (T)(beta != R(0) ? u[v] + beta * widen(p[v]) : u[v]);
       }
     }
   }
