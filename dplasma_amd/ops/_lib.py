@@ -140,7 +140,7 @@ _SIGS = {
     "dpl_lora_ws_bytes": [c_vp, c_int],
     "dpl_lora_args_bytes": [],
     "dpl_moe": [c_vp, c_vp],
-    "dpl_moe_ws_bytes": [c_vp],
+    "dpl_moe_ws_bytes": [c_vp, c_vp],
     "dpl_moe_args_bytes": [],
 }
 _OPTIONAL = set()

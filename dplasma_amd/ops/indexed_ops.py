@@ -91,7 +91,9 @@ def moe_call(device, topk, norm, G, W1, W2, alpha, X, beta, Y):
     a = MoeArgs(G=pointer(G), W1=pointer(W1), W2=pointer(W2), X=pointer(X), Y=pointer(Y), ldg=G.ld, ld1=W1.ld,
                 ld2=W2.ld, ldx=X.ld, ldy=Y.ld, alpha=alpha, beta=beta, prec=CODE[X.dtype], T=X.n, H=X.m, I=W2.m,
                 E=G.n, topk=topk, norm=int(norm))
-    return _Call(device, "dpl_moe", a, lib.dpl_moe_ws_bytes(ctypes.byref(a)), [G, W1, W2, X, Y], 4 * X.n)
+    zero = _ll()
+    size = lib.dpl_moe_ws_bytes(ctypes.byref(a), ctypes.byref(zero))
+    return _Call(device, "dpl_moe", a, size, [G, W1, W2, X, Y], zero.value)
 
 
 # ----------------------------------------------------------------------------- CPU path
