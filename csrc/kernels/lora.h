@@ -47,6 +47,12 @@ template <typename T> __device__ inline void put_low(const LowOut& o, int t, int
     if (Mid<T>::PARTS == 2) ((M*)o.tlo)[at] = l;
   }
 }
+template <typename T> __device__ inline void pad_low(const LowOut& o, int t, int j) {
+  typedef typename Mid<T>::elem M;
+  if (!o.hi) return;
+  ((M*)o.hi)[(long long)t * o.rp + j] = (M)0;
+  if (Mid<T>::PARTS == 2) ((M*)o.lo)[(long long)t * o.rp + j] = (M)0;
+}
 
 static inline int low_pitch(int prec, int r) {
   const int ks = prec == DPL_D ? 8 : prec == DPL_S ? 16 : 32;
@@ -54,15 +60,24 @@ static inline int low_pitch(int prec, int r) {
 }
 static inline size_t mid_bytes(int prec) { return prec == DPL_D ? 8 : prec == DPL_S ? 4 : 2; }
 
-// out(t, j) = s_l sum_c x[t*ldx + c] F[(l*r + j)*ldf + c],  l = ids[t]
+// out(t, j) = s_l sum_c x[t*ldx + c] F[(l*r + j)*ldf + c],  l = ids[t], for one or two sets of the same tokens.
+// share: splits * nt * r numbers of the working precision; arrived: tiles * blocks ints that are zero before the first
+// run and left so by every run (each set its own).
 struct LowArgs {
   const void *x, *F, *scale;
   const int* ids;
   long long ldx, ldf;
   int prec, nt, C, r, L;
   LowOut out;
+  void* share;
+  int* arrived;
 };
-int lora_low(const LowArgs& a, hipStream_t st);
+constexpr int LOW_SPLITS = 8;
+struct LowPlan {
+  int jf, tf, tiles, blocks, splits;  // tf 0: one wave per token and j
+};
+LowPlan low_plan(size_t size, int nt, int r, int sets);
+int lora_low(const LowArgs* sets, int n, hipStream_t st);
 
 // y[t*ldy + n] = alpha (sum_c x[t*ldx + c] W(n, c) + sum_j low(t, j) F[(l*N + n)*ldf + j]) + beta y[t*ldy + n];
 // nt: W(n, c) = W[n*ldw + c], else W[c*ldw + n] (h and b only)
@@ -77,5 +92,5 @@ struct TileArgs {
 int lora_tile(const TileArgs& a, bool nt, hipStream_t st);
 
 // Gradient in h and b (lora_grad.hip).
-size_t lora_grad_ws(const LoraArgs& g);
+size_t lora_grad_ws(const LoraArgs& g, size_t* zero);
 int lora_grad_half(const LoraArgs& g, hipStream_t st);

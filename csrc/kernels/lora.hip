@@ -213,34 +213,56 @@ template <typename T> int run_grad(const LoraArgs& g, hipStream_t st) {
 }
 
 // T > 64: the low-rank vectors, then the shared product that adds the adapters' parts
-size_t forward_ws(const LoraArgs& g) {
-  return g.T <= 64 ? lora_few_ws(g) : ((size_t)g.T * low_pitch(g.prec, g.r) * mid_bytes(g.prec) + 255 & ~(size_t)255) * 2;
-}
+struct ForwardWs {
+  int* arrived;
+  char *hi, *lo, *share;
+  int rp;
+  size_t zero, bytes;
+  ForwardWs(const LoraArgs& g, void* ws) {
+    rp = low_pitch(g.prec, g.r);
+    const size_t n = (size_t)g.T * rp, working = g.prec == DPL_D ? 8 : 4;
+    const LowPlan p = low_plan(mid_bytes(g.prec), g.T, g.r, 1);
+    Carve c{(char*)ws};
+    arrived = c.take<int>((size_t)p.tiles * p.blocks);  // first: zero before the first run
+    zero = c.used;
+    hi = c.take<char>(n * mid_bytes(g.prec));
+    lo = c.take<char>(n * mid_bytes(g.prec));
+    share = c.take<char>(p.splits > 1 ? n * p.splits * working : 0);
+    bytes = c.used;
+  }
+};
 
 int forward(const LoraArgs& g, hipStream_t st) {
-  if ((size_t)g.ws_bytes < forward_ws(g)) return -2;
-  if (g.T <= 64) return lora_few(g, st);
-  const int rp = low_pitch(g.prec, g.r);
+  if (g.T <= 64) return (size_t)g.ws_bytes < lora_few_ws(g) ? -2 : lora_few(g, st);
+  ForwardWs w(g, g.ws);
+  if ((size_t)g.ws_bytes < w.bytes) return -2;
   const int* ids = (const int*)g.ids;
-  char *hi = (char*)g.ws, *lo = hi + forward_ws(g) / 2;
   if (g.L > 0) {
-    const int rc = lora_low({g.X, g.A, g.scale, ids, g.ldx, g.lda, g.prec, g.T, g.K, g.r, g.L, {hi, lo, nullptr, nullptr, nullptr, 0, rp}}, st);
+    const LowArgs a{g.X, g.A, g.scale, ids, g.ldx, g.lda, g.prec, g.T, g.K, g.r, g.L, {w.hi, w.lo, nullptr, nullptr, nullptr, 0, w.rp}, w.share, w.arrived};
+    const int rc = lora_low(&a, 1, st);
     if (rc) return rc;
   }
-  return lora_tile({g.X, g.W, g.B, hi, lo, ids, g.Y, g.ldx, g.ldw, g.ldb, g.ldy, g.alpha, g.beta, g.prec, g.T, g.K, g.N, g.r, rp, g.L}, true, st);
+  return lora_tile({g.X, g.W, g.B, w.hi, w.lo, ids, g.Y, g.ldx, g.ldw, g.ldb, g.ldy, g.alpha, g.beta, g.prec, g.T, g.K, g.N, g.r, w.rp, g.L}, true, st);
 }
 
 }  // namespace
 
 DPL_API int dpl_lora_args_bytes() { return (int)sizeof(LoraArgs); }
 
-DPL_API long long dpl_lora_ws_bytes(const LoraArgs* g, int grad) {
-  if (!grad) return (long long)forward_ws(*g);
-  switch (g->prec) {
-    case DPL_S: return (long long)PlainWs<float>(*g, nullptr).bytes;
-    case DPL_D: return (long long)PlainWs<double>(*g, nullptr).bytes;
+// zero: bytes at its beginning that are zero before the first run
+DPL_API long long dpl_lora_ws_bytes(const LoraArgs* g, int grad, long long* zero) {
+  size_t z = 0, bytes;
+  if (!grad) {
+    const ForwardWs w(*g, nullptr);
+    z = g->T <= 64 ? 0 : w.zero;
+    bytes = g->T <= 64 ? lora_few_ws(*g) : w.bytes;
+  } else if (g->prec == DPL_S || g->prec == DPL_D) {
+    bytes = g->prec == DPL_S ? PlainWs<float>(*g, nullptr).bytes : PlainWs<double>(*g, nullptr).bytes;
+  } else {
+    bytes = lora_grad_ws(*g, &z);
   }
-  return (long long)lora_grad_ws(*g);
+  *zero = (long long)z;
+  return (long long)bytes;
 }
 
 DPL_API int dpl_lora(const LoraArgs* g, hipStream_t st) { return g->T == 0 || g->N == 0 ? 0 : forward(*g, st); }

@@ -30,10 +30,16 @@ __global__ __launch_bounds__(256) void k_few_low(const T* __restrict__ x, long l
   if (lane == 0) S[(long long)t * r + j] = s;
 }
 
-// 16 output features per workgroup, the contraction split over 8 waves and joined in LDS; G groups of 16 tokens.
+// 16 NF output features per workgroup, the contraction split over 8 waves and joined in LDS; G groups of 16 tokens.
 // W's fragments go straight from memory to the matrix instruction (each element is used by one wave once); x comes
-// from the caches.
-template <typename T, int G>
+// from the caches.  A wave has one batch of fragments under way after another, as large as the registers of one
+// workgroup per CU allow; what the adapters' parts need is asked for before and beside them.
+template <int N> struct Int {
+  static constexpr int value = N;
+};
+constexpr int S_MAX = 64;  // r up to which the low-rank vectors go through LDS
+
+template <typename T, int G, int NF>
 __global__ __launch_bounds__(512) void k_few_apply(const T* __restrict__ x, long long ldx, const T* __restrict__ W,
                                                    long long ldw, const T* __restrict__ B, long long ldb,
                                                    const int* __restrict__ ids,
@@ -42,25 +48,45 @@ __global__ __launch_bounds__(512) void k_few_apply(const T* __restrict__ x, long
                                                    typename Num<T>::acc beta, T* __restrict__ y, long long ldy) {
   typedef typename Num<T>::acc R;
   typedef typename Op<T>::vec V;
-  constexpr int E = Op<T>::E, KS = Op<T>::KS, U = G == 1 ? 8 : G == 2 ? 6 : 4;
-  __shared__ R red[8][16 * G][17];
+  constexpr int E = Op<T>::E, KS = Op<T>::KS, ROW = 16 * NF, LANES = 512 / ROW;  // tokens finished at a time
+  constexpr int TI = (16 * G + LANES - 1) / LANES, SI = 16 * G * S_MAX / 512;
+  __shared__ R red[8][16 * G][ROW + 1], low[16 * G * S_MAX];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, q = lane >> 4, c = lane & 15;
-  const int n0 = blockIdx.x * 16;
-  const int steps = (K + KS - 1) / KS, each = (steps + 7) / 8;
-  const int s0 = min(steps, w * each), s1 = min(steps, s0 + each);
-  typename Op<T>::out acc[G];
+  const int n0 = blockIdx.x * ROW;
+  const int steps = (K + KS - 1) / KS, s0 = steps * w / 8, s1 = steps * (w + 1) / 8, whole = min(s1, K / KS);
+  typename Op<T>::out acc[NF][G];
 #pragma unroll
-  for (int g = 0; g < G; ++g) acc[g] = typename Op<T>::out{R(0), R(0), R(0), R(0)};
-  const T* pw = W + (long long)min(n0 + c, N - 1) * ldw + q * E;
-  const T* px[G];
+  for (int f = 0; f < NF; ++f)
+#pragma unroll
+    for (int g = 0; g < G; ++g) acc[f][g] = typename Op<T>::out{R(0), R(0), R(0), R(0)};
+  const T *pw[NF], *px[G];
+#pragma unroll
+  for (int f = 0; f < NF; ++f) pw[f] = W + (long long)min(n0 + 16 * f + c, N - 1) * ldw + q * E;
 #pragma unroll
   for (int g = 0; g < G; ++g) px[g] = x + (long long)min(16 * g + c, nt - 1) * ldx + q * E;
-  const int whole = min(s1, K / KS);  // steps without an end of the rows in them
-  int s = s0;
-  for (; s + U <= whole; s += U) {
-    V a[U], b[U][G];
+  // this thread finishes feature n of tokens tid / ROW + LANES k
+  const int col = tid % ROW, n = n0 + col;
+  int lid[TI];
 #pragma unroll
-    for (int u = 0; u < U; ++u) a[u] = load_vec(pw + (long long)(s + u) * KS);
+  for (int k = 0; k < TI; ++k) {
+    const int t = tid / ROW + LANES * k;
+    lid[k] = L > 0 && t < nt ? ids[t] : -1;
+    if ((unsigned)lid[k] >= (unsigned)L) lid[k] = -1;
+  }
+  R sv[SI];
+  if (r <= S_MAX && L > 0) {
+#pragma unroll
+    for (int k = 0; k < SI; ++k)
+      if (tid + 512 * k < nt * r) sv[k] = S[tid + 512 * k];
+  }
+  int s = s0;
+  auto run = [&](auto width) {
+    constexpr int U = decltype(width)::value;
+    V a[U][NF], b[U][G];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int f = 0; f < NF; ++f) a[u][f] = load_vec(pw[f] + (long long)(s + u) * KS);
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -68,35 +94,81 @@ __global__ __launch_bounds__(512) void k_few_apply(const T* __restrict__ x, long
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int g = 0; g < G; ++g) acc[g] = Op<T>::mma(a[u], b[u][g], acc[g]);
-  }
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int f = 0; f < NF; ++f) acc[f][g] = Op<T>::mma(a[u][f], b[u][g], acc[f][g]);
+    s += U;
+  };
+  if constexpr (G == 1)
+    while (s + 16 <= whole) run(Int<16>());
+  if constexpr (sizeof(T) < 8)
+    while (s + 8 <= whole) run(Int<8>());
+  while (s + 4 <= whole) run(Int<4>());
+  while (s + 2 <= whole) run(Int<2>());
+  if (s < whole) run(Int<1>());
   for (; s < s1; ++s) {
     const int left = K - s * KS - q * E;
-    const V a = load_part(pw + (long long)s * KS, left);
+    V a[NF];
 #pragma unroll
-    for (int g = 0; g < G; ++g) acc[g] = Op<T>::mma(a, load_part(px[g] + (long long)s * KS, left), acc[g]);
+    for (int f = 0; f < NF; ++f) a[f] = load_part(pw[f] + (long long)s * KS, left);
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const V b = load_part(px[g] + (long long)s * KS, left);
+#pragma unroll
+      for (int f = 0; f < NF; ++f) acc[f][g] = Op<T>::mma(a[f], b, acc[f][g]);
+    }
   }
+  // the first two vectors of the adapters' rows, on their way during the join
+  const int nv = min(2, r / E);
+  V bv[TI][2];
+#pragma unroll
+  for (int k = 0; k < TI; ++k)
+    if (lid[k] >= 0 && n < N) {
+      const T* b = B + ((long long)lid[k] * N + n) * ldb;
+#pragma unroll
+      for (int v = 0; v < 2; ++v)
+        if (v < nv) bv[k][v] = load_vec(b + v * E);
+    }
 #pragma unroll
   for (int g = 0; g < G; ++g)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) red[w][16 * g + c][out_row<T>(lane, i)] = acc[g][i];
+    for (int f = 0; f < NF; ++f)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) red[w][16 * g + c][16 * f + out_row<T>(lane, i)] = acc[f][g][i];
+  if (r <= S_MAX && L > 0) {
+#pragma unroll
+    for (int k = 0; k < SI; ++k)
+      if (tid + 512 * k < nt * r) low[tid + 512 * k] = sv[k];
+  }
   __syncthreads();
-  const int n = n0 + c;
   if (n >= N) return;
-  for (int t = tid >> 4; t < nt; t += 32) {
+#pragma unroll
+  for (int k = 0; k < TI; ++k) {
+    const int t = tid / ROW + LANES * k;
+    if (t >= nt) continue;
     R v = 0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v += red[k][t][c];
-    const int l = ids[t];
-    if ((unsigned)l < (unsigned)L) {
-      const T* b = B + ((long long)l * N + n) * ldb;
-      const R* p = S + (long long)t * r;
-      for (int j = 0; j < r; j += E) {
-        const V f = load_part(b + j, r - j);
+    for (int i = 0; i < 8; ++i) v += red[i][t][col];
+    if (lid[k] >= 0) {
+      const T* b = B + ((long long)lid[k] * N + n) * ldb;
+      auto add = [&](const R* p) {
 #pragma unroll
-        for (int i = 0; i < E; ++i)
-          if (j + i < r) v = fma(p[j + i], (R)f[i], v);
-      }
+        for (int e = 0; e < 2; ++e)
+          if (e < nv) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) v = fma(p[e * E + i], (R)bv[k][e][i], v);
+          }
+        int j = nv * E;
+#pragma unroll 2
+        for (; j + E <= r; j += E) {
+          const V f = load_vec(b + j);
+#pragma unroll
+          for (int i = 0; i < E; ++i) v = fma(p[j + i], (R)f[i], v);
+        }
+        for (; j < r; ++j) v = fma(p[j], widen(b[j]), v);
+      };
+      if (r <= S_MAX) add(&low[t * r]);
+      else add(S + (long long)t * r);
     }
     T* o = &y[(long long)t * ldy + n];
     R u = alpha == R(0) ? R(0) : alpha * v;
@@ -111,13 +183,25 @@ template <typename T> int run(const LoraArgs& g, hipStream_t st) {
   const T *X = (const T*)g.X, *A = (const T*)g.A, *B = (const T*)g.B, *W = (const T*)g.W;
   const int* ids = (const int*)g.ids;
   if (g.L > 0) k_few_low<T><<<dim3(g.T, cdiv(g.r, 4)), 256, 0, st>>>(X, g.ldx, A, g.lda, ids, (const R*)g.scale, g.K, g.r, g.L, S);
+  // two fragments of features for a fragment of tokens where that leaves a workgroup for every CU: x is read half as
+  // often, and what a CU can have under way is the bound (48 tokens, 4096 x 8192: 43.4 us with one, 30.6 with two; 48
+  // tokens, 4096 x 4096: 23.2 with one, 27.0 with two)
+  const int nf = sizeof(T) < 8 && g.T > 16 && g.N >= 32 * 256 ? 2 : 1;
   auto apply = [&](auto kernel) {
-    kernel<<<cdiv(g.N, 16), 512, 0, st>>>(X, g.ldx, W, g.ldw, B, g.ldb, ids, S, g.T, g.K, g.N, g.r, g.L, (R)g.alpha, (R)g.beta,
+    kernel<<<cdiv(g.N, 16 * nf), 512, 0, st>>>(X, g.ldx, W, g.ldw, B, g.ldb, ids, S, g.T, g.K, g.N, g.r, g.L, (R)g.alpha, (R)g.beta,
                                           (T*)g.Y, g.ldy);
   };
-  if (g.T <= 16) apply(k_few_apply<T, 1>);
-  else if (g.T <= 32) apply(k_few_apply<T, 2>);
-  else apply(k_few_apply<T, 4>);
+  if constexpr (sizeof(T) < 8)
+    if (nf == 2) {
+      if (g.T <= 32) apply(k_few_apply<T, 2, 2>);
+      else if (g.T <= 48) apply(k_few_apply<T, 3, 2>);
+      else apply(k_few_apply<T, 4, 2>);
+      return (int)hipGetLastError();
+    }
+  if (g.T <= 16) apply(k_few_apply<T, 1, 1>);
+  else if (g.T <= 32) apply(k_few_apply<T, 2, 1>);
+  else if (g.T <= 48) apply(k_few_apply<T, 3, 1>);
+  else apply(k_few_apply<T, 4, 1>);
   return (int)hipGetLastError();
 }
 

@@ -9,127 +9,193 @@
 
 namespace {
 
-// ---------------------------------------------------------------- tokens in the order of their adapters
-// off[l] tokens have a smaller adapter, perm[off[l] ..] lists adapter l's tokens in their own order, pos is its inverse.
-// One workgroup per adapter reads all ids, so the order never depends on timing.
-__global__ __launch_bounds__(256) void k_sort(const int* __restrict__ ids, int nt, int L, int* __restrict__ off,
-                                              int* __restrict__ perm, int* __restrict__ pos, int4* __restrict__ zero) {
-  __shared__ int part[4], base;
-  const int l = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  if (l == 0 && tid == 0) *zero = int4{0, 0, 0, 0};
-  int below = 0;
-  for (int t = tid; t < nt; t += 256) {
-    const int id = ids[t];
-    below += id >= 0 && id < l;
+// ---------------------------------------------------------------- tokens in the order of their adapters; factors turned
+// off[l] tokens have a smaller adapter; adapter l's tokens take the places begin_of(l) .. in their own order: perm lists
+// them by place, pos is its inverse.  Places begin at multiples of 8 (16 bytes of the low-rank vectors) without any
+// workgroup having to know the others' counts: ceil8(off[l]) + 8 l leaves room for every rounding before.
+__device__ inline int begin_of(const int* off, int l) { return (off[l] + 7 & ~7) + 8 * l; }
+
+struct PrepareArgs {
+  const int* ids;
+  int *off, *perm, *pos;
+  int4* zero;
+  __bf16* low[4];  // places after an adapter's last token, up to a multiple of 8, are zeroed here (null: not in use)
+  long long tp;
+  int nt, L, r;
+  struct Turn {
+    const void* src;
+    void* dst;
+    long long lds;
+    int ldd, R, C, wgs;  // per adapter
+  } turn[2];
+};
+
+// dst[l][c][r] = src[l][r][c], rows of dst padded with zeros to ldd; 64 x 64 elements per workgroup
+template <typename T> __device__ inline void turn_tile(const PrepareArgs::Turn& a, int block) {
+  __shared__ T s[64][66];
+  const int tr = (a.ldd + 63) / 64;
+  const long long m = block / a.wgs;
+  const int in = block % a.wgs, r0 = in % tr * 64, c0 = in / tr * 64, tid = threadIdx.x;
+  const T* src = (const T*)a.src;
+  T v[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const int r = r0 + (tid >> 6) + 4 * k, c = c0 + (tid & 63);
+    v[k] = r < a.R && c < a.C ? src[(m * a.R + r) * a.lds + c] : (T)0;
   }
-  for (int o = 32; o; o >>= 1) below += __shfl_xor(below, o);
-  if (lane == 0) part[w] = below;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) s[(tid >> 6) + 4 * k][tid & 63] = v[k];
   __syncthreads();
-  if (tid == 0) base = part[0] + part[1] + part[2] + part[3];
-  __syncthreads();
-  int at0 = base;
-  if (tid == 0) off[l] = at0;
-  for (int t0 = 0; t0 < nt; t0 += 256) {
-    const bool mine = t0 + tid < nt && ids[t0 + tid] == l;
-    const unsigned long long m = __ballot(mine);
-    __syncthreads();
-    if (lane == 0) part[w] = __popcll(m);
-    __syncthreads();
-    int at = at0;
-    for (int v = 0; v < w; ++v) at += part[v];
-    at += __popcll(m & ((1ull << lane) - 1));
-    if (mine) {
-      perm[at] = t0 + tid;
-      pos[t0 + tid] = at;
-    }
-    at0 += part[0] + part[1] + part[2] + part[3];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const int c = (tid >> 6) + 4 * k, r = tid & 63;
+    if (c0 + c < a.C && r0 + r < a.ldd) ((T*)a.dst)[(m * a.C + c0 + c) * a.ldd + r0 + r] = s[r][c];
   }
-  if (tid == 0 && l == L - 1) off[L] = at0;
 }
 
-// dst[m][c][r] = src[m][r][c], rows of dst padded with zeros to ldd; 64 x 64 elements per workgroup
-template <typename T>
-__global__ __launch_bounds__(256) void k_turn(const T* __restrict__ src, long long lds, T* __restrict__ dst, int ldd,
-                                              int R, int C) {
-  __shared__ T s[64][66];
-  const long long m = blockIdx.z;
-  const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
-  for (int k = threadIdx.x; k < 4096; k += 256) {
-    const int r = k >> 6, c = k & 63;
-    s[r][c] = r0 + r < R && c0 + c < C ? src[(m * R + r0 + r) * lds + c0 + c] : (T)0;
+// One workgroup per adapter reads all ids, each thread a run of them, so the order never depends on timing.
+__device__ inline void sort_one(const PrepareArgs& a, int l) {
+  __shared__ int sums[2][4];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  if (l == 0 && tid == 0) *a.zero = int4{0, 0, 0, 0};
+  const int each = (a.nt + 255) / 256, t0 = min(a.nt, tid * each), t1 = min(a.nt, t0 + each);
+  int below = 0, mine = 0;
+#pragma unroll 8
+  for (int t = t0; t < t1; ++t) {
+    const int id = a.ids[t];
+    below += id >= 0 && id < l;
+    mine += id == l;
   }
+  int upto = mine;
+  for (int o = 1; o < 64; o <<= 1) {
+    const int b = __shfl_up(upto, o);
+    if (lane >= o) upto += b;
+  }
+  for (int o = 32; o; o >>= 1) below += __shfl_xor(below, o);
+  if (lane == 63) sums[0][w] = upto;
+  if (lane == 0) sums[1][w] = below;
   __syncthreads();
-  for (int k = threadIdx.x; k < 4096; k += 256) {
-    const int c = k >> 6, r = k & 63;
-    if (c0 + c < C && r0 + r < ldd) dst[(m * C + c0 + c) * ldd + r0 + r] = s[r][c];
+  const int first = sums[1][0] + sums[1][1] + sums[1][2] + sums[1][3];
+  const int count = sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3];
+  if (tid == 0) {
+    a.off[l] = first;
+    if (l == a.L - 1) a.off[l + 1] = first + count;
   }
+  const int begin = (first + 7 & ~7) + 8 * l;
+  int at = begin + upto - mine;
+  for (int k = 0; k < w; ++k) at += sums[0][k];
+  for (int t = t0; t < t1; ++t)
+    if (a.ids[t] == l) {
+      a.perm[at] = t;
+      a.pos[t] = at++;
+    }
+  const int end = begin + count, pad = (8 - count % 8) % 8;
+  for (int k = 0; k < 4; ++k)
+    if (a.low[k])
+      for (int i = tid; i < a.r * pad; i += 256) a.low[k][(i / pad) * a.tp + end + i % pad] = (__bf16)0.f;
+}
+
+template <typename T> __global__ __launch_bounds__(256) void k_prepare(PrepareArgs a) {
+  int b = blockIdx.x;
+  if (b < a.L) return sort_one(a, b);
+  b -= a.L;
+  if (b < a.turn[0].wgs * a.L) return turn_tile<T>(a.turn[0], b);
+  turn_tile<T>(a.turn[1], b - a.turn[0].wgs * a.L);
 }
 
 // ---------------------------------------------------------------- gradients of the factors
-// g_l(j, c) = alpha sum_{t of l} low(t, j) z[t*ldz + c].  An item is the part of one adapter's (sorted) tokens that lies
-// in one window of `win` positions; the items of windows and adapters are counted through (window + adapter).  An
-// adapter inside one window is finished here, others leave 32-bit parts that k_join adds in the order of the windows:
-// slot 2 w for the adapter that came in from window w - 1, 2 w + 1 for one that begins in w and goes on.
-// COLS columns per workgroup, 16 JF rows j; z goes through LDS in steps of 64 tokens as [token][column] and is read by
-// the transposing LDS read, low comes from memory as it is (both are laid out as in k_tile).
-struct OuterArgs {
+// g_l(j, c) = alpha sum_{t of l} low(t, j) z[t*ldz + c].  An item is the part of one adapter's places that lies in one
+// window of `win`; the items of windows and adapters are counted through (window + adapter).  An adapter inside one window
+// is finished here (one without tokens gets its zeros), others leave 32-bit parts that k_join adds in the order of the
+// windows: slot 2 w for the adapter that came in from window w - 1, 2 w + 1 for one that begins in w and goes on.
+// COLS columns per workgroup, 16 JF rows j.  Steps of 64 tokens go through a ring of LDS buffers: z as [token][column],
+// read by the transposing LDS read, low as [j][token] in its two parts (both laid out as in k_tile).
+struct OuterSet {
   const void *z, *thi, *tlo;
-  const int *off, *perm;
-  const int4* zero;
   void* out;
   float* part;
-  long long ldz, ldo, tp;
-  double alpha;
-  int C, r, L, win, items;
+  long long ldz, ldo;
+  int C, win, items, jc;  // jc: g is stored [j][c] (dA), else [c][j] (dB)
 };
-
-__device__ inline int find_item(const OuterArgs& a, int item, int& w) {
-  int lo = 0, hi = a.L - 1;  // the largest l whose first item is not past this one
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.off[mid] / a.win + mid <= item) lo = mid;
-    else hi = mid - 1;
-  }
-  w = item - lo;
-  return lo;
-}
+struct OuterArgs {
+  OuterSet set[2];
+  const int *off, *perm;
+  const int4* zero;
+  long long tp;
+  double alpha;
+  int r, L, wgs0;  // workgroups of the first set
+};
 
 constexpr int COLS = 256, WIN_MAX = 2048;
 
-// JC: g is stored [j][c] (dA), else [c][j] (dB)
-template <typename T, int JF, bool JC, bool DMA> __global__ __launch_bounds__(256, 2) void k_outer(OuterArgs a) {
+template <typename T, int JF, bool DMA> __global__ __launch_bounds__(256, 1) void k_outer(OuterArgs a) {
   typedef typename Op<T>::vec V;
-  typedef __bf16 M;
   constexpr int FN = COLS / 64, CH = COLS / 8, J = 64 * CH / 256;  // 4 waves of 64 columns; chunks of a row; per thread
-  __shared__ __attribute__((aligned(1024))) char sm[2][64 * COLS * 2];
+  constexpr int ZB = 64 * COLS * 2, PB = JF * 16 * 128, STAGE = ZB + 2 * PB, RING = DMA ? (JF == 1 ? 4 : 3) : 2;
+  constexpr int PJ = 2 * PB / 4096, LOADS = J + PJ;
+  __shared__ __attribute__((aligned(1024))) char sm[RING * STAGE];
   __shared__ int rows[WIN_MAX];
-  const int ct = (a.C + COLS - 1) / COLS;
-  const int c0 = blockIdx.x % ct * COLS, j0 = blockIdx.y * 16 * JF;
-  int w;
-  const int l = find_item(a, blockIdx.x / ct, w);
-  const int lo = a.off[l], end = a.off[l + 1];
-  const int p0 = max(lo, w * a.win), p1 = min(end, (w + 1) * a.win);
-  if (p0 >= p1) return;
+  const bool second = (int)blockIdx.x >= a.wgs0;
+  const OuterSet& g = a.set[second];
+  const int block = second ? blockIdx.x - a.wgs0 : blockIdx.x;
+  const int ct = (g.C + COLS - 1) / COLS, item = block / ct;
+  const int c0 = block % ct * COLS, j0 = blockIdx.y * 16 * JF;
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, c16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  for (int k = tid; k < p1 - p0; k += 256) rows[k] = a.perm[p0 + k];
+  int l = 0;
+  for (int hi = a.L - 1; l < hi;) {  // the largest adapter whose first item is not past this one
+    const int mid = (l + hi + 1) >> 1;
+    if (begin_of(a.off, mid) / g.win + mid <= item) l = mid;
+    else hi = mid - 1;
+  }
+  const int w = item - l, lo = begin_of(a.off, l), count = a.off[l + 1] - a.off[l], end = lo + count;
+  T* out = (T*)g.out;
+  auto where = [&](int j, int c) { return g.jc ? ((long long)l * a.r + j) * g.ldo + c : ((long long)l * g.C + c) * g.ldo + j; };
+  if (count == 0) {
+    if (w == lo / g.win)
+      for (int i = tid; i < 16 * JF * COLS; i += 256) {
+        const int j = j0 + (g.jc ? i / COLS : i % (16 * JF)), c = c0 + (g.jc ? i % COLS : i / (16 * JF));
+        if (j < a.r && c < g.C) out[where(j, c)] = (T)0;
+      }
+    return;
+  }
+  const int p0 = max(lo, w * g.win), p1 = min(end, (w + 1) * g.win), n = p1 - p0;
+  if (n <= 0) return;
+  for (int k = tid; k < n; k += 256) rows[k] = a.perm[p0 + k];
   __syncthreads();
-  const T* z = (const T*)a.z;
+  const T* z = (const T*)g.z;
   auto turn = [](int step) { return (step & 3) + 4 * ((step >> 3) & 1); };
-  const int sr = tid / CH, pc = tid % CH;  // chunk tid + 256 j: row sr + 8 j, whose turn only depends on sr and j's parity
-  V g[DMA ? 1 : J];
-  auto stage = [&](int b, int s) {
+  const int sr = tid / CH, pc = tid % CH;
+  V v[DMA ? 1 : J];
+  auto stage_low = [&](char* b, int s) {
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const int row = sr + j * (256 / CH), k = s + row;
+    for (int k = 0; k < PJ; ++k) {
+      const int part = k >= PJ / 2, half = k % (PJ / 2 ? PJ / 2 : 1);
+      const int id = PJ / 2 ? tid + 256 * half : tid & 127, pt = PJ / 2 ? part : tid >> 7;
+      const int row = id >> 3, at = s + 8 * ((id & 7) ^ (row & 7));
+      const __bf16* src = (const __bf16*)(pt ? g.tlo : g.thi) + min(j0 + row, a.r - 1) * a.tp + p0 + at;
+      dma_global(at < n ? (const void*)src : (const void*)a.zero, b + ZB + wave * 1024 + k * 4096);
+    }
+  };
+  auto stage = [&](int s) {
+    char* b = &sm[(s / 64) % RING * STAGE];
+#pragma unroll
+    for (int k = 0; k < J; ++k) {
+      const int row = sr + k * (256 / CH), t = s + row;
       const int c = c0 + (2 * ((pc >> 1) ^ turn(row)) + (pc & 1)) * 8;
       if constexpr (DMA) {
-        const void* p = k < p1 - p0 && c < a.C ? (const void*)(z + (long long)rows[k] * a.ldz + c) : (const void*)a.zero;
-        dma_global(p, &sm[b][wave * 1024 + j * 4096]);
+        const void* p = t < n && c < g.C ? (const void*)(z + (long long)rows[min(t, n - 1)] * g.ldz + c) : (const void*)a.zero;
+        dma_global(p, b + wave * 1024 + k * 4096);
       } else {
-        g[j] = load_part(z + (k < p1 - p0 ? (long long)rows[k] * a.ldz + c : 0), k < p1 - p0 ? a.C - c : 0);
+        v[k] = load_part(z + (t < n ? (long long)rows[t] * g.ldz + c : 0), t < n ? g.C - c : 0);
       }
     }
+    stage_low(b, s);
+  };
+  auto put = [&](int s) {
+    char* b = &sm[(s / 64) % RING * STAGE];
+#pragma unroll
+    for (int k = 0; k < J; ++k) *(V*)(b + (tid + 256 * k) * 16) = v[k];
   };
   typename Op<T>::out acc[JF][FN];
 #pragma unroll
@@ -138,182 +204,210 @@ template <typename T, int JF, bool JC, bool DMA> __global__ __launch_bounds__(25
     for (int f = 0; f < FN; ++f) acc[i][f] = f4_t{0, 0, 0, 0};
   const int ftr = (8 * q + (c16 >> 2)) * (COLS * 2) + (c16 & 3) * 8;
   const int tw = (c16 >> 2) + 4 * (q & 1);
-  const int n = p1 - p0;
-  stage(0, 0);
-  for (int s = 0, b = 0; s < n; s += 64, b ^= 1) {
-    // low's fragments of this step; zeros past the adapter's last token
-    b8_t hi[2][JF], lw[2][JF];
+  const int fp = ZB + c16 * 128 + ((q ^ (c16 & 7)) << 4);
+  auto multiply = [&](int s) {
+    const char* b = &sm[(s / 64) % RING * STAGE];
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
+    for (int kk = 0; kk < 2; ++kk) {
+      b8_t hi[JF], lw[JF];
 #pragma unroll
       for (int i = 0; i < JF; ++i) {
-        const int j = min(j0 + 16 * i + c16, a.r - 1), k = s + kk * 32 + q * 8;
-        const long long at = j * a.tp + p0 + k;
-        hi[kk][i] = load_vec((const M*)a.thi + at);
-        lw[kk][i] = load_vec((const M*)a.tlo + at);
-        if (s + 64 > n) {
-#pragma unroll
-          for (int v = 0; v < 8; ++v) {
-            hi[kk][i][v] = k + v < n ? hi[kk][i][v] : (M)0.f;
-            lw[kk][i][v] = k + v < n ? lw[kk][i][v] : (M)0.f;
-          }
-        }
+        hi[i] = *(const b8_t*)(b + (fp ^ (64 * kk)) + i * 2048);
+        lw[i] = *(const b8_t*)(b + (fp ^ (64 * kk)) + PB + i * 2048);
       }
-    if constexpr (!DMA) {
-#pragma unroll
-      for (int j = 0; j < J; ++j) *(V*)&sm[b][(tid + 256 * j) * 16] = g[j];
-    }
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-    if (s + 64 < n) stage(b ^ 1, s + 64);
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
       for (int f = 0; f < FN; ++f) {
         typedef short s4_t __attribute__((ext_vector_type(4)));
         typedef short s8_t __attribute__((ext_vector_type(8)));
         typedef __attribute__((address_space(3))) s4_t* lp;
-        const char* p = &sm[b][ftr + (((wave * FN + f) ^ tw) << 5) + kk * 32 * COLS * 2];
+        const char* p = b + ftr + (((wave * FN + f) ^ tw) << 5) + kk * 32 * COLS * 2;
         const s4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p));
         const s4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p + 4 * COLS * 2));
         const s8_t both = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
         MidOp<T> x;
         x.set(__builtin_bit_cast(V, both));
 #pragma unroll
-        for (int i = 0; i < JF; ++i) acc[i][f] = x.mma_first(hi[kk][i], lw[kk][i], acc[i][f]);
+        for (int i = 0; i < JF; ++i) acc[i][f] = x.mma_first(hi[i], lw[i], acc[i][f]);
       }
+    }
+  };
+  auto meet = [&]() {
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if constexpr (DMA) {
+#pragma unroll
+    for (int k = 0; k < RING - 1; ++k) stage(64 * k);  // past the last token: zeros
+    for (int s = 0; s < n; s += 64) {
+      // this step has arrived, and every wave has read the one before, whose buffer is filled next
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS * (RING - 2)) : "memory");
+      meet();
+      stage(s + 64 * (RING - 1));
+      multiply(s);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing is on its way to LDS when the workgroup ends
+  } else {
+    stage(0);
+    put(0);
+    for (int s = 0; s < n; s += 64) {
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      meet();
+      if (s + 64 < n) stage(s + 64);
+      multiply(s);
+      if (s + 64 < n) put(s + 64);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
-  const bool whole = lo / a.win == (end - 1) / a.win;
+  const bool whole = lo / g.win == (end - 1) / g.win;
   const float alpha = (float)a.alpha;
-  float* part = a.part + (long long)(2 * w + (lo >= w * a.win)) * a.r * a.C;
-  T* out = (T*)a.out;
+  float* part = g.part + (long long)(2 * w + (lo >= w * g.win)) * a.r * g.C;
 #pragma unroll
   for (int f = 0; f < FN; ++f) {
     const int c = c0 + (wave * FN + f) * 16 + c16;
-    if (c >= a.C) continue;
+    if (c >= g.C) continue;
 #pragma unroll
     for (int i = 0; i < JF; ++i)
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const int j = j0 + 16 * i + 4 * q + v;
+      for (int k = 0; k < 4; ++k) {
+        const int j = j0 + 16 * i + 4 * q + k;
         if (j >= a.r) continue;
-        if (whole) {
-          const T o = (T)(alpha == 0.f ? 0.f : alpha * acc[i][f][v]);
-          out[JC ? ((long long)l * a.r + j) * a.ldo + c : ((long long)l * a.C + c) * a.ldo + j] = o;
-        } else {
-          part[JC ? (long long)j * a.C + c : (long long)c * a.r + j] = acc[i][f][v];
-        }
+        if (whole) out[where(j, c)] = (T)(alpha == 0.f ? 0.f : alpha * acc[i][f][k]);
+        else part[g.jc ? (long long)j * g.C + c : (long long)c * a.r + j] = acc[i][f][k];
       }
   }
 }
 
-// Parts of an adapter's windows added in order; zeros for an adapter without tokens.
-template <typename T, bool JC> __global__ __launch_bounds__(256) void k_join(OuterArgs a) {
-  const int l = blockIdx.y, lo = a.off[l], end = a.off[l + 1];
-  const int w0 = lo / a.win, w1 = lo < end ? (end - 1) / a.win : w0 - 1;
+// Parts of the adapters that go over several windows, added in the windows' order.
+template <typename T> __global__ __launch_bounds__(256) void k_join(OuterArgs a) {
+  const OuterSet& g = a.set[blockIdx.z];
+  const int l = blockIdx.y, lo = begin_of(a.off, l), count = a.off[l + 1] - a.off[l];
+  if (!g.out || count == 0) return;
+  const int w0 = lo / g.win, w1 = (lo + count - 1) / g.win;
   if (w0 == w1) return;
-  const long long n = (long long)a.r * a.C;
-  const int width = JC ? a.C : a.r;
+  const long long n = (long long)a.r * g.C;
+  const int width = g.jc ? g.C : a.r;
   const float alpha = (float)a.alpha;
   for (long long e = blockIdx.x * 256ll + threadIdx.x; e < n; e += gridDim.x * 256ll) {
     float v = 0;
-    for (int w = w0; w <= w1; ++w) v += a.part[(2 * w + (w == w0)) * n + e];
-    ((T*)a.out)[((long long)l * (n / width) + e / width) * a.ldo + e % width] = (T)(alpha == 0.f ? 0.f : alpha * v);
+#pragma unroll 4
+    for (int w = w0; w <= w1; ++w) v += g.part[(2 * w + (w == w0)) * n + e];
+    ((T*)g.out)[((long long)l * (n / width) + e / width) * g.ldo + e % width] = (T)(alpha == 0.f ? 0.f : alpha * v);
   }
 }
 
-// Window length: about 512 workgroups (2 per CU), in whole steps, the ids of a window in LDS.
-int window(int T, int C, int r) {
-  const int tiles = cdiv(C, COLS) * cdiv(r, 64), parts = max(1, 512 / max(1, tiles));
-  return min(WIN_MAX, max(64, cdiv(cdiv(T, parts), 64) * 64));
+// places in all, and a window's length: about 512 workgroups, in whole steps, a window's tokens in LDS; few tokens stay
+// in one window, which needs no join
+long long places(const LoraArgs& g) { return cdiv(g.T, 8) * 8ll + 8ll * (g.L + 1); }
+int window(const LoraArgs& g, int C) {
+  if (places(g) <= 512) return 512;
+  const int tiles = cdiv(C, COLS) * cdiv(g.r, 64), parts = max(1, 512 / max(1, tiles));
+  return min(WIN_MAX, max(256, cdiv(cdiv(g.T, parts), 64) * 64));
 }
 
 template <typename T> struct GradWs {
+  int *arrived[2], *off, *perm, *pos;
   __bf16 *hi = nullptr, *lo = nullptr, *pthi = nullptr, *ptlo = nullptr, *sthi = nullptr, *stlo = nullptr;
   T *At = nullptr, *Bt = nullptr;
-  int *off, *perm, *pos;
-  int4* zero;
-  float *pa = nullptr, *pb = nullptr;
+  int4* zeros;
+  float *share[2], *pa = nullptr, *pb = nullptr;
+  bool dx, da, db;
   int rp, ldb, wa, wb;
   long long tp;
-  size_t bytes;
+  size_t zero, bytes;
   GradWs(const LoraArgs& g, void* ws) {
+    dx = g.dX && g.K > 0 && g.T > 0;
+    da = g.dA && g.K > 0 && g.L > 0;
+    db = g.dB && g.N > 0 && g.L > 0;
     rp = low_pitch(g.prec, g.r);
     ldb = cdiv(g.N, 8) * 8;
-    tp = cdiv(g.T, 64) * 64 + 64;  // fragments past the last token stay inside
-    wa = window(g.T, g.K, g.r);
-    wb = window(g.T, g.N, g.r);
-    const bool fac = g.dA || g.dB;
+    tp = (places(g) + 63) / 64 * 64 + 64;
+    wa = window(g, g.K);
+    wb = window(g, g.N);
+    const LowPlan p = low_plan(sizeof(T), g.T, g.r, 1);  // one set has the most splits
     Carve c{(char*)ws};
-    zero = c.take<int4>(1);
+    for (int k = 0; k < 2; ++k) arrived[k] = c.take<int>((size_t)p.tiles * p.blocks);  // first: zero before the first run
+    zero = c.used;
+    zeros = c.take<int4>(1);
     off = c.take<int>(g.L + 1);
-    perm = c.take<int>(g.T);
+    perm = c.take<int>(places(g));
     pos = c.take<int>(g.T);
-    if (g.dX) {
+    for (int k = 0; k < 2; ++k) share[k] = c.take<float>(p.splits > 1 ? (size_t)p.splits * g.T * rp : 0);
+    if (dx) {
       hi = c.take<__bf16>((size_t)g.T * rp);
       lo = c.take<__bf16>((size_t)g.T * rp);
       At = c.take<T>((size_t)g.L * g.K * rp);
     }
-    if (g.dX || g.dA) Bt = c.take<T>((size_t)g.L * g.r * ldb);
-    if (fac) {
-      if (g.dA) pthi = c.take<__bf16>(g.r * tp), ptlo = c.take<__bf16>(g.r * tp);
-      if (g.dB) sthi = c.take<__bf16>(g.r * tp), stlo = c.take<__bf16>(g.r * tp);
-      if (g.dA) pa = c.take<float>((size_t)2 * (g.T / wa + 1) * g.r * g.K);
-      if (g.dB) pb = c.take<float>((size_t)2 * (g.T / wb + 1) * g.r * g.N);
+    if (dx || da) Bt = c.take<T>((size_t)g.L * g.r * ldb);
+    if (da) {
+      pthi = c.take<__bf16>(g.r * tp);
+      ptlo = c.take<__bf16>(g.r * tp);
+      pa = c.take<float>((size_t)2 * (places(g) / wa + 1) * g.r * g.K);
+    }
+    if (db) {
+      sthi = c.take<__bf16>(g.r * tp);
+      stlo = c.take<__bf16>(g.r * tp);
+      pb = c.take<float>((size_t)2 * (places(g) / wb + 1) * g.r * g.N);
     }
     bytes = c.used;
   }
 };
 
-template <typename T, bool JC> void run_outer(OuterArgs a, int nt, hipStream_t st) {
-  const bool dma = ((uintptr_t)a.z | (uintptr_t)(a.ldz * sizeof(T))) % 16 == 0 && a.C % 8 == 0;
-  a.items = nt / a.win + a.L;
-  const int jf = a.r <= 16 ? 1 : a.r <= 32 ? 2 : 4;
-  const dim3 grid((unsigned)(cdiv(a.C, COLS) * a.items), cdiv(a.r, 16 * jf));
-  auto go = [&](auto kernel) { kernel<<<grid, 256, 0, st>>>(a); };
-  if (nt > 0) {
-    if (jf == 1) dma ? go(k_outer<T, 1, JC, true>) : go(k_outer<T, 1, JC, false>);
-    else if (jf == 2) dma ? go(k_outer<T, 2, JC, true>) : go(k_outer<T, 2, JC, false>);
-    else dma ? go(k_outer<T, 4, JC, true>) : go(k_outer<T, 4, JC, false>);
-  }
-  k_join<T, JC><<<dim3(min(512, cdiv(a.r, 1) * cdiv(a.C, 256)), a.L), 256, 0, st>>>(a);
-}
-
 template <typename T> int run(const LoraArgs& g, hipStream_t st) {
   GradWs<T> w(g, g.ws);
   if ((size_t)g.ws_bytes < w.bytes) return -2;
   const int* ids = (const int*)g.ids;
-  const bool dx = g.dX && g.K > 0 && g.T > 0, da = g.dA && g.K > 0 && g.L > 0, db = g.dB && g.N > 0 && g.L > 0;
-  if (g.L > 0) k_sort<<<g.L, 256, 0, st>>>(ids, g.T, g.L, w.off, w.perm, w.pos, w.zero);
-  if (g.L > 0 && g.T > 0 && (dx || da) && g.N > 0)
-    k_turn<T><<<dim3(cdiv(g.r, 64), cdiv(w.ldb, 64), g.L), 256, 0, st>>>((const T*)g.B, g.ldb, w.Bt, w.ldb, g.N, g.r);
-  if (g.L > 0 && dx)
-    k_turn<T><<<dim3(cdiv(g.K, 64), cdiv(w.rp, 64), g.L), 256, 0, st>>>((const T*)g.A, g.lda, w.At, w.rp, g.r, g.K);
+  const bool low = g.L > 0 && g.T > 0, p = low && (w.dx || w.da), s = low && w.db;
+  if (g.L > 0) {
+    PrepareArgs a{ids, w.off, w.perm, w.pos, w.zeros, {w.pthi, w.ptlo, w.sthi, w.stlo}, w.tp, g.T, g.L, g.r, {}};
+    if (p && g.N > 0) a.turn[0] = {g.B, w.Bt, g.ldb, w.ldb, g.N, g.r, cdiv(w.ldb, 64) * cdiv(g.r, 64)};
+    if (low && w.dx) a.turn[1] = {g.A, w.At, g.lda, w.rp, g.r, g.K, cdiv(w.rp, 64) * cdiv(g.K, 64)};
+    k_prepare<T><<<(unsigned)(g.L * (1ll + a.turn[0].wgs + a.turn[1].wgs)), 256, 0, st>>>(a);
+  }
   int rc = 0;
-  if (g.L > 0 && g.T > 0 && (dx || da)) {
-    LowArgs a{g.dY, w.Bt, g.scale, ids, g.ldy, w.ldb, g.prec, g.T, g.N, g.r, g.L,
-              {dx ? w.hi : nullptr, w.lo, da ? w.pthi : nullptr, w.ptlo, w.pos, w.tp, w.rp}};
-    rc = lora_low(a, st);
+  if (p || s) {
+    LowArgs a[2];
+    int n = 0;
+    if (p)
+      a[n++] = {g.dY, w.Bt, g.scale, ids, g.ldy, w.ldb, g.prec, g.T, g.N, g.r, g.L,
+                {w.dx ? w.hi : nullptr, w.lo, w.da ? w.pthi : nullptr, w.ptlo, w.pos, w.tp, w.rp}, w.share[0], w.arrived[0]};
+    if (s)
+      a[n++] = {g.X, g.A, g.scale, ids, g.ldx, g.lda, g.prec, g.T, g.K, g.r, g.L,
+                {nullptr, nullptr, w.sthi, w.stlo, w.pos, w.tp, g.r}, w.share[1], w.arrived[1]};
+    rc = lora_low(a, n, st);
   }
-  if (!rc && db && g.T > 0) {
-    LowArgs a{g.X, g.A, g.scale, ids, g.ldx, g.lda, g.prec, g.T, g.K, g.r, g.L, {nullptr, nullptr, w.sthi, w.stlo, w.pos, w.tp, g.r}};
-    rc = lora_low(a, st);
+  if (!rc && w.dx)
+    rc = lora_tile({g.dY, g.W, w.At, w.hi, w.lo, ids, g.dX, g.ldy, g.ldw, w.rp, g.lddx, g.alpha, 0.0, g.prec, g.T, g.N, g.K, g.r, w.rp, g.L}, false, st);
+  if (rc || !(w.da || w.db)) return rc;
+  OuterArgs a{{}, w.off, w.perm, w.zeros, w.tp, g.alpha, g.r, g.L, 0};
+  auto wgs = [&](const OuterSet& o) { return o.out ? cdiv(o.C, COLS) * o.items : 0; };
+  if (w.da) a.set[0] = {g.X, w.pthi, w.ptlo, g.dA, w.pa, g.ldx, g.ldda, g.K, w.wa, (int)(places(g) / w.wa) + g.L, 1};
+  if (w.db) a.set[1] = {g.dY, w.sthi, w.stlo, g.dB, w.pb, g.ldy, g.lddb, g.N, w.wb, (int)(places(g) / w.wb) + g.L, 0};
+  a.wgs0 = wgs(a.set[0]);
+  auto aligned = [&](const OuterSet& o) { return !o.out || (((uintptr_t)o.z | (uintptr_t)(o.ldz * sizeof(T))) % 16 == 0 && o.C % 8 == 0); };
+  const bool dma = aligned(a.set[0]) && aligned(a.set[1]);
+  const int jf = g.r <= 16 ? 1 : g.r <= 32 ? 2 : 4;
+  const dim3 grid((unsigned)(a.wgs0 + wgs(a.set[1])), cdiv(g.r, 16 * jf));
+  auto go = [&](auto kernel) { kernel<<<grid, 256, 0, st>>>(a); };
+  if (jf == 1) dma ? go(k_outer<T, 1, true>) : go(k_outer<T, 1, false>);
+  else if (jf == 2) dma ? go(k_outer<T, 2, true>) : go(k_outer<T, 2, false>);
+  else dma ? go(k_outer<T, 4, true>) : go(k_outer<T, 4, false>);
+  if ((w.da && places(g) > w.wa) || (w.db && places(g) > w.wb)) {
+    const long long most = (long long)g.r * max(w.da ? g.K : 0, w.db ? g.N : 0);
+    k_join<T><<<dim3((unsigned)min(512ll, (most + 255) / 256), g.L, 2), 256, 0, st>>>(a);
   }
-  if (!rc && dx) {
-    TileArgs a{g.dY, g.W, w.At, w.hi, w.lo, ids, g.dX, g.ldy, g.ldw, w.rp, g.lddx, g.alpha, 0.0, g.prec, g.T, g.N, g.K, g.r, w.rp, g.L};
-    rc = lora_tile(a, false, st);
-  }
-  if (rc) return rc;
-  if (da) run_outer<T, true>({g.X, w.pthi, w.ptlo, w.off, w.perm, w.zero, g.dA, w.pa, g.ldx, g.ldda, w.tp, g.alpha, g.K, g.r, g.L, w.wa, 0}, g.T, st);
-  if (db) run_outer<T, false>({g.dY, w.sthi, w.stlo, w.off, w.perm, w.zero, g.dB, w.pb, g.ldy, g.lddb, w.tp, g.alpha, g.N, g.r, g.L, w.wb, 0}, g.T, st);
   return (int)hipGetLastError();
 }
 
 }  // namespace
 
-size_t lora_grad_ws(const LoraArgs& g) { return g.prec == DPL_H ? GradWs<_Float16>(g, nullptr).bytes : GradWs<__bf16>(g, nullptr).bytes; }
+size_t lora_grad_ws(const LoraArgs& g, size_t* zero) {
+  auto get = [&](auto w) {
+    *zero = w.zero;
+    return w.bytes;
+  };
+  return g.prec == DPL_H ? get(GradWs<_Float16>(g, nullptr)) : get(GradWs<__bf16>(g, nullptr));
+}
 
 int lora_grad_half(const LoraArgs& g, hipStream_t st) {
   return g.prec == DPL_H ? run<_Float16>(g, st) : run<__bf16>(g, st);

@@ -5,41 +5,47 @@
 namespace {
 
 // ---------------------------------------------------------------- low-rank vectors
+// One or two sets of them (the gradient's P and S) in a launch.
+struct LowSets {
+  LowArgs set[2];
+  int sets, splits;
+};
+
 // One wave per (token, j): for few tokens, where the tokens of a workgroup's rows would mostly have adapters of their own.
-template <typename T> __global__ __launch_bounds__(256) void k_low_dot(LowArgs a) {
+template <typename T> __global__ __launch_bounds__(256) void k_low_dot(LowSets sets) {
   typedef typename Num<T>::acc R;
   constexpr int E = Op<T>::E;
+  const LowArgs& a = sets.set[blockIdx.z];
   const int t = blockIdx.x, j = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int l = a.ids[t];
-  if (j >= a.out.rp || (unsigned)l >= (unsigned)a.L) return;
+  if (j >= a.r || (unsigned)l >= (unsigned)a.L) return;
+  if (j == 0 && lane < a.out.rp - a.r) pad_low<T>(a.out, t, a.r + lane);
   R s = 0;
-  if (j < a.r) {
-    const T* f = (const T*)a.F + ((long long)l * a.r + j) * a.ldf;
-    const T* p = (const T*)a.x + (long long)t * a.ldx;
+  const T* f = (const T*)a.F + ((long long)l * a.r + j) * a.ldf;
+  const T* p = (const T*)a.x + (long long)t * a.ldx;
 #pragma unroll 4
-    for (int c = lane * E; c < a.C; c += 64 * E) {
-      const typename Op<T>::vec u = load_part(f + c, a.C - c), v = load_part(p + c, a.C - c);
+  for (int c = lane * E; c < a.C; c += 64 * E) {
+    const typename Op<T>::vec u = load_part(f + c, a.C - c), v = load_part(p + c, a.C - c);
 #pragma unroll
-      for (int i = 0; i < E; ++i) s = fma((R)u[i], (R)v[i], s);
-    }
-    for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
-    s *= a.scale ? ((const R*)a.scale)[l] : R(1);
+    for (int i = 0; i < E; ++i) s = fma((R)u[i], (R)v[i], s);
   }
-  if (lane == 0) {
-    LowOut o = a.out;
-    if (j >= a.r) o.thi = nullptr;
-    put_low<T>(o, t, j, s);
-  }
+  for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
+  s *= a.scale ? ((const R*)a.scale)[l] : R(1);
+  if (lane == 0) put_low<T>(a.out, t, j, s);
 }
 
 // 16 TF tokens and 16 JF rows of the factors per workgroup, the contraction split over 8 waves and joined in LDS, one
-// adapter of these tokens at a time.
-template <typename T, int JF, int TF> __global__ __launch_bounds__(512) void k_low_tile(LowArgs a) {
+// adapter of these tokens at a time.  Many tokens per workgroup keep the factors' traffic down (each workgroup reads its
+// adapters' rows from the caches); `splits` workgroups then share the contraction, and the last one to arrive adds their
+// parts in order.
+template <typename T, int JF, int TF> __global__ __launch_bounds__(512) void k_low_tile(LowSets sets) {
   typedef typename Num<T>::acc R;
   typedef typename Op<T>::vec V;
-  constexpr int E = Op<T>::E, KS = Op<T>::KS, U = 2;
-  __shared__ R red[8][16 * JF][16 * TF + 1];
-  __shared__ int sid[16 * TF];
+  constexpr int E = Op<T>::E, KS = Op<T>::KS, U = JF * TF <= 2 ? 4 : 2;
+  __shared__ R red[8][16][16 * TF + 1];
+  __shared__ int sid[16 * TF], last;
+  const LowArgs& a = sets.set[blockIdx.z / sets.splits];
+  const int splits = sets.splits, z = blockIdx.z % splits;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, q = lane >> 4, c = lane & 15;
   const int t0 = blockIdx.x * 16 * TF, j0 = blockIdx.y * 16 * JF;
   int mine = -1;
@@ -49,8 +55,10 @@ template <typename T, int JF, int TF> __global__ __launch_bounds__(512) void k_l
   const T* px[TF];
 #pragma unroll
   for (int f = 0; f < TF; ++f) px[f] = (const T*)a.x + (long long)min(t0 + 16 * f + c, a.nt - 1) * a.ldx + q * E;
-  const int steps = (a.C + KS - 1) / KS, each = (steps + 7) / 8;
-  const int s0 = min(steps, w * each), s1 = min(steps, s0 + each), whole = min(s1, a.C / KS);
+  const int steps = (a.C + KS - 1) / KS, parts = 8 * splits, part = 8 * z + w;
+  const int s0 = (int)((long long)steps * part / parts), s1 = (int)((long long)steps * (part + 1) / parts), whole = min(s1, a.C / KS);
+  auto scale = [&](int l) { return a.scale ? ((const R*)a.scale)[l] : R(1); };
+  R* share = (R*)a.share;
   unsigned long long todo = __ballot(mine >= 0);
   while (todo) {
     const int l = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
@@ -94,59 +102,77 @@ template <typename T, int JF, int TF> __global__ __launch_bounds__(512) void k_l
       }
     }
 #pragma unroll
-    for (int i = 0; i < JF; ++i)
+    for (int i = 0; i < JF; ++i) {
+      __syncthreads();
 #pragma unroll
       for (int k = 0; k < TF; ++k)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) red[w][16 * i + out_row<T>(lane, v)][16 * k + c] = acc[i][k][v];
-    __syncthreads();
-    const R sc = a.scale ? ((const R*)a.scale)[l] : R(1);
-    for (int p = tid; p < 256 * JF * TF; p += 512) {
-      const int j = p % (16 * JF), t = p / (16 * JF);
-      if (sid[t] != l || j0 + j >= a.out.rp) continue;
-      R v = 0;
-      if (j0 + j < a.r) {
+        for (int v = 0; v < 4; ++v) red[w][out_row<T>(lane, v)][16 * k + c] = acc[i][k][v];
+      __syncthreads();
+      for (int p = tid; p < 256 * TF; p += 512) {
+        const int j = j0 + 16 * i + p % 16, t = p / 16;
+        if (sid[t] != l || j >= a.r) continue;
+        R v = 0;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v += red[k][j][t];
-        put_low<T>(a.out, t0 + t, j0 + j, sc * v);
-      } else {
-        LowOut o = a.out;
-        o.thi = nullptr;
-        put_low<T>(o, t0 + t, j0 + j, v);
+        for (int k = 0; k < 8; ++k) v += red[k][p % 16][t];
+        if (splits == 1) put_low<T>(a.out, t0 + t, j, scale(l) * v);
+        else __hip_atomic_store(&share[((long long)z * a.nt + t0 + t) * a.r + j], v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
     }
-    __syncthreads();
+  }
+  const int pad = a.out.rp - a.r;
+  if (z == 0 && blockIdx.y == 0)
+    for (int p = tid; p < pad * 16 * TF; p += 512)
+      if (sid[p / pad] >= 0) pad_low<T>(a.out, t0 + p / pad, a.r + p % pad);
+  if (splits == 1) return;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tid == 0) {
+    int* count = a.arrived + blockIdx.y * gridDim.x + blockIdx.x;
+    last = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == splits - 1;
+    if (last) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next run
+  }
+  __syncthreads();
+  if (!last) return;
+  for (int p = tid; p < 256 * JF * TF; p += 512) {
+    const int j = j0 + p % (16 * JF), t = p / (16 * JF), l = sid[t];
+    if (l < 0 || j >= a.r) continue;
+    R each[LOW_SPLITS], v = 0;
+#pragma unroll
+    for (int k = 0; k < LOW_SPLITS; ++k)  // all asked for before the first is waited for
+      each[k] = k < splits ? __hip_atomic_load(&share[((long long)k * a.nt + t0 + t) * a.r + j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : R(0);
+#pragma unroll
+    for (int k = 0; k < LOW_SPLITS; ++k) v += each[k];
+    put_low<T>(a.out, t0 + t, j, scale(l) * v);
   }
 }
 
-template <typename T> int run_low(const LowArgs& a, hipStream_t st) {
-  if (a.nt <= 256) {
-    k_low_dot<T><<<dim3(a.nt, cdiv(a.out.rp, 4)), 256, 0, st>>>(a);
+template <typename T> int run_low(const LowSets& sets, hipStream_t st) {
+  const LowArgs& a = sets.set[0];
+  const LowPlan p = low_plan(sizeof(T), a.nt, a.r, sets.sets);
+  if (p.tf == 0) {
+    k_low_dot<T><<<dim3(a.nt, cdiv(a.r, 4), sets.sets), 256, 0, st>>>(sets);
     return (int)hipGetLastError();
   }
-  const int jf = a.r <= 16 ? 1 : a.r <= 32 ? 2 : 4;
-  const int rows = max(a.r, a.out.rp);  // the zeros up to rp are written here too
-  if constexpr (sizeof(T) == 2)
-    if (a.nt >= 4096) {
-      const int tt = cdiv(a.nt, 32);
-      if (jf == 1) k_low_tile<T, 1, 2><<<dim3(tt, cdiv(rows, 16)), 512, 0, st>>>(a);
-      else if (jf == 2) k_low_tile<T, 2, 2><<<dim3(tt, cdiv(rows, 32)), 512, 0, st>>>(a);
-      else k_low_tile<T, 4, 2><<<dim3(tt, cdiv(rows, 64)), 512, 0, st>>>(a);
-      return (int)hipGetLastError();
-    }
-  const int tt = cdiv(a.nt, 16);
-  if (jf == 1) k_low_tile<T, 1, 1><<<dim3(tt, cdiv(rows, 16)), 512, 0, st>>>(a);
-  else if (jf == 2) k_low_tile<T, 2, 1><<<dim3(tt, cdiv(rows, 32)), 512, 0, st>>>(a);
-  else k_low_tile<T, 4, 1><<<dim3(tt, cdiv(rows, 64)), 512, 0, st>>>(a);
+  const dim3 grid(p.tiles, p.blocks, sets.sets * p.splits);
+  auto go = [&](auto kernel) { kernel<<<grid, 512, 0, st>>>(sets); };
+  if constexpr (sizeof(T) == 2) {
+    if (p.tf == 4) p.jf == 1 ? go(k_low_tile<T, 1, 4>) : p.jf == 2 ? go(k_low_tile<T, 2, 4>) : go(k_low_tile<T, 4, 4>);
+    else p.jf == 1 ? go(k_low_tile<T, 1, 1>) : p.jf == 2 ? go(k_low_tile<T, 2, 1>) : go(k_low_tile<T, 4, 1>);
+  } else {
+    p.jf == 1 ? go(k_low_tile<T, 1, 1>) : p.jf == 2 ? go(k_low_tile<T, 2, 1>) : go(k_low_tile<T, 4, 1>);
+  }
   return (int)hipGetLastError();
 }
 
 // ---------------------------------------------------------------- shared product
 // A workgroup owns BT tokens x BN features, WT x WN waves of (BT / WT) x (BN / WN).  The contraction goes in steps of 128
 // bytes of a row (whole cache lines: with 64-byte steps the same lines were asked for twice, 1.12 against 1.13 PFLOP/s at
-// 16384 x 4096 x 16384, and 1.26 against 1.38 where all of it lies in the L2) through two LDS buffers, each step in two halves of one fragment.  While a half is multiplied
+// 16384 x 4096 x 16384, and 1.26 against 1.38 where all of it lies in the L2) through a ring of LDS buffers, each step in two halves of one fragment.  While a half is multiplied
 // from registers the fragments of the next one are read from LDS; when a step's second half is in registers its buffer
-// takes the step after next.  So neither latency is waited for, and a step has one barrier.
+// takes a later step.  So neither latency is waited for, and a step has one barrier.  RING buffers: 2 where the tile is
+// large (the products of a step take as long as its loads), 4 where few workgroups share the chip and a step's
+// products are much shorter than the way from memory.
 //   DMA: rows begin at multiples of 16 bytes and the tile's rows lie within 2^30 bytes: memory to LDS directly.
 //        A chunk past the rows' end is fetched from past the buffer descriptor's end, which reads as zero.
 //   else: through registers, 16 bytes from any address, with zeros past the rows' end.
@@ -155,15 +181,16 @@ template <typename T> int run_low(const LowArgs& a, hipStream_t st) {
 // [step][features], and read through the transposing LDS read: a group of 16 lanes takes 4 steps x 16 features; the
 // 32-byte pair of such a read is displaced by the step's place in the instruction (16 steps of one instruction: 8 pairs).
 // The result has the tokens in its columns: a lane holds one token and 4 neighbouring features.
-template <typename T, int BT, int BN, int WT, int WN, bool NT, bool DMA>
+template <typename T, int BT, int BN, int WT, int WN, int RING, bool NT, bool DMA>
 __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
   typedef typename Num<T>::acc R;
   typedef typename Op<T>::vec V;
   constexpr int THREADS = 64 * WT * WN, E = Op<T>::E, BK = 2 * Op<T>::KS, STAGE = (BT + BN) * 128;
   constexpr int FT = BT / WT / 16, FN = BN / WN / 16;
   constexpr int JX = BT * 8 / THREADS, JW = BN * 8 / THREADS, CH = BN / E;  // CH: chunks of a [step][features] row
+  static_assert(DMA || RING == 2, "one step ahead in registers");
   static_assert(NT || sizeof(T) == 2, "the transposing LDS read is for 16-bit elements");
-  __shared__ __attribute__((aligned(1024))) char sm[2 * STAGE];
+  __shared__ __attribute__((aligned(1024))) char sm[RING * STAGE];
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, c16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wt = wave / WN, wn = wave % WN;
   // tiles of one XCD's workgroups: 4 tile rows of tokens at a time, tokens fastest, so that they share rows in its L2
@@ -208,7 +235,7 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
   auto stage_dma = [&](int s) {  // steps past the last one read as zero too
     const int k0 = place(s);
     const bool in = k0 + xc * E < a.C;
-    char* sx = &sm[(s & 1) * STAGE + wave * 1024];
+    char* sx = &sm[(s & (RING - 1)) * STAGE + wave * 1024];
 #pragma unroll
     for (int j = 0; j < JX; ++j) dma_buffer(x, xbytes, sx + j * THREADS * 16, in ? ox[j] : NOWHERE, k0 * (int)sizeof(T));
     char* sw = sx + BT * 128;
@@ -238,7 +265,7 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
     }
   };
   auto put = [&](int s) {
-    char* b = &sm[(s & 1) * STAGE + tid * 16];
+    char* b = &sm[(s & (RING - 1)) * STAGE + tid * 16];
 #pragma unroll
     for (int j = 0; j < JX; ++j) *(V*)(b + j * THREADS * 16) = gx[j];
 #pragma unroll
@@ -258,7 +285,7 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
     V x[FT], w[FN];
   };
   auto read = [&](Frag& r, int s, int half) {
-    const char* b = &sm[(s & 1) * STAGE];
+    const char* b = &sm[(s & (RING - 1)) * STAGE];
 #pragma unroll
     for (int i = 0; i < FN; ++i) {
       if constexpr (NT) {
@@ -290,6 +317,7 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
     __builtin_amdgcn_sched_barrier(0);
   };
   constexpr int LOADS = JX + JW, READS = FT + (NT ? FN : 2 * FN), PRODUCTS = FT * FN, EARLY = READS / 2;
+  static_assert(LOADS * (RING - 1) < 64, "the wait counts 6 bits");
   auto pace = [&](int loads) {
     // the reads early among the products, then the loads: left alone, the compiler puts the reads where the next half
     // waits for them
@@ -311,9 +339,9 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
   if (steps > 0) {
     Frag one, two;
     if constexpr (DMA) {
-      stage_dma(0);
-      stage_dma(1);
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
+#pragma unroll
+      for (int s = 0; s < RING; ++s) stage_dma(s);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS * (RING - 1)) : "memory");
     } else {
       fetch(0);
       put(0);
@@ -329,11 +357,12 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
       multiply(one);
       pace(0);
       // step s + 1 has arrived, and this step is in registers: its buffer is free
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      if constexpr (DMA) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS * (RING - 2)) : "memory");
+      else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       meet();
       read(one, s + 1, 0);
       if constexpr (DMA) {
-        stage_dma(s + 2);
+        stage_dma(s + RING);
       } else {
         put(s + 2);
         fetch(s + 3);
@@ -403,7 +432,7 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
   // accumulators a store would write 32 bytes of each of 16 rows)
   const R alpha = (R)a.alpha, beta = (R)a.beta;
   constexpr int ROW = FN * 16, PITCH = ROW + 16 / sizeof(R), OW = 16 / sizeof(T), LANES = ROW / OW;  // lanes of a row
-  static_assert(WT * WN * 16 * PITCH * sizeof(R) <= 2 * STAGE && 64 % LANES == 0, "staging");
+  static_assert(WT * WN * 16 * PITCH * sizeof(R) <= RING * STAGE && 64 % LANES == 0, "staging");
   __syncthreads();
   R* mine = (R*)sm + wave * 16 * PITCH;
   const int col = lane % LANES * OW, n = n0 + wn * ROW + col;
@@ -447,8 +476,8 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
   }
 }
 
-template <typename T, int BT, int BN, int WT, int WN, bool NT, bool DMA> void launch(const TileArgs& a, hipStream_t st) {
-  k_tile<T, BT, BN, WT, WN, NT, DMA><<<cdiv(a.T, BT) * cdiv(a.N, BN), 64 * WT * WN, 0, st>>>(a);
+template <typename T, int BT, int BN, int WT, int WN, int RING, bool NT, bool DMA> void launch(const TileArgs& a, hipStream_t st) {
+  k_tile<T, BT, BN, WT, WN, RING, NT, DMA><<<cdiv(a.T, BT) * cdiv(a.N, BN), 64 * WT * WN, 0, st>>>(a);
 }
 
 template <typename T, bool NT> int run_tile(const TileArgs& a, hipStream_t st) {
@@ -461,27 +490,45 @@ template <typename T, bool NT> int run_tile(const TileArgs& a, hipStream_t st) {
   auto tiles = [&](int b) { return (long long)cdiv(a.T, b) * cdiv(a.N, b); };
   if constexpr (sizeof(T) == 2)
     if (dma && tiles(256) >= 160) {
-      launch<T, 256, 256, 2, 4, NT, true>(a, st);
+      launch<T, 256, 256, 2, 4, 2, NT, true>(a, st);
       return (int)hipGetLastError();
     }
+  // RING 4 where it leaves every workgroup a CU (T x K x N, us with 2 and 4, 8 buffers: bf16 256 x 4096 x 4096 38.5, 22.4,
+  // 25.1; 1024 x 4096 x 4096 56.9, 49.1; with W's features contiguous 77.0, 84.5; fp64 1000 x 1000 x 2000 143, 175)
   if (tiles(128) >= 160 || sizeof(T) == 8) {
-    if (dma) launch<T, 128, 128, 2, 2, NT, true>(a, st);
-    else launch<T, 128, 128, 2, 2, NT, false>(a, st);
+    if (!dma) launch<T, 128, 128, 2, 2, 2, NT, false>(a, st);
+    else if (NT && sizeof(T) < 8 && tiles(128) <= 256) launch<T, 128, 128, 2, 2, 4, true, true>(a, st);
+    else launch<T, 128, 128, 2, 2, 2, NT, true>(a, st);
   } else {
-    if (dma) launch<T, 64, 64, 2, 2, NT, true>(a, st);
-    else launch<T, 64, 64, 2, 2, NT, false>(a, st);
+    if (!dma) launch<T, 64, 64, 2, 2, 2, NT, false>(a, st);
+    else if (tiles(64) <= 512) launch<T, 64, 64, 2, 2, 4, NT, true>(a, st);
+    else launch<T, 64, 64, 2, 2, 2, NT, true>(a, st);
   }
   return (int)hipGetLastError();
 }
 
 }  // namespace
 
-int lora_low(const LowArgs& a, hipStream_t st) {
-  switch (a.prec) {
-    case DPL_S: return run_low<float>(a, st);
-    case DPL_D: return run_low<double>(a, st);
-    case DPL_H: return run_low<_Float16>(a, st);
-    case DPL_B: return run_low<__bf16>(a, st);
+LowPlan low_plan(size_t size, int nt, int r, int sets) {
+  LowPlan p;
+  p.jf = r <= 16 ? 1 : r <= 32 ? 2 : 4;
+  p.blocks = cdiv(r, 16 * p.jf);
+  p.tf = nt <= 256 ? 0 : size == 2 && nt >= 1024 ? 4 : 1;
+  p.tiles = cdiv(nt, 16 * max(1, p.tf));
+  p.splits = p.tf == 0 ? 1 : max(1, min(LOW_SPLITS, 512 / (p.tiles * p.blocks * sets)));
+  return p;
+}
+
+int lora_low(const LowArgs* sets, int n, hipStream_t st) {
+  LowSets s;
+  s.sets = n;
+  for (int k = 0; k < n; ++k) s.set[k] = sets[k];
+  s.splits = low_plan(mid_bytes(sets[0].prec), sets[0].nt, sets[0].r, n).splits;
+  switch (sets[0].prec) {
+    case DPL_S: return run_low<float>(s, st);
+    case DPL_D: return run_low<double>(s, st);
+    case DPL_H: return run_low<_Float16>(s, st);
+    case DPL_B: return run_low<__bf16>(s, st);
   }
   return -1;
 }
