@@ -4,7 +4,7 @@
 
 // 16 bytes per lane from memory to LDS (lane i to lds + 16 i; lds is the same for the whole wave).  The buffer form reads
 // base[off + soff ..], zeros where that is past `bytes`.
-__device__ inline void dma_buffer(const void* base, int bytes, void* lds, unsigned off, int soff) {
+__device__ inline void dma_buffer(const void* base, unsigned bytes, void* lds, unsigned off, int soff) {
 #ifdef __HIP_DEVICE_COMPILE__
   __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void*)base, 0, bytes, 0x00020000),
                                            (__attribute__((address_space(3))) void*)lds, 16, off, soff, 0, 0);
@@ -61,22 +61,13 @@ static inline int low_pitch(int prec, int r) {
 static inline size_t mid_bytes(int prec) { return prec == DPL_D ? 8 : prec == DPL_S ? 4 : 2; }
 
 // out(t, j) = s_l sum_c x[t*ldx + c] F[(l*r + j)*ldf + c],  l = ids[t], for one or two sets of the same tokens.
-// share: splits * nt * r numbers of the working precision; arrived: tiles * blocks ints that are zero before the first
-// run and left so by every run (each set its own).
 struct LowArgs {
   const void *x, *F, *scale;
   const int* ids;
   long long ldx, ldf;
   int prec, nt, C, r, L;
   LowOut out;
-  void* share;
-  int* arrived;
 };
-constexpr int LOW_SPLITS = 8;
-struct LowPlan {
-  int jf, tf, tiles, blocks, splits;  // tf 0: one wave per token and j
-};
-LowPlan low_plan(size_t size, int nt, int r, int sets);
 int lora_low(const LowArgs* sets, int n, hipStream_t st);
 
 // y[t*ldy + n] = alpha (sum_c x[t*ldx + c] W(n, c) + sum_j low(t, j) F[(l*N + n)*ldf + j]) + beta y[t*ldy + n];
@@ -92,5 +83,5 @@ struct TileArgs {
 int lora_tile(const TileArgs& a, bool nt, hipStream_t st);
 
 // Gradient in h and b (lora_grad.hip).
-size_t lora_grad_ws(const LoraArgs& g, size_t* zero);
+size_t lora_grad_ws(const LoraArgs& g);
 int lora_grad_half(const LoraArgs& g, hipStream_t st);

@@ -214,20 +214,15 @@ template <typename T> int run_grad(const LoraArgs& g, hipStream_t st) {
 
 // T > 64: the low-rank vectors, then the shared product that adds the adapters' parts
 struct ForwardWs {
-  int* arrived;
-  char *hi, *lo, *share;
+  char *hi, *lo;
   int rp;
-  size_t zero, bytes;
+  size_t bytes;
   ForwardWs(const LoraArgs& g, void* ws) {
     rp = low_pitch(g.prec, g.r);
-    const size_t n = (size_t)g.T * rp, working = g.prec == DPL_D ? 8 : 4;
-    const LowPlan p = low_plan(mid_bytes(g.prec), g.T, g.r, 1);
+    const size_t n = (size_t)g.T * rp * mid_bytes(g.prec);
     Carve c{(char*)ws};
-    arrived = c.take<int>((size_t)p.tiles * p.blocks);  // first: zero before the first run
-    zero = c.used;
-    hi = c.take<char>(n * mid_bytes(g.prec));
-    lo = c.take<char>(n * mid_bytes(g.prec));
-    share = c.take<char>(p.splits > 1 ? n * p.splits * working : 0);
+    hi = c.take<char>(n);
+    lo = c.take<char>(n);
     bytes = c.used;
   }
 };
@@ -238,7 +233,7 @@ int forward(const LoraArgs& g, hipStream_t st) {
   if ((size_t)g.ws_bytes < w.bytes) return -2;
   const int* ids = (const int*)g.ids;
   if (g.L > 0) {
-    const LowArgs a{g.X, g.A, g.scale, ids, g.ldx, g.lda, g.prec, g.T, g.K, g.r, g.L, {w.hi, w.lo, nullptr, nullptr, nullptr, 0, w.rp}, w.share, w.arrived};
+    const LowArgs a{g.X, g.A, g.scale, ids, g.ldx, g.lda, g.prec, g.T, g.K, g.r, g.L, {w.hi, w.lo, nullptr, nullptr, nullptr, 0, w.rp}};
     const int rc = lora_low(&a, 1, st);
     if (rc) return rc;
   }
@@ -249,20 +244,13 @@ int forward(const LoraArgs& g, hipStream_t st) {
 
 DPL_API int dpl_lora_args_bytes() { return (int)sizeof(LoraArgs); }
 
-// zero: bytes at its beginning that are zero before the first run
-DPL_API long long dpl_lora_ws_bytes(const LoraArgs* g, int grad, long long* zero) {
-  size_t z = 0, bytes;
-  if (!grad) {
-    const ForwardWs w(*g, nullptr);
-    z = g->T <= 64 ? 0 : w.zero;
-    bytes = g->T <= 64 ? lora_few_ws(*g) : w.bytes;
-  } else if (g->prec == DPL_S || g->prec == DPL_D) {
-    bytes = g->prec == DPL_S ? PlainWs<float>(*g, nullptr).bytes : PlainWs<double>(*g, nullptr).bytes;
-  } else {
-    bytes = lora_grad_ws(*g, &z);
+DPL_API long long dpl_lora_ws_bytes(const LoraArgs* g, int grad) {
+  if (!grad) return (long long)(g->T <= 64 ? lora_few_ws(*g) : ForwardWs(*g, nullptr).bytes);
+  switch (g->prec) {
+    case DPL_S: return (long long)PlainWs<float>(*g, nullptr).bytes;
+    case DPL_D: return (long long)PlainWs<double>(*g, nullptr).bytes;
   }
-  *zero = (long long)z;
-  return (long long)bytes;
+  return (long long)lora_grad_ws(*g);
 }
 
 DPL_API int dpl_lora(const LoraArgs* g, hipStream_t st) { return g->T == 0 || g->N == 0 ? 0 : forward(*g, st); }

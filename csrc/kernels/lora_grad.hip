@@ -306,15 +306,15 @@ int window(const LoraArgs& g, int C) {
 }
 
 template <typename T> struct GradWs {
-  int *arrived[2], *off, *perm, *pos;
+  int *off, *perm, *pos;
   __bf16 *hi = nullptr, *lo = nullptr, *pthi = nullptr, *ptlo = nullptr, *sthi = nullptr, *stlo = nullptr;
   T *At = nullptr, *Bt = nullptr;
   int4* zeros;
-  float *share[2], *pa = nullptr, *pb = nullptr;
+  float *pa = nullptr, *pb = nullptr;
   bool dx, da, db;
   int rp, ldb, wa, wb;
   long long tp;
-  size_t zero, bytes;
+  size_t bytes;
   GradWs(const LoraArgs& g, void* ws) {
     dx = g.dX && g.K > 0 && g.T > 0;
     da = g.dA && g.K > 0 && g.L > 0;
@@ -324,15 +324,11 @@ template <typename T> struct GradWs {
     tp = (places(g) + 63) / 64 * 64 + 64;
     wa = window(g, g.K);
     wb = window(g, g.N);
-    const LowPlan p = low_plan(sizeof(T), g.T, g.r, 1);  // one set has the most splits
     Carve c{(char*)ws};
-    for (int k = 0; k < 2; ++k) arrived[k] = c.take<int>((size_t)p.tiles * p.blocks);  // first: zero before the first run
-    zero = c.used;
     zeros = c.take<int4>(1);
     off = c.take<int>(g.L + 1);
     perm = c.take<int>(places(g));
     pos = c.take<int>(g.T);
-    for (int k = 0; k < 2; ++k) share[k] = c.take<float>(p.splits > 1 ? (size_t)p.splits * g.T * rp : 0);
     if (dx) {
       hi = c.take<__bf16>((size_t)g.T * rp);
       lo = c.take<__bf16>((size_t)g.T * rp);
@@ -370,10 +366,10 @@ template <typename T> int run(const LoraArgs& g, hipStream_t st) {
     int n = 0;
     if (p)
       a[n++] = {g.dY, w.Bt, g.scale, ids, g.ldy, w.ldb, g.prec, g.T, g.N, g.r, g.L,
-                {w.dx ? w.hi : nullptr, w.lo, w.da ? w.pthi : nullptr, w.ptlo, w.pos, w.tp, w.rp}, w.share[0], w.arrived[0]};
+                {w.dx ? w.hi : nullptr, w.lo, w.da ? w.pthi : nullptr, w.ptlo, w.pos, w.tp, w.rp}};
     if (s)
       a[n++] = {g.X, g.A, g.scale, ids, g.ldx, g.lda, g.prec, g.T, g.K, g.r, g.L,
-                {nullptr, nullptr, w.sthi, w.stlo, w.pos, w.tp, g.r}, w.share[1], w.arrived[1]};
+                {nullptr, nullptr, w.sthi, w.stlo, w.pos, w.tp, g.r}};
     rc = lora_low(a, n, st);
   }
   if (!rc && w.dx)
@@ -401,13 +397,7 @@ template <typename T> int run(const LoraArgs& g, hipStream_t st) {
 
 }  // namespace
 
-size_t lora_grad_ws(const LoraArgs& g, size_t* zero) {
-  auto get = [&](auto w) {
-    *zero = w.zero;
-    return w.bytes;
-  };
-  return g.prec == DPL_H ? get(GradWs<_Float16>(g, nullptr)) : get(GradWs<__bf16>(g, nullptr));
-}
+size_t lora_grad_ws(const LoraArgs& g) { return g.prec == DPL_H ? GradWs<_Float16>(g, nullptr).bytes : GradWs<__bf16>(g, nullptr).bytes; }
 
 int lora_grad_half(const LoraArgs& g, hipStream_t st) {
   return g.prec == DPL_H ? run<_Float16>(g, st) : run<__bf16>(g, st);

@@ -8,7 +8,7 @@ namespace {
 // One or two sets of them (the gradient's P and S) in a launch.
 struct LowSets {
   LowArgs set[2];
-  int sets, splits;
+  int sets;
 };
 
 // One wave per (token, j): for few tokens, where the tokens of a workgroup's rows would mostly have adapters of their own.
@@ -34,134 +34,146 @@ template <typename T> __global__ __launch_bounds__(256) void k_low_dot(LowSets s
   if (lane == 0) put_low<T>(a.out, t, j, s);
 }
 
-// 16 TF tokens and 16 JF rows of the factors per workgroup, the contraction split over 8 waves and joined in LDS, one
-// adapter of these tokens at a time.  Many tokens per workgroup keep the factors' traffic down (each workgroup reads its
-// adapters' rows from the caches); `splits` workgroups then share the contraction, and the last one to arrive adds their
-// parts in order.
-template <typename T, int JF, int TF> __global__ __launch_bounds__(512) void k_low_tile(LowSets sets) {
+// 16 tokens and 16 JF rows of the factors per workgroup, the contraction split over the waves and joined in LDS, one adapter
+// of these tokens at a time.
+//   DMA (rows begin at multiples of 16 bytes): each wave has a ring of LDS buffers of its own for steps of 128 bytes, laid
+//     out as in k_tile and filled straight from memory; no barrier before the join.  (Fragments read where they are used,
+//     16 rows x 64 bytes a load, come out of the L2 at 37 GB/s per CU, whole lines at 130.)
+//   else: fragments from any address.
+template <typename T, int JF, bool DMA>
+__global__ __launch_bounds__(DMA && JF == 4 ? 256 : 512) void k_low_tile(LowSets sets) {
   typedef typename Num<T>::acc R;
   typedef typename Op<T>::vec V;
-  constexpr int E = Op<T>::E, KS = Op<T>::KS, U = JF * TF <= 2 ? 4 : 2;
-  __shared__ R red[8][16][16 * TF + 1];
-  __shared__ int sid[16 * TF], last;
-  const LowArgs& a = sets.set[blockIdx.z / sets.splits];
-  const int splits = sets.splits, z = blockIdx.z % splits;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, q = lane >> 4, c = lane & 15;
-  const int t0 = blockIdx.x * 16 * TF, j0 = blockIdx.y * 16 * JF;
+  constexpr int WAVES = DMA && JF == 4 ? 4 : 8, E = Op<T>::E, KS = Op<T>::KS;
+  constexpr int RING = JF == 1 ? 4 : 3, LOADS = 2 + 2 * JF, STAGE = LOADS * 1024;
+  constexpr int JOIN = WAVES * 16 * 17 * (int)sizeof(R);
+  __shared__ __attribute__((aligned(1024))) char sm[DMA ? WAVES * RING * STAGE : JOIN];
+  static_assert(!DMA || JOIN <= WAVES * RING * STAGE, "the join's place");
+  __shared__ int sid[16];
+  const LowArgs& a = sets.set[blockIdx.z];
+  const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, c = lane & 15;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int t0 = blockIdx.x * 16, j0 = blockIdx.y * 16 * JF;
+  R(*red)[16][17] = (R(*)[16][17])sm;
   int mine = -1;
-  if (lane < 16 * TF && t0 + lane < a.nt) mine = a.ids[t0 + lane];
+  if (lane < 16 && t0 + lane < a.nt) mine = a.ids[t0 + lane];
   if ((unsigned)mine >= (unsigned)a.L) mine = -1;
-  if (tid < 16 * TF) sid[tid] = mine;
-  const T* px[TF];
-#pragma unroll
-  for (int f = 0; f < TF; ++f) px[f] = (const T*)a.x + (long long)min(t0 + 16 * f + c, a.nt - 1) * a.ldx + q * E;
-  const int steps = (a.C + KS - 1) / KS, parts = 8 * splits, part = 8 * z + w;
-  const int s0 = (int)((long long)steps * part / parts), s1 = (int)((long long)steps * (part + 1) / parts), whole = min(s1, a.C / KS);
-  auto scale = [&](int l) { return a.scale ? ((const R*)a.scale)[l] : R(1); };
-  R* share = (R*)a.share;
+  if (tid < 16) {
+    sid[tid] = mine;
+    if (mine >= 0 && blockIdx.y == 0)
+      for (int j = a.r; j < a.out.rp; ++j) pad_low<T>(a.out, t0 + tid, j);
+  }
   unsigned long long todo = __ballot(mine >= 0);
   while (todo) {
     const int l = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
     todo &= ~__ballot(mine == l);
-    const T* pf[JF];
+    const T *x = (const T*)a.x + (long long)t0 * a.ldx, *f = (const T*)a.F + ((long long)l * a.r + j0) * a.ldf;
+    const int rt = min(16, a.nt - t0), rj = min(16 * JF, a.r - j0);
+    typename Op<T>::out acc[JF];
 #pragma unroll
-    for (int f = 0; f < JF; ++f)
-      pf[f] = (const T*)a.F + ((long long)l * a.r + min(j0 + 16 * f + c, a.r - 1)) * a.ldf + q * E;
-    typename Op<T>::out acc[JF][TF];
+    for (int i = 0; i < JF; ++i) acc[i] = typename Op<T>::out{R(0), R(0), R(0), R(0)};
+    if constexpr (DMA) {
+      constexpr int BK = 2 * KS;
+      constexpr unsigned NOWHERE = 0x80000000u;
+      const int steps = (a.C + BK - 1) / BK, s0 = steps * w / WAVES, s1 = steps * (w + 1) / WAVES;
+      const int row = lane >> 3, chunk = (lane & 7) ^ row;
+      const unsigned xbytes = (unsigned)(((rt - 1) * a.ldx + a.C) * (long long)sizeof(T));
+      const unsigned fbytes = (unsigned)(((rj - 1) * a.ldf + a.C) * (long long)sizeof(T));
+      unsigned ox[2], of[2 * JF];
 #pragma unroll
-    for (int i = 0; i < JF; ++i)
+      for (int k = 0; k < 2; ++k) ox[k] = (unsigned)(min(row + 8 * k, rt - 1) * (int)a.ldx + chunk * E) * sizeof(T);
 #pragma unroll
-      for (int f = 0; f < TF; ++f) acc[i][f] = typename Op<T>::out{R(0), R(0), R(0), R(0)};
-    int s = s0;
-    for (; s + U <= whole; s += U) {
-      V x[U][TF], f[U][JF];
+      for (int k = 0; k < 2 * JF; ++k) of[k] = (unsigned)(min(row + 8 * k, rj - 1) * (int)a.ldf + chunk * E) * sizeof(T);
+      char* ring = sm + w * RING * STAGE;
+      auto stage = [&](int s) {
+        char* b = ring + (s - s0) % RING * STAGE;
+        const bool in = s < s1 && s * BK + chunk * E < a.C;
+        const int at = s < s1 ? s * BK * (int)sizeof(T) : 0;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
+        for (int k = 0; k < 2; ++k) dma_buffer(x, xbytes, b + k * 1024, in ? ox[k] : NOWHERE, at);
 #pragma unroll
-        for (int i = 0; i < TF; ++i) x[u][i] = load_vec(px[i] + (long long)(s + u) * KS);
+        for (int k = 0; k < 2 * JF; ++k) dma_buffer(f, fbytes, b + 2048 + k * 1024, in ? of[k] : NOWHERE, at);
+      };
 #pragma unroll
-        for (int i = 0; i < JF; ++i) f[u][i] = load_vec(pf[i] + (long long)(s + u) * KS);
+      for (int k = 0; k < RING - 1; ++k) stage(s0 + k);
+      const int fr = c * 128 + ((q ^ (c & 7)) << 4);
+      for (int s = s0; s < s1; ++s) {
+        // this step has arrived, and the one before has been read: its buffer is filled next
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS * (RING - 2)) : "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        stage(s + RING - 1);
+        const char* b = ring + (s - s0) % RING * STAGE;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const V v = *(const V*)(b + (fr ^ (64 * half)));
+#pragma unroll
+          for (int i = 0; i < JF; ++i) acc[i] = Op<T>::mma(*(const V*)(b + 2048 + (fr ^ (64 * half)) + i * 2048), v, acc[i]);
+        }
       }
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    } else {
+      constexpr int U = JF <= 2 ? 4 : 2;
+      const T *px = x + min(c, rt - 1) * a.ldx + q * E, *pf[JF];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int i = 0; i < JF; ++i) pf[i] = f + min(16 * i + c, rj - 1) * a.ldf + q * E;
+      const int steps = (a.C + KS - 1) / KS, s0 = steps * w / WAVES, s1 = steps * (w + 1) / WAVES, whole = min(s1, a.C / KS);
+      int s = s0;
+      for (; s + U <= whole; s += U) {
+        V xv[U], fv[U][JF];
 #pragma unroll
-        for (int i = 0; i < JF; ++i)
+        for (int u = 0; u < U; ++u) {
+          xv[u] = load_vec(px + (long long)(s + u) * KS);
 #pragma unroll
-          for (int k = 0; k < TF; ++k) acc[i][k] = Op<T>::mma(f[u][i], x[u][k], acc[i][k]);
-    }
-    for (; s < s1; ++s) {
-      const int left = a.C - s * KS - q * E;
-      V x[TF];
+          for (int i = 0; i < JF; ++i) fv[u][i] = load_vec(pf[i] + (long long)(s + u) * KS);
+        }
 #pragma unroll
-      for (int k = 0; k < TF; ++k) x[k] = load_part(px[k] + (long long)s * KS, left);
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int i = 0; i < JF; ++i) {
-        const V f = load_part(pf[i] + (long long)s * KS, left);
+          for (int i = 0; i < JF; ++i) acc[i] = Op<T>::mma(fv[u][i], xv[u], acc[i]);
+      }
+      for (; s < s1; ++s) {
+        const int left = a.C - s * KS - q * E;
+        const V xv = load_part(px + (long long)s * KS, left);
 #pragma unroll
-        for (int k = 0; k < TF; ++k) acc[i][k] = Op<T>::mma(f, x[k], acc[i][k]);
+        for (int i = 0; i < JF; ++i) acc[i] = Op<T>::mma(load_part(pf[i] + (long long)s * KS, left), xv, acc[i]);
       }
     }
+    const R scale = a.scale ? ((const R*)a.scale)[l] : R(1);
 #pragma unroll
     for (int i = 0; i < JF; ++i) {
-      __syncthreads();
+      __syncthreads();  // the waves are through with their buffers, or with the join before
 #pragma unroll
-      for (int k = 0; k < TF; ++k)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) red[w][out_row<T>(lane, v)][16 * k + c] = acc[i][k][v];
+      for (int v = 0; v < 4; ++v) red[w][out_row<T>(lane, v)][c] = acc[i][v];
       __syncthreads();
-      for (int p = tid; p < 256 * TF; p += 512) {
-        const int j = j0 + 16 * i + p % 16, t = p / 16;
-        if (sid[t] != l || j >= a.r) continue;
+      const int j = j0 + 16 * i + tid % 16, t = tid / 16;
+      if (t < 16 && sid[t] == l && j < a.r) {
         R v = 0;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v += red[k][p % 16][t];
-        if (splits == 1) put_low<T>(a.out, t0 + t, j, scale(l) * v);
-        else __hip_atomic_store(&share[((long long)z * a.nt + t0 + t) * a.r + j], v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        for (int k = 0; k < WAVES; ++k) v += red[k][tid % 16][t];
+        put_low<T>(a.out, t0 + t, j, scale * v);
       }
     }
-  }
-  const int pad = a.out.rp - a.r;
-  if (z == 0 && blockIdx.y == 0)
-    for (int p = tid; p < pad * 16 * TF; p += 512)
-      if (sid[p / pad] >= 0) pad_low<T>(a.out, t0 + p / pad, a.r + p % pad);
-  if (splits == 1) return;
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  if (tid == 0) {
-    int* count = a.arrived + blockIdx.y * gridDim.x + blockIdx.x;
-    last = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == splits - 1;
-    if (last) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next run
-  }
-  __syncthreads();
-  if (!last) return;
-  for (int p = tid; p < 256 * JF * TF; p += 512) {
-    const int j = j0 + p % (16 * JF), t = p / (16 * JF), l = sid[t];
-    if (l < 0 || j >= a.r) continue;
-    R each[LOW_SPLITS], v = 0;
-#pragma unroll
-    for (int k = 0; k < LOW_SPLITS; ++k)  // all asked for before the first is waited for
-      each[k] = k < splits ? __hip_atomic_load(&share[((long long)k * a.nt + t0 + t) * a.r + j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : R(0);
-#pragma unroll
-    for (int k = 0; k < LOW_SPLITS; ++k) v += each[k];
-    put_low<T>(a.out, t0 + t, j, scale(l) * v);
+    __syncthreads();
   }
 }
 
 template <typename T> int run_low(const LowSets& sets, hipStream_t st) {
   const LowArgs& a = sets.set[0];
-  const LowPlan p = low_plan(sizeof(T), a.nt, a.r, sets.sets);
-  if (p.tf == 0) {
+  if (a.nt <= 256) {
     k_low_dot<T><<<dim3(a.nt, cdiv(a.r, 4), sets.sets), 256, 0, st>>>(sets);
     return (int)hipGetLastError();
   }
-  const dim3 grid(p.tiles, p.blocks, sets.sets * p.splits);
-  auto go = [&](auto kernel) { kernel<<<grid, 512, 0, st>>>(sets); };
-  if constexpr (sizeof(T) == 2) {
-    if (p.tf == 4) p.jf == 1 ? go(k_low_tile<T, 1, 4>) : p.jf == 2 ? go(k_low_tile<T, 2, 4>) : go(k_low_tile<T, 4, 4>);
-    else p.jf == 1 ? go(k_low_tile<T, 1, 1>) : p.jf == 2 ? go(k_low_tile<T, 2, 1>) : go(k_low_tile<T, 4, 1>);
-  } else {
-    p.jf == 1 ? go(k_low_tile<T, 1, 1>) : p.jf == 2 ? go(k_low_tile<T, 2, 1>) : go(k_low_tile<T, 4, 1>);
+  bool dma = true;
+  for (int k = 0; k < sets.sets; ++k) {
+    const LowArgs& s = sets.set[k];
+    auto wide = [](const void* q, long long ld) { return ((uintptr_t)q | (uintptr_t)(ld * sizeof(T))) % 16 == 0 && ld * (long long)sizeof(T) * 64 < (1ll << 30); };
+    dma = dma && wide(s.x, s.ldx) && wide(s.F, s.ldf) && s.C % Op<T>::E == 0;
   }
+  const int jf = a.r <= 16 ? 1 : a.r <= 32 ? 2 : 4;
+  const dim3 grid(cdiv(a.nt, 16), cdiv(a.r, 16 * jf), sets.sets);
+  auto go = [&](auto kernel, int threads) { kernel<<<grid, threads, 0, st>>>(sets); };
+  if (dma) jf == 1 ? go(k_low_tile<T, 1, true>, 512) : jf == 2 ? go(k_low_tile<T, 2, true>, 512) : go(k_low_tile<T, 4, true>, 256);
+  else jf == 1 ? go(k_low_tile<T, 1, false>, 512) : jf == 2 ? go(k_low_tile<T, 2, false>, 512) : go(k_low_tile<T, 4, false>, 512);
   return (int)hipGetLastError();
 }
 
@@ -226,7 +238,8 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
     }
   }
   const int xbytes = DMA ? (int)(((rt - 1) * a.ldx + a.C) * (long long)sizeof(T)) : 0;
-  const int wbytes = DMA && NT ? (int)(((rn - 1) * a.ldw + a.C) * (long long)sizeof(T)) : 0;
+  const unsigned pitch = (unsigned)a.ldw * sizeof(T);
+  const unsigned wbytes = DMA ? (unsigned)((NT ? (rn - 1) * a.ldw + a.C : (a.C - 1) * a.ldw + rn) * (long long)sizeof(T)) : 0;
   const int steps = (a.C + BK - 1) / BK;
   // each XCD begins at another eighth of the contraction: beginning together they all ask for the same rows of W at
   // once (1.13 -> 1.20 PFLOP/s at 16384 x 4096 x 16384, 1.26 -> 1.35 at 8192^3)
@@ -244,10 +257,8 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
       for (int j = 0; j < JW; ++j) dma_buffer(W, wbytes, sw + j * THREADS * 16, in ? ow[j] : NOWHERE, k0 * (int)sizeof(T));
     } else {
       // the descriptor ends with W's last row
-      const int pitch = (int)a.ldw * (int)sizeof(T);
-      const int bytes = __builtin_amdgcn_readfirstlane(max(0, max(0, min(BK, a.C - k0)) * pitch - (pitch - rn * (int)sizeof(T))));
 #pragma unroll
-      for (int j = 0; j < JW; ++j) dma_buffer(W + (long long)k0 * a.ldw, bytes, sw + j * THREADS * 16, ow[j], 0);
+      for (int j = 0; j < JW; ++j) dma_buffer(W, wbytes, sw + j * THREADS * 16, ow[j] + (unsigned)k0 * pitch, 0);
     }
   };
   auto fetch = [&](int s) {
@@ -485,20 +496,22 @@ template <typename T, bool NT> int run_tile(const TileArgs& a, hipStream_t st) {
   auto wide = [&](const void* p, long long ld, int rows) {
     return ((uintptr_t)p | (uintptr_t)(ld * size)) % 16 == 0 && ld * size * rows < span;
   };
-  // W with its features contiguous also needs whole chunks of them within a row
-  const bool dma = wide(a.x, a.ldx, 256) && wide(a.W, a.ldw, 256) && a.C % Op<T>::E == 0 && (NT || a.N % 8 == 0);
+  // W with its features contiguous also needs whole chunks of them within a row, and offsets in 32 bits over all of it
+  const bool dma = wide(a.x, a.ldx, 256) && wide(a.W, a.ldw, 256) && a.C % Op<T>::E == 0 &&
+                   (NT || (a.N % 8 == 0 && (a.C + 1024ll) * a.ldw * size < (1ll << 32)));
   auto tiles = [&](int b) { return (long long)cdiv(a.T, b) * cdiv(a.N, b); };
   if constexpr (sizeof(T) == 2)
     if (dma && tiles(256) >= 160) {
       launch<T, 256, 256, 2, 4, 2, NT, true>(a, st);
       return (int)hipGetLastError();
     }
-  // RING 4 where it leaves every workgroup a CU (T x K x N, us with 2 and 4, 8 buffers: bf16 256 x 4096 x 4096 38.5, 22.4,
-  // 25.1; 1024 x 4096 x 4096 56.9, 49.1; with W's features contiguous 77.0, 84.5; fp64 1000 x 1000 x 2000 143, 175)
+  // RING 4 where it leaves every workgroup a CU, and 8 waves on a 128 tile (T x K x N, us with 2 and 4 buffers: bf16
+  // 256 x 4096 x 4096 38.5, 22.4; 1024 x 4096 x 4096 56.9, 49.1 with 4 waves, 42.1 with 8; with W's features contiguous
+  // 67.9 with 2 and 4 waves, 61.4 with 4 and 8; fp64 1000 x 1000 x 2000 143, 175, with 2 and 8 waves 137)
   if (tiles(128) >= 160 || sizeof(T) == 8) {
     if (!dma) launch<T, 128, 128, 2, 2, 2, NT, false>(a, st);
-    else if (NT && sizeof(T) < 8 && tiles(128) <= 256) launch<T, 128, 128, 2, 2, 4, true, true>(a, st);
-    else launch<T, 128, 128, 2, 2, 2, NT, true>(a, st);
+    else if (sizeof(T) < 8 && tiles(128) <= 256) launch<T, 128, 128, 2, 4, 4, NT, true>(a, st);
+    else launch<T, 128, 128, 2, 4, 2, NT, true>(a, st);
   } else {
     if (!dma) launch<T, 64, 64, 2, 2, 2, NT, false>(a, st);
     else if (tiles(64) <= 512) launch<T, 64, 64, 2, 2, 4, NT, true>(a, st);
@@ -509,21 +522,10 @@ template <typename T, bool NT> int run_tile(const TileArgs& a, hipStream_t st) {
 
 }  // namespace
 
-LowPlan low_plan(size_t size, int nt, int r, int sets) {
-  LowPlan p;
-  p.jf = r <= 16 ? 1 : r <= 32 ? 2 : 4;
-  p.blocks = cdiv(r, 16 * p.jf);
-  p.tf = nt <= 256 ? 0 : size == 2 && nt >= 1024 ? 4 : 1;
-  p.tiles = cdiv(nt, 16 * max(1, p.tf));
-  p.splits = p.tf == 0 ? 1 : max(1, min(LOW_SPLITS, 512 / (p.tiles * p.blocks * sets)));
-  return p;
-}
-
 int lora_low(const LowArgs* sets, int n, hipStream_t st) {
-  LowSets s;
+  LowSets s{};
   s.sets = n;
   for (int k = 0; k < n; ++k) s.set[k] = sets[k];
-  s.splits = low_plan(mid_bytes(sets[0].prec), sets[0].nt, sets[0].r, n).splits;
   switch (sets[0].prec) {
     case DPL_S: return run_low<float>(s, st);
     case DPL_D: return run_low<double>(s, st);

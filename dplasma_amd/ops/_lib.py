@@ -137,7 +137,7 @@ _SIGS = {
     # products whose matrix depends on the column (lora.hip, moe.hip): argument record, [gradient,] stream
     "dpl_lora": [c_vp, c_vp],
     "dpl_lora_grad": [c_vp, c_vp],
-    "dpl_lora_ws_bytes": [c_vp, c_int, c_vp],
+    "dpl_lora_ws_bytes": [c_vp, c_int],
     "dpl_lora_args_bytes": [],
     "dpl_moe": [c_vp, c_vp],
     "dpl_moe_ws_bytes": [c_vp, c_vp],

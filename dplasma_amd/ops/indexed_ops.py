@@ -82,9 +82,8 @@ def lora_call(device, alpha, W, X, A, B, ids, scale, beta=0.0, Y=None, dY=None, 
     else:
         a.Y = pointer(Y)
     keep = [W, X, A, B, ids, scale, Y, dY, dX, dA, dB]
-    zero = _ll()
-    size = lib.dpl_lora_ws_bytes(ctypes.byref(a), int(grad), ctypes.byref(zero))
-    return _Call(device, "dpl_lora_grad" if grad else "dpl_lora", a, size, keep, zero.value)
+    return _Call(device, "dpl_lora_grad" if grad else "dpl_lora", a, lib.dpl_lora_ws_bytes(ctypes.byref(a), int(grad)),
+                 keep)
 
 
 def moe_call(device, topk, norm, G, W1, W2, alpha, X, beta, Y):
