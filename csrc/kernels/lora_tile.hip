@@ -34,31 +34,31 @@ template <typename T> __global__ __launch_bounds__(256) void k_low_dot(LowSets s
   if (lane == 0) put_low<T>(a.out, t, j, s);
 }
 
-// 16 tokens and 16 JF rows of the factors per workgroup, the contraction split over the waves and joined in LDS, one adapter
+// 16 TF tokens and 16 JF rows of the factors per workgroup, the contraction split over the waves and joined in LDS, one adapter
 // of these tokens at a time.
 //   DMA (rows begin at multiples of 16 bytes): each wave has a ring of LDS buffers of its own for steps of 128 bytes, laid
 //     out as in k_tile and filled straight from memory; no barrier before the join.  (Fragments read where they are used,
 //     16 rows x 64 bytes a load, come out of the L2 at 37 GB/s per CU, whole lines at 130.)
 //   else: fragments from any address.
-template <typename T, int JF, bool DMA>
-__global__ __launch_bounds__(DMA && JF == 4 ? 256 : 512) void k_low_tile(LowSets sets) {
+template <typename T, int JF, int TF, bool DMA>
+__global__ __launch_bounds__(DMA && JF * TF >= 4 ? 256 : 512) void k_low_tile(LowSets sets) {
   typedef typename Num<T>::acc R;
   typedef typename Op<T>::vec V;
-  constexpr int WAVES = DMA && JF == 4 ? 4 : 8, E = Op<T>::E, KS = Op<T>::KS;
-  constexpr int RING = JF == 1 ? 4 : 3, LOADS = 2 + 2 * JF, STAGE = LOADS * 1024;
-  constexpr int JOIN = WAVES * 16 * 17 * (int)sizeof(R);
+  constexpr int WAVES = DMA && JF * TF >= 4 ? 4 : 8, E = Op<T>::E, KS = Op<T>::KS;
+  constexpr int RING = JF == 4 || JF + TF == 3 ? 3 : 4, LOADS = 2 * TF + 2 * JF, STAGE = LOADS * 1024;
+  constexpr int JOIN = WAVES * 16 * (16 * TF + 1) * (int)sizeof(R);
   __shared__ __attribute__((aligned(1024))) char sm[DMA ? WAVES * RING * STAGE : JOIN];
   static_assert(!DMA || JOIN <= WAVES * RING * STAGE, "the join's place");
-  __shared__ int sid[16];
+  __shared__ int sid[16 * TF];
   const LowArgs& a = sets.set[blockIdx.z];
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, c = lane & 15;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int t0 = blockIdx.x * 16, j0 = blockIdx.y * 16 * JF;
-  R(*red)[16][17] = (R(*)[16][17])sm;
+  const int t0 = blockIdx.x * 16 * TF, j0 = blockIdx.y * 16 * JF;
+  R(*red)[16][16 * TF + 1] = (R(*)[16][16 * TF + 1])sm;
   int mine = -1;
-  if (lane < 16 && t0 + lane < a.nt) mine = a.ids[t0 + lane];
+  if (lane < 16 * TF && t0 + lane < a.nt) mine = a.ids[t0 + lane];
   if ((unsigned)mine >= (unsigned)a.L) mine = -1;
-  if (tid < 16) {
+  if (tid < 16 * TF) {
     sid[tid] = mine;
     if (mine >= 0 && blockIdx.y == 0)
       for (int j = a.r; j < a.out.rp; ++j) pad_low<T>(a.out, t0 + tid, j);
@@ -68,10 +68,12 @@ __global__ __launch_bounds__(DMA && JF == 4 ? 256 : 512) void k_low_tile(LowSets
     const int l = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
     todo &= ~__ballot(mine == l);
     const T *x = (const T*)a.x + (long long)t0 * a.ldx, *f = (const T*)a.F + ((long long)l * a.r + j0) * a.ldf;
-    const int rt = min(16, a.nt - t0), rj = min(16 * JF, a.r - j0);
-    typename Op<T>::out acc[JF];
+    const int rt = min(16 * TF, a.nt - t0), rj = min(16 * JF, a.r - j0);
+    typename Op<T>::out acc[JF][TF];
 #pragma unroll
-    for (int i = 0; i < JF; ++i) acc[i] = typename Op<T>::out{R(0), R(0), R(0), R(0)};
+    for (int i = 0; i < JF; ++i)
+#pragma unroll
+      for (int k = 0; k < TF; ++k) acc[i][k] = typename Op<T>::out{R(0), R(0), R(0), R(0)};
     if constexpr (DMA) {
       constexpr int BK = 2 * KS;
       constexpr unsigned NOWHERE = 0x80000000u;
@@ -79,9 +81,9 @@ __global__ __launch_bounds__(DMA && JF == 4 ? 256 : 512) void k_low_tile(LowSets
       const int row = lane >> 3, chunk = (lane & 7) ^ row;
       const unsigned xbytes = (unsigned)(((rt - 1) * a.ldx + a.C) * (long long)sizeof(T));
       const unsigned fbytes = (unsigned)(((rj - 1) * a.ldf + a.C) * (long long)sizeof(T));
-      unsigned ox[2], of[2 * JF];
+      unsigned ox[2 * TF], of[2 * JF];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) ox[k] = (unsigned)(min(row + 8 * k, rt - 1) * (int)a.ldx + chunk * E) * sizeof(T);
+      for (int k = 0; k < 2 * TF; ++k) ox[k] = (unsigned)(min(row + 8 * k, rt - 1) * (int)a.ldx + chunk * E) * sizeof(T);
 #pragma unroll
       for (int k = 0; k < 2 * JF; ++k) of[k] = (unsigned)(min(row + 8 * k, rj - 1) * (int)a.ldf + chunk * E) * sizeof(T);
       char* ring = sm + w * RING * STAGE;
@@ -90,9 +92,9 @@ __global__ __launch_bounds__(DMA && JF == 4 ? 256 : 512) void k_low_tile(LowSets
         const bool in = s < s1 && s * BK + chunk * E < a.C;
         const int at = s < s1 ? s * BK * (int)sizeof(T) : 0;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) dma_buffer(x, xbytes, b + k * 1024, in ? ox[k] : NOWHERE, at);
+        for (int k = 0; k < 2 * TF; ++k) dma_buffer(x, xbytes, b + k * 1024, in ? ox[k] : NOWHERE, at);
 #pragma unroll
-        for (int k = 0; k < 2 * JF; ++k) dma_buffer(f, fbytes, b + 2048 + k * 1024, in ? of[k] : NOWHERE, at);
+        for (int k = 0; k < 2 * JF; ++k) dma_buffer(f, fbytes, b + TF * 2048 + k * 1024, in ? of[k] : NOWHERE, at);
       };
 #pragma unroll
       for (int k = 0; k < RING - 1; ++k) stage(s0 + k);
@@ -105,13 +107,20 @@ __global__ __launch_bounds__(DMA && JF == 4 ? 256 : 512) void k_low_tile(LowSets
         const char* b = ring + (s - s0) % RING * STAGE;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          const V v = *(const V*)(b + (fr ^ (64 * half)));
+          V v[TF];
 #pragma unroll
-          for (int i = 0; i < JF; ++i) acc[i] = Op<T>::mma(*(const V*)(b + 2048 + (fr ^ (64 * half)) + i * 2048), v, acc[i]);
+          for (int k = 0; k < TF; ++k) v[k] = *(const V*)(b + (fr ^ (64 * half)) + k * 2048);
+#pragma unroll
+          for (int i = 0; i < JF; ++i) {
+            const V fv = *(const V*)(b + TF * 2048 + (fr ^ (64 * half)) + i * 2048);
+#pragma unroll
+            for (int k = 0; k < TF; ++k) acc[i][k] = Op<T>::mma(fv, v[k], acc[i][k]);
+          }
         }
       }
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     } else {
+      static_assert(TF == 1, "one fragment of tokens");
       constexpr int U = JF <= 2 ? 4 : 2;
       const T *px = x + min(c, rt - 1) * a.ldx + q * E, *pf[JF];
 #pragma unroll
@@ -129,13 +138,13 @@ __global__ __launch_bounds__(DMA && JF == 4 ? 256 : 512) void k_low_tile(LowSets
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int i = 0; i < JF; ++i) acc[i] = Op<T>::mma(fv[u][i], xv[u], acc[i]);
+          for (int i = 0; i < JF; ++i) acc[i][0] = Op<T>::mma(fv[u][i], xv[u], acc[i][0]);
       }
       for (; s < s1; ++s) {
         const int left = a.C - s * KS - q * E;
         const V xv = load_part(px + (long long)s * KS, left);
 #pragma unroll
-        for (int i = 0; i < JF; ++i) acc[i] = Op<T>::mma(load_part(pf[i] + (long long)s * KS, left), xv, acc[i]);
+        for (int i = 0; i < JF; ++i) acc[i][0] = Op<T>::mma(load_part(pf[i] + (long long)s * KS, left), xv, acc[i][0]);
       }
     }
     const R scale = a.scale ? ((const R*)a.scale)[l] : R(1);
@@ -143,13 +152,16 @@ __global__ __launch_bounds__(DMA && JF == 4 ? 256 : 512) void k_low_tile(LowSets
     for (int i = 0; i < JF; ++i) {
       __syncthreads();  // the waves are through with their buffers, or with the join before
 #pragma unroll
-      for (int v = 0; v < 4; ++v) red[w][out_row<T>(lane, v)][c] = acc[i][v];
+      for (int k = 0; k < TF; ++k)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) red[w][out_row<T>(lane, v)][16 * k + c] = acc[i][k][v];
       __syncthreads();
-      const int j = j0 + 16 * i + tid % 16, t = tid / 16;
-      if (t < 16 && sid[t] == l && j < a.r) {
+      for (int p = tid; p < 256 * TF; p += 64 * WAVES) {
+        const int j = j0 + 16 * i + p % 16, t = p / 16;
+        if (sid[t] != l || j >= a.r) continue;
         R v = 0;
 #pragma unroll
-        for (int k = 0; k < WAVES; ++k) v += red[k][tid % 16][t];
+        for (int k = 0; k < WAVES; ++k) v += red[k][p % 16][t];
         put_low<T>(a.out, t0 + t, j, scale * v);
       }
     }
@@ -170,10 +182,17 @@ template <typename T> int run_low(const LowSets& sets, hipStream_t st) {
     dma = dma && wide(s.x, s.ldx) && wide(s.F, s.ldf) && s.C % Op<T>::E == 0;
   }
   const int jf = a.r <= 16 ? 1 : a.r <= 32 ? 2 : 4;
-  const dim3 grid(cdiv(a.nt, 16), cdiv(a.r, 16 * jf), sets.sets);
+  // two fragments of tokens, which halves the factors' traffic, where that leaves a workgroup for every CU
+  const int tf = dma && sizeof(T) == 2 && a.nt >= 8192 ? 2 : 1;
+  const dim3 grid(cdiv(a.nt, 16 * tf), cdiv(a.r, 16 * jf), sets.sets);
   auto go = [&](auto kernel, int threads) { kernel<<<grid, threads, 0, st>>>(sets); };
-  if (dma) jf == 1 ? go(k_low_tile<T, 1, true>, 512) : jf == 2 ? go(k_low_tile<T, 2, true>, 512) : go(k_low_tile<T, 4, true>, 256);
-  else jf == 1 ? go(k_low_tile<T, 1, false>, 512) : jf == 2 ? go(k_low_tile<T, 2, false>, 512) : go(k_low_tile<T, 4, false>, 512);
+  if constexpr (sizeof(T) == 2)
+    if (tf == 2) {
+      jf == 1 ? go(k_low_tile<T, 1, 2, true>, 512) : jf == 2 ? go(k_low_tile<T, 2, 2, true>, 256) : go(k_low_tile<T, 4, 2, true>, 256);
+      return (int)hipGetLastError();
+    }
+  if (dma) jf == 1 ? go(k_low_tile<T, 1, 1, true>, 512) : jf == 2 ? go(k_low_tile<T, 2, 1, true>, 512) : go(k_low_tile<T, 4, 1, true>, 256);
+  else jf == 1 ? go(k_low_tile<T, 1, 1, false>, 512) : jf == 2 ? go(k_low_tile<T, 2, 1, false>, 512) : go(k_low_tile<T, 4, 1, false>, 512);
   return (int)hipGetLastError();
 }
 
