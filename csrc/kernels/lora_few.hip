@@ -30,13 +30,119 @@ __global__ __launch_bounds__(256) void k_few_low(const T* __restrict__ x, long l
   if (lane == 0) S[(long long)t * r + j] = s;
 }
 
+template <int N> struct Int {
+  static constexpr int value = N;
+};
+
+// One token: rows of W and of its adapter's A against x, one wave per row with its lanes along K (whole lines).  8 waves
+// take the workgroup's 8 M features (M: 1 or 2) while 8 others make the low-rank vector, every workgroup for itself: A
+// then comes from the caches, and that is less than a second launch and the way of the vector through memory, as long
+// as a workgroup has not much more of A to read than of W and one wave's loads of W are enough to fill the memory:
+//   2048 x 2048: r 16 5.9 us against 8.9 with two launches, r 64 9.5 us both ways
+//   4096 x 4096: r 16 10.6 against 12.9, r 64 14.4 against 13.4;  4096 x 16384, r 8: 46.6 against 31.7
+constexpr int ONE_R = 32, ONE_N = 4096;
+
+template <typename T>
+__global__ __launch_bounds__(1024) void k_one(const T* __restrict__ x, const T* __restrict__ W, long long ldw,
+                                              const T* __restrict__ A, long long lda, const T* __restrict__ B,
+                                              long long ldb, const int* __restrict__ ids,
+                                              const typename Num<T>::acc* __restrict__ scale, int K, int N, int r, int L,
+                                              int M, typename Num<T>::acc alpha, typename Num<T>::acc beta,
+                                              T* __restrict__ y) {
+  typedef typename Num<T>::acc R;
+  typedef typename Op<T>::vec V;
+  constexpr int E = Op<T>::E, STEP = 64 * E;
+  __shared__ R low[ONE_R];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int l = L > 0 ? ids[0] : -1;
+  const bool has = (unsigned)l < (unsigned)L;
+  // the rows p[0 .. ROWS) against x, in every lane
+  auto dots = [&](auto rows, const T* const* p, R* out) {
+    constexpr int ROWS = decltype(rows)::value;
+    R s[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) s[i] = 0;
+    int k = lane * E, left = K / STEP;
+    auto run = [&](auto width) {
+      constexpr int U = decltype(width)::value;
+      V a[U][ROWS], b[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) a[u][i] = load_vec(p[i] + k + u * STEP);
+        b[u] = load_vec(x + k + u * STEP);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+          for (int e = 0; e < E; ++e) s[i] = fma((R)a[u][i][e], (R)b[u][e], s[i]);
+      k += U * STEP;
+      left -= U;
+    };
+    while (left >= 4) run(Int<4>());
+    if (left >= 2) run(Int<2>());
+    if (left) run(Int<1>());
+    if (k < K) {
+      const V b = load_part(x + k, K - k);
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        const V a = load_part(p[i] + k, K - k);
+#pragma unroll
+        for (int e = 0; e < E; ++e) s[i] = fma((R)a[e], (R)b[e], s[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      for (int o = 32; o; o >>= 1) s[i] += __shfl_xor(s[i], o);
+      out[i] = s[i];
+    }
+  };
+  if (w >= 8) {
+    if (has) {
+      const T* a = A + (long long)l * r * lda;
+      const R f = scale ? scale[l] : R(1);
+      for (int j = w - 8; j < r; j += 16) {
+        const T* p[2] = {a + j * lda, a + min(j + 8, r - 1) * lda};
+        R v[2];
+        dots(Int<2>(), p, v);
+        if (lane == 0) {
+          low[j] = f * v[0];
+          if (j + 8 < r) low[j + 8] = f * v[1];
+        }
+      }
+    }
+    __syncthreads();
+    return;
+  }
+  const int n = blockIdx.x * M * 8 + w, n2 = M > 1 ? n + 8 : N;
+  R v[2] = {0, 0}, f[2] = {0, 0};
+  const T* p[2] = {W + min(n, N - 1) * ldw, W + min(n2, N - 1) * ldw};
+  if (n2 < N) dots(Int<2>(), p, v);
+  else if (n < N) dots(Int<1>(), p, v);
+  if (has && lane < r) {
+    if (n < N) f[0] = widen(B[((long long)l * N + n) * ldb + lane]);
+    if (n2 < N) f[1] = widen(B[((long long)l * N + n2) * ldb + lane]);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int at = i ? n2 : n;
+    R u = has && lane < r ? low[lane] * f[i] : R(0);
+    for (int o = 32; o; o >>= 1) u += __shfl_xor(u, o);
+    if (lane == 0 && at < N) {
+      R z = alpha == R(0) ? R(0) : alpha * (v[i] + u);
+      if (beta != R(0)) z += beta * widen(y[at]);
+      y[at] = (T)z;
+    }
+  }
+}
+
 // 16 NF output features per workgroup, the contraction split over 8 waves and joined in LDS; G groups of 16 tokens.
 // W's fragments go straight from memory to the matrix instruction (each element is used by one wave once); x comes
 // from the caches.  A wave has one batch of fragments under way after another, as large as the registers of one
 // workgroup per CU allow; what the adapters' parts need is asked for before and beside them.
-template <int N> struct Int {
-  static constexpr int value = N;
-};
 constexpr int S_MAX = 64;  // r up to which the low-rank vectors go through LDS
 
 template <typename T, int G, int NF>
@@ -182,6 +288,12 @@ template <typename T> int run(const LoraArgs& g, hipStream_t st) {
   R* S = (R*)g.ws;
   const T *X = (const T*)g.X, *A = (const T*)g.A, *B = (const T*)g.B, *W = (const T*)g.W;
   const int* ids = (const int*)g.ids;
+  if (g.T == 1 && g.r <= ONE_R && g.N <= ONE_N) {
+    const int M = g.N <= 8 * 256 ? 1 : 2;  // a workgroup per CU at most
+    k_one<T><<<cdiv(g.N, 8 * M), 1024, 0, st>>>(X, W, g.ldw, A, g.lda, B, g.ldb, ids, (const R*)g.scale, g.K, g.N, g.r, g.L, M,
+                                               (R)g.alpha, (R)g.beta, (T*)g.Y);
+    return (int)hipGetLastError();
+  }
   if (g.L > 0) k_few_low<T><<<dim3(g.T, cdiv(g.r, 4)), 256, 0, st>>>(X, g.ldx, A, g.lda, ids, (const R*)g.scale, g.K, g.r, g.L, S);
   // two fragments of features for a fragment of tokens where that leaves a workgroup for every CU: x is read half as
   // often, and what a CU can have under way is the bound (48 tokens, 4096 x 8192: 43.4 us with one, 30.6 with two; 48

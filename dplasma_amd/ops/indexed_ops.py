@@ -44,7 +44,8 @@ class _Call:
 
     def __init__(self, device, name, args, ws_bytes, keep, zero=0):
         """zero: bytes at the workspace's beginning that start as zeros (every run leaves them so)."""
-        self.name, self.args, self.device = name, args, device
+        self.name, self.args = name, args
+        self.index = torch.cuda.current_device() if device.index is None else device.index
         self.keep = keep  # tensors whose addresses the record holds
         self.ws = torch.empty(max(256, ws_bytes), dtype=torch.uint8, device=device)
         self.ws[:zero].zero_()
@@ -57,10 +58,13 @@ class _Call:
         self.fn, self.ref = getattr(_lib.load(), name), ctypes.byref(args)
 
     def __call__(self):
-        s = torch.cuda.current_stream(self.device)
-        if s.cuda_stream != self.home and not torch.cuda.is_current_stream_capturing():
+        s = torch.cuda.current_stream(self.index)
+        stream = s.cuda_stream
+        if stream != self.home and not torch.cuda.is_current_stream_capturing():
             self.ws.record_stream(s)
-        _lib.check(self.fn(self.ref, s.cuda_stream), self.name)
+        rc = self.fn(self.ref, stream)
+        if rc:
+            _lib.check(rc, self.name)
 
 
 def _checked(lib, name, record):

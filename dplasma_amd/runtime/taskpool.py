@@ -103,6 +103,17 @@ class Taskpool:
     def run(self, ctx=None):
         from ..utils import trace
         ctx = ctx or self.ctx
+        if len(self.tasks) == 1 and self.tasks[0].stream == "caller" and ctx is not None and ctx.is_gpu \
+                and not trace.enabled(ctx):
+            # one task on the caller's stream and nobody watching: nothing to order (on a product of one token the
+            # spans and the schedule below are half of the host's time, 14 us against 9)
+            self._t_run = time.perf_counter()
+            if torch.cuda.current_device() == ctx.device.index:
+                self.tasks[0].fn()
+            else:
+                with torch.cuda.device(ctx.device):
+                    self.tasks[0].fn()
+            return
         with trace.span(ctx, self.name, "taskpool", args={"tasks": len(self.tasks), "gflop": self.flops / 1e9}):
             self._run(ctx)
 

@@ -136,6 +136,11 @@ def _null():
     yield
 
 
+def enabled(ctx) -> bool:
+    """Whether a span of this context is recorded or printed."""
+    return TRACE_KERNELS or getattr(ctx, "profiling", None) is not None
+
+
 def span(ctx, name, cat="task", stream=None, args=None, gpu=True):
     """Span on ctx's tracer if profiling is on (cheap no-op otherwise)."""
     tr = getattr(ctx, "profiling", None) if ctx is not None else None
