@@ -197,13 +197,15 @@ template <typename T> int run_low(const LowSets& sets, hipStream_t st) {
 }
 
 // ---------------------------------------------------------------- shared product
-// A workgroup owns BT tokens x BN features, WT x WN waves of (BT / WT) x (BN / WN).  The contraction goes in steps of 128
+// A workgroup owns B tokens x B features, WT x WN waves of (B / WT) x (B / WN).  The contraction goes in steps of 128
 // bytes of a row (whole cache lines: with 64-byte steps the same lines were asked for twice, 1.12 against 1.13 PFLOP/s at
 // 16384 x 4096 x 16384, and 1.26 against 1.38 where all of it lies in the L2) through a ring of LDS buffers, each step in two halves of one fragment.  While a half is multiplied
-// from registers the fragments of the next one are read from LDS; when a step's second half is in registers its buffer
-// takes a later step.  So neither latency is waited for, and a step has one barrier.  RING buffers: 2 where the tile is
-// large (the products of a step take as long as its loads), 4 where few workgroups share the chip and a step's
-// products are much shorter than the way from memory.
+// from registers the fragments of the next one are read from LDS; when a step's second half is in registers its buffers
+// take a later step.  So neither latency is waited for, and a step has one barrier.  SLOTS buffers, each of one
+// operand's part of a step, X and W in turn: 4 (a step ahead) where several workgroups share a CU, 8 where few share the
+// chip and a step's products are much shorter than the way from memory, and 5, all of the LDS, with the largest tile: X
+// then has two steps to arrive (16384 x 4096 x 16384: 1.28 PFLOP/s with 4, 1.37 with 5; W two steps: the same; W's
+// features contiguous: 1.16 and 1.17).
 //   DMA: rows begin at multiples of 16 bytes and the tile's rows lie within 2^30 bytes: memory to LDS directly.
 //        A chunk past the rows' end is fetched from past the buffer descriptor's end, which reads as zero.
 //   else: through registers, 16 bytes from any address, with zeros past the rows' end.
@@ -212,27 +214,27 @@ template <typename T> int run_low(const LowSets& sets, hipStream_t st) {
 // [step][features], and read through the transposing LDS read: a group of 16 lanes takes 4 steps x 16 features; the
 // 32-byte pair of such a read is displaced by the step's place in the instruction (16 steps of one instruction: 8 pairs).
 // The result has the tokens in its columns: a lane holds one token and 4 neighbouring features.
-template <typename T, int BT, int BN, int WT, int WN, int RING, bool NT, bool DMA>
+template <typename T, int B, int WT, int WN, int SLOTS, bool NT, bool DMA>
 __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
   typedef typename Num<T>::acc R;
   typedef typename Op<T>::vec V;
-  constexpr int THREADS = 64 * WT * WN, E = Op<T>::E, BK = 2 * Op<T>::KS, STAGE = (BT + BN) * 128;
-  constexpr int FT = BT / WT / 16, FN = BN / WN / 16;
-  constexpr int JX = BT * 8 / THREADS, JW = BN * 8 / THREADS, CH = BN / E;  // CH: chunks of a [step][features] row
-  static_assert(DMA || RING == 2, "one step ahead in registers");
+  constexpr int THREADS = 64 * WT * WN, E = Op<T>::E, BK = 2 * Op<T>::KS, SLOT = B * 128;
+  constexpr int FT = B / WT / 16, FN = B / WN / 16;
+  constexpr int J = B * 8 / THREADS, CH = B / E;  // CH: chunks of a [step][features] row
+  static_assert(SLOTS >= 4 && (DMA || SLOTS == 4), "without DMA the step after next is in registers");
   static_assert(NT || sizeof(T) == 2, "the transposing LDS read is for 16-bit elements");
-  __shared__ __attribute__((aligned(1024))) char sm[RING * STAGE];
+  __shared__ __attribute__((aligned(1024))) char sm[SLOTS * SLOT];
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, c16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wt = wave / WN, wn = wave % WN;
   // tiles of one XCD's workgroups: 4 tile rows of tokens at a time, tokens fastest, so that they share rows in its L2
   // (4 / 8 / 16 rows: 1.12 / 1.03 / 1.04 PFLOP/s at 16384 x 4096 x 16384)
-  const int tt = (a.T + BT - 1) / BT, tn = (a.N + BN - 1) / BN;
+  const int tt = (a.T + B - 1) / B, tn = (a.N + B - 1) / B;
   const int id = xcd_remap(blockIdx.x, tt * tn);
   const int group = id / (4 * tn), in = id % (4 * tn), gs = min(4, tt - group * 4);
-  const int t0 = (group * 4 + in % gs) * BT, n0 = in / gs * BN;
+  const int t0 = (group * 4 + in % gs) * B, n0 = in / gs * B;
   const T* x = (const T*)a.x + (long long)t0 * a.ldx;
   const T* W = (const T*)a.W + (NT ? (long long)n0 * a.ldw : n0);
-  const int rt = min(BT, a.T - t0), rn = min(BN, a.N - n0);
+  const int rt = min(B, a.T - t0), rn = min(B, a.N - n0);
 
   // staging: chunk id tid + j * THREADS of either operand
   const int xr = tid >> 3, xc = (tid & 7) ^ (xr & 7);
@@ -240,14 +242,14 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
   const int wmask = CH / 2 - 1;
   auto turn = [&](int step) { return ((step & 3) + 4 * ((step >> 3) & 1)) & wmask; };
   auto wchunk = [&](int row, int pc) { return 2 * ((pc >> 1) ^ turn(row)) + (pc & 1); };
-  V gx[DMA ? 1 : JX], gw[DMA ? 1 : JW];
-  unsigned ox[DMA ? JX : 1], ow[DMA ? JW : 1];
+  V gx[DMA ? 1 : J], gw[DMA ? 1 : J];
+  unsigned ox[DMA ? J : 1], ow[DMA ? J : 1];
   constexpr unsigned NOWHERE = 0x80000000u;
   if constexpr (DMA) {
 #pragma unroll
-    for (int j = 0; j < JX; ++j) ox[j] = (unsigned)(min(xr + j * (THREADS / 8), rt - 1) * (int)a.ldx + xc * E) * sizeof(T);
+    for (int j = 0; j < J; ++j) ox[j] = (unsigned)(min(xr + j * (THREADS / 8), rt - 1) * (int)a.ldx + xc * E) * sizeof(T);
 #pragma unroll
-    for (int j = 0; j < JW; ++j) {
+    for (int j = 0; j < J; ++j) {
       if (NT) {
         ow[j] = (unsigned)(min(wr + j * (THREADS / 8), rn - 1) * (int)a.ldw + xc * E) * sizeof(T);
       } else {
@@ -264,28 +266,30 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
   // once (1.13 -> 1.20 PFLOP/s at 16384 x 4096 x 16384, 1.26 -> 1.35 at 8192^3)
   const int turned = steps / 8 * (blockIdx.x & 7);
   auto place = [&](int s) { return (s >= steps ? s : s + turned >= steps ? s + turned - steps : s + turned) * BK; };
-  auto stage_dma = [&](int s) {  // steps past the last one read as zero too
+  auto stage_x = [&](int s, char* slot) {  // steps past the last one read as zero
     const int k0 = place(s);
     const bool in = k0 + xc * E < a.C;
-    char* sx = &sm[(s & (RING - 1)) * STAGE + wave * 1024];
 #pragma unroll
-    for (int j = 0; j < JX; ++j) dma_buffer(x, xbytes, sx + j * THREADS * 16, in ? ox[j] : NOWHERE, k0 * (int)sizeof(T));
-    char* sw = sx + BT * 128;
+    for (int j = 0; j < J; ++j) dma_buffer(x, xbytes, slot + j * THREADS * 16, in ? ox[j] : NOWHERE, k0 * (int)sizeof(T));
+  };
+  auto stage_w = [&](int s, char* slot) {
+    const int k0 = place(s);
     if (NT) {
+      const bool in = k0 + xc * E < a.C;
 #pragma unroll
-      for (int j = 0; j < JW; ++j) dma_buffer(W, wbytes, sw + j * THREADS * 16, in ? ow[j] : NOWHERE, k0 * (int)sizeof(T));
+      for (int j = 0; j < J; ++j) dma_buffer(W, wbytes, slot + j * THREADS * 16, in ? ow[j] : NOWHERE, k0 * (int)sizeof(T));
     } else {
       // the descriptor ends with W's last row
 #pragma unroll
-      for (int j = 0; j < JW; ++j) dma_buffer(W, wbytes, sw + j * THREADS * 16, ow[j] + (unsigned)k0 * pitch, 0);
+      for (int j = 0; j < J; ++j) dma_buffer(W, wbytes, slot + j * THREADS * 16, ow[j] + (unsigned)k0 * pitch, 0);
     }
   };
   auto fetch = [&](int s) {
     const int k0 = place(s), left = a.C - k0 - xc * E;
 #pragma unroll
-    for (int j = 0; j < JX; ++j) gx[j] = load_part(x + (long long)min(xr + j * (THREADS / 8), rt - 1) * a.ldx + k0 + xc * E, left);
+    for (int j = 0; j < J; ++j) gx[j] = load_part(x + (long long)min(xr + j * (THREADS / 8), rt - 1) * a.ldx + k0 + xc * E, left);
 #pragma unroll
-    for (int j = 0; j < JW; ++j) {
+    for (int j = 0; j < J; ++j) {
       if (NT) {
         gw[j] = load_part(W + (long long)min(wr + j * (THREADS / 8), rn - 1) * a.ldw + k0 + xc * E, left);
       } else {
@@ -294,12 +298,11 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
       }
     }
   };
-  auto put = [&](int s) {
-    char* b = &sm[(s & (RING - 1)) * STAGE + tid * 16];
+  auto put = [&](char* sx, char* sw) {
 #pragma unroll
-    for (int j = 0; j < JX; ++j) *(V*)(b + j * THREADS * 16) = gx[j];
+    for (int j = 0; j < J; ++j) *(V*)(sx + tid * 16 + j * THREADS * 16) = gx[j];
 #pragma unroll
-    for (int j = 0; j < JW; ++j) *(V*)(b + BT * 128 + j * THREADS * 16) = gw[j];
+    for (int j = 0; j < J; ++j) *(V*)(sw + tid * 16 + j * THREADS * 16) = gw[j];
   };
 
   typename Op<T>::out acc[FN][FT];
@@ -308,31 +311,30 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
 #pragma unroll
     for (int f = 0; f < FT; ++f) acc[i][f] = typename Op<T>::out{R(0), R(0), R(0), R(0)};
   const int fx = (wt * FT * 16 + c16) * 128 + ((q ^ (c16 & 7)) << 4);  // ^ 64: the second half of the step
-  const int fw = BT * 128 + (wn * FN * 16 + c16) * 128 + ((q ^ (c16 & 7)) << 4);
-  const int ftr = BT * 128 + (8 * q + (c16 >> 2)) * (BN * 2) + (c16 & 3) * 8;  // + pair * 32
+  const int fw = (wn * FN * 16 + c16) * 128 + ((q ^ (c16 & 7)) << 4);
+  const int ftr = (8 * q + (c16 >> 2)) * (B * 2) + (c16 & 3) * 8;  // + pair * 32
   const int tw = ((c16 >> 2) + 4 * (q & 1)) & wmask;
   struct Frag {
     V x[FT], w[FN];
   };
-  auto read = [&](Frag& r, int s, int half) {
-    const char* b = &sm[(s & (RING - 1)) * STAGE];
+  auto read = [&](Frag& r, const char* sx, const char* sw, int half) {
 #pragma unroll
     for (int i = 0; i < FN; ++i) {
       if constexpr (NT) {
-        r.w[i] = *(const V*)(b + (fw ^ (64 * half)) + i * 2048);
+        r.w[i] = *(const V*)(sw + (fw ^ (64 * half)) + i * 2048);
       } else {
         typedef short s4_t __attribute__((ext_vector_type(4)));
         typedef short s8_t __attribute__((ext_vector_type(8)));
         typedef __attribute__((address_space(3))) s4_t* lp;
-        const char* p = b + ftr + (((wn * FN + i) ^ tw) << 5) + half * 32 * BN * 2;
+        const char* p = sw + ftr + (((wn * FN + i) ^ tw) << 5) + half * 32 * B * 2;
         const s4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p));
-        const s4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p + 4 * BN * 2));
+        const s4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p + 4 * B * 2));
         const s8_t both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         r.w[i] = __builtin_bit_cast(V, both);
       }
     }
 #pragma unroll
-    for (int f = 0; f < FT; ++f) r.x[f] = *(const V*)(b + (fx ^ (64 * half)) + f * 2048);
+    for (int f = 0; f < FT; ++f) r.x[f] = *(const V*)(sx + (fx ^ (64 * half)) + f * 2048);
   };
   auto multiply = [&](const Frag& r) {
 #pragma unroll
@@ -346,8 +348,8 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
-  constexpr int LOADS = JX + JW, READS = FT + (NT ? FN : 2 * FN), PRODUCTS = FT * FN, EARLY = READS / 2;
-  static_assert(LOADS * (RING - 1) < 64, "the wait counts 6 bits");
+  constexpr int LOADS = 2 * J, READS = FT + (NT ? FN : 2 * FN), PRODUCTS = FT * FN, EARLY = READS / 2;
+  static_assert(J * (SLOTS - 2) < 64, "the wait counts 6 bits");
   auto pace = [&](int loads) {
     // the reads early among the products, then the loads: left alone, the compiler puts the reads where the next half
     // waits for them
@@ -368,34 +370,44 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
   };
   if (steps > 0) {
     Frag one, two;
+    int sx = 0, sw = SLOT;  // where this step's parts are
+    auto next = [&](int slot) { return slot + 2 * SLOT >= SLOTS * SLOT ? slot + (2 - SLOTS) * SLOT : slot + 2 * SLOT; };
+    char* own = sm + wave * 1024;  // where this wave's loads go within a buffer
     if constexpr (DMA) {
 #pragma unroll
-      for (int s = 0; s < RING; ++s) stage_dma(s);
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS * (RING - 1)) : "memory");
+      for (int k = 0; k < SLOTS; ++k) k & 1 ? stage_w(k / 2, own + k * SLOT) : stage_x(k / 2, own + k * SLOT);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(J * (SLOTS - 2)) : "memory");
     } else {
       fetch(0);
-      put(0);
+      put(sm, sm + SLOT);
       fetch(1);
-      put(1);
+      put(sm + 2 * SLOT, sm + 3 * SLOT);
       fetch(2);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
     meet();
-    read(one, 0, 0);
+    read(one, sm + sx, sm + sw, 0);
     for (int s = 0; s < steps; ++s) {
-      read(two, s, 1);
+      read(two, sm + sx, sm + sw, 1);
       multiply(one);
       pace(0);
-      // step s + 1 has arrived, and this step is in registers: its buffer is free
-      if constexpr (DMA) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS * (RING - 2)) : "memory");
+      // step s + 1 has arrived, and this step is in registers: its buffers are free
+      if constexpr (DMA) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(J * (SLOTS - 4)) : "memory");
       else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       meet();
-      read(one, s + 1, 0);
-      if constexpr (DMA) {
-        stage_dma(s + RING);
-      } else {
-        put(s + 2);
+      const int fx0 = sx, fw0 = sw;
+      sx = next(sx);
+      sw = next(sw);
+      read(one, sm + sx, sm + sw, 0);
+      if constexpr (!DMA) {
+        put(sm + fx0, sm + fw0);
         fetch(s + 3);
+      } else if constexpr (SLOTS & 1) {  // an odd number: the operands change places
+        stage_w(s + SLOTS / 2, own + fx0);
+        stage_x(s + SLOTS / 2 + 1, own + fw0);
+      } else {
+        stage_x(s + SLOTS / 2, own + fx0);
+        stage_w(s + SLOTS / 2, own + fw0);
       }
       multiply(two);
       pace(1);
@@ -462,7 +474,7 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
   // accumulators a store would write 32 bytes of each of 16 rows)
   const R alpha = (R)a.alpha, beta = (R)a.beta;
   constexpr int ROW = FN * 16, PITCH = ROW + 16 / sizeof(R), OW = 16 / sizeof(T), LANES = ROW / OW;  // lanes of a row
-  static_assert(WT * WN * 16 * PITCH * sizeof(R) <= RING * STAGE && 64 % LANES == 0, "staging");
+  static_assert(WT * WN * 16 * PITCH * sizeof(R) <= SLOTS * SLOT && 64 % LANES == 0, "staging");
   __syncthreads();
   R* mine = (R*)sm + wave * 16 * PITCH;
   const int col = lane % LANES * OW, n = n0 + wn * ROW + col;
@@ -506,8 +518,8 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
   }
 }
 
-template <typename T, int BT, int BN, int WT, int WN, int RING, bool NT, bool DMA> void launch(const TileArgs& a, hipStream_t st) {
-  k_tile<T, BT, BN, WT, WN, RING, NT, DMA><<<cdiv(a.T, BT) * cdiv(a.N, BN), 64 * WT * WN, 0, st>>>(a);
+template <typename T, int B, int WT, int WN, int SLOTS, bool NT, bool DMA> void launch(const TileArgs& a, hipStream_t st) {
+  k_tile<T, B, WT, WN, SLOTS, NT, DMA><<<cdiv(a.T, B) * cdiv(a.N, B), 64 * WT * WN, 0, st>>>(a);
 }
 
 template <typename T, bool NT> int run_tile(const TileArgs& a, hipStream_t st) {
@@ -521,20 +533,20 @@ template <typename T, bool NT> int run_tile(const TileArgs& a, hipStream_t st) {
   auto tiles = [&](int b) { return (long long)cdiv(a.T, b) * cdiv(a.N, b); };
   if constexpr (sizeof(T) == 2)
     if (dma && tiles(256) >= 160) {
-      launch<T, 256, 256, 2, 4, 2, NT, true>(a, st);
+      launch<T, 256, 2, 4, 5, NT, true>(a, st);
       return (int)hipGetLastError();
     }
-  // RING 4 where it leaves every workgroup a CU, and 8 waves on a 128 tile (T x K x N, us with 2 and 4 buffers: bf16
+  // 8 buffers where they leave every workgroup a CU, and 8 waves on a 128 tile (T x K x N, us with 4 and 8 buffers: bf16
   // 256 x 4096 x 4096 38.5, 22.4; 1024 x 4096 x 4096 56.9, 49.1 with 4 waves, 42.1 with 8; with W's features contiguous
-  // 67.9 with 2 and 4 waves, 61.4 with 4 and 8; fp64 1000 x 1000 x 2000 143, 175, with 2 and 8 waves 137)
+  // 67.9 with 4 and 4 waves, 61.4 with 8 and 8; fp64 1000 x 1000 x 2000 143, 175, with 4 and 8 waves 137)
   if (tiles(128) >= 160 || sizeof(T) == 8) {
-    if (!dma) launch<T, 128, 128, 2, 2, 2, NT, false>(a, st);
-    else if (sizeof(T) < 8 && tiles(128) <= 256) launch<T, 128, 128, 2, 4, 4, NT, true>(a, st);
-    else launch<T, 128, 128, 2, 4, 2, NT, true>(a, st);
+    if (!dma) launch<T, 128, 2, sizeof(T) == 8 ? 4 : 2, 4, NT, false>(a, st);
+    else if (sizeof(T) < 8 && tiles(128) <= 256) launch<T, 128, 2, 4, 8, NT, true>(a, st);
+    else launch<T, 128, 2, 4, 4, NT, true>(a, st);
   } else {
-    if (!dma) launch<T, 64, 64, 2, 2, 2, NT, false>(a, st);
-    else if (tiles(64) <= 512) launch<T, 64, 64, 2, 2, 4, NT, true>(a, st);
-    else launch<T, 64, 64, 2, 2, 2, NT, true>(a, st);
+    if (!dma) launch<T, 64, 2, 2, 4, NT, false>(a, st);
+    else if (tiles(64) <= 512) launch<T, 64, 2, 2, 8, NT, true>(a, st);
+    else launch<T, 64, 2, 2, 4, NT, true>(a, st);
   }
   return (int)hipGetLastError();
 }
