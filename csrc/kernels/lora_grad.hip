@@ -217,12 +217,10 @@ template <typename T, int JF, bool DMA> __global__ __launch_bounds__(256, 1) voi
       }
 #pragma unroll
       for (int f = 0; f < FN; ++f) {
-        typedef short s4_t __attribute__((ext_vector_type(4)));
         typedef short s8_t __attribute__((ext_vector_type(8)));
-        typedef __attribute__((address_space(3))) s4_t* lp;
         const char* p = b + ftr + (((wave * FN + f) ^ tw) << 5) + kk * 32 * COLS * 2;
-        const s4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p));
-        const s4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p + 4 * COLS * 2));
+        const s4_t v0 = read_turned(p);
+        const s4_t v1 = read_turned(p + 4 * COLS * 2);
         const s8_t both = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
         MidOp<T> x;
         x.set(__builtin_bit_cast(V, both));

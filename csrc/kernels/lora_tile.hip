@@ -323,12 +323,10 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
       if constexpr (NT) {
         r.w[i] = *(const V*)(sw + (fw ^ (64 * half)) + i * 2048);
       } else {
-        typedef short s4_t __attribute__((ext_vector_type(4)));
         typedef short s8_t __attribute__((ext_vector_type(8)));
-        typedef __attribute__((address_space(3))) s4_t* lp;
         const char* p = sw + ftr + (((wn * FN + i) ^ tw) << 5) + half * 32 * B * 2;
-        const s4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p));
-        const s4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p + 4 * B * 2));
+        const s4_t lo = read_turned(p);
+        const s4_t hi = read_turned(p + 4 * B * 2);
         const s8_t both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         r.w[i] = __builtin_bit_cast(V, both);
       }
