@@ -63,6 +63,36 @@ def test_lora_grad(ctx, case):
         assert torch.equal(one, two)
 
 
+# sizes on both sides of every choice between the kernels' variants: features per workgroup and launches of one token, two
+# fragments of features for few tokens, tiles of 64, 128 and 256 with each number of buffers, through registers and
+# directly to LDS, one and two fragments of tokens of the low-rank vectors
+VARIANTS = [
+    (B, 1, 300, 2500, 20, 2, "one", 0), (H, 1, 256, 4097, 8, 2, "one", 0), (D, 1, 130, 2100, 32, 2, "one", 0),
+    (S, 1, 64, 40, 33, 2, "one", 0), (B, 20, 72, 8200, 16, 3, "tokens", 0), (H, 40, 40, 8193, 70, 4, "tokens", 0),
+    (B, 64, 64, 8192, 8, 9, "tokens", 0), (S, 50, 72, 8200, 8, 3, "tokens", 0), (D, 64, 40, 520, 8, 3, "tokens", 0),
+    (B, 1536, 72, 1664, 16, 4, "runs", 0), (H, 1536, 1664, 72, 8, 5, "tokens", 8), (B, 1700, 1704, 1704, 16, 3, "runs", 0),
+    (H, 2100, 72, 2100, 32, 6, "tokens", 0), (B, 2100, 2104, 72, 16, 2, "runs", 0), (S, 1700, 136, 1704, 8, 3, "runs", 0),
+    (S, 2100, 68, 2100, 16, 3, "tokens", 0), (B, 1700, 201, 1703, 12, 5, "runs", 0), (H, 1700, 1703, 201, 12, 5, "tokens", 1),
+    (D, 130, 101, 201, 9, 5, "tokens", 0), (D, 300, 256, 512, 16, 2, "runs", 0), (B, 4100, 200, 2600, 16, 5, "runs", 0),
+    (H, 4100, 2600, 136, 24, 7, "tokens", 8), (B, 8200, 136, 1304, 64, 9, "tokens", 0), (H, 8200, 1304, 136, 20, 4, "runs", 0),
+    (B, 8200, 264, 72, 8, 300, "tokens", 0), (H, 8200, 64, 64, 130, 1, "one", 0),
+]
+
+
+@pytest.mark.parametrize("case", VARIANTS, ids=str)
+def test_lora_variants(ctx, case):
+    c = lora(*case)
+    y = c.forward(ctx, -0.5, 2.0)
+    within(y[:, :c.N], *c.plain(-0.5, 2.0), "y")
+    assert torch.equal(y[:, c.N:], c.y[:, c.N:]) and torch.equal(y, c.forward(ctx, -0.5, 2.0))
+    first = c.backward(ctx)
+    for got, (want, bound), what in zip((first[0][:, :c.K], *first[1:]), c.plain_backward(), ("dx", "da", "db")):
+        within(got, want, bound, what)
+    assert (first[0][:, c.K:] == 7).all()
+    for one, two in zip(first, c.backward(ctx)):
+        assert torch.equal(one, two)
+
+
 @pytest.mark.parametrize("case", [(B, 300, 512, 256, 16, 3, "runs", 0), (H, 40, 256, 300, 8, 5, "tokens", 0)], ids=str)
 def test_lora_grad_parts_alone(ctx, case):
     c = lora(*case)
@@ -198,7 +228,12 @@ def test_lora_nothing_to_do(ctx):
 MOE = [(B, 1, 64, 32, 4, 1), (B, 1, 2048, 1024, 64, 8), (B, 2, 512, 256, 8, 2), (H, 5, 333, 77, 5, 3), (B, 16, 256, 264, 16, 4),
        (H, 24, 1000, 728, 30, 3), (B, 37, 520, 136, 10, 10), (B, 64, 512, 128, 64, 8), (B, 64, 256, 64, 2, 2),
        (H, 64, 130, 50, 3, 1), (B, 100, 264, 72, 7, 2), (B, 200, 128, 64, 2, 1), (S, 3, 100, 60, 6, 2), (S, 20, 256, 130, 9, 3),
-       (D, 9, 65, 33, 5, 2), (D, 1, 128, 64, 8, 8), (B, 7, 1, 1, 3, 2), (B, 4, 64, 32, 300, 5), (H, 2, 4096, 40, 4, 2)]
+       (D, 9, 65, 33, 5, 2), (D, 1, 128, 64, 8, 8), (B, 7, 1, 1, 3, 2), (B, 4, 64, 32, 300, 5), (H, 2, 4096, 40, 4, 2),
+       # the most experts of a token, the most experts, groups of 32 and 64 tokens of an expert on 4 and 8 waves, several
+       # batches, shares of the second product
+       (B, 1, 64, 32, 300, 256), (B, 5, 40, 16, 256, 256), (H, 3, 64, 16, 4096, 2), (B, 24, 2048, 64, 4, 2),
+       (B, 64, 2048, 40, 2, 2), (S, 64, 300, 40, 2, 2), (S, 40, 1100, 24, 5, 2), (D, 40, 128, 40, 2, 2), (D, 30, 600, 24, 4, 2),
+       (B, 150, 64, 300, 6, 6), (H, 129, 24, 1000, 12, 5)]
 
 
 @pytest.mark.parametrize("case", MOE, ids=str)
