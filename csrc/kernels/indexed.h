@@ -1,5 +1,5 @@
 // Products whose matrix depends on the column (lora*.hip, moe.hip): element types, the argument records shared with
-// dplasma_amd/ops/indexed_ops.py, and the plain tile product.
+// dplasma_amd/ops/indexed_ops.py, and fragments for the matrix instructions.
 //
 // Matrices are column-major with one token per column, so a token's features are contiguous: X(c, t) = X[t * ldx + c].
 #pragma once
@@ -171,90 +171,3 @@ struct Carve {
     return q;
   }
 };
-
-// ---------------------------------------------------------------- 64 x 64 tile product in fp32 / fp64
-// acc += sum_c a(row, c) b(col, c) over 64 rows and 64 columns, 256 threads, four waves of 32 x 32 (2 x 2 MFMA
-// 16x16x4).  The operands come through functors that return zero outside their extent, so any stride, alignment or
-// gather works; CA / CB say whether an operand is contiguous in c (then 16 neighbouring threads read along c) or in
-// the row (64 neighbouring threads read along the row).
-template <typename R> struct Mfma16;
-template <> struct Mfma16<float> {
-  typedef f4_t vec;
-  static __device__ inline vec fma(float a, float b, vec c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
-  static __device__ inline int row(int lane, int i) { return 4 * (lane >> 4) + i; }
-};
-template <> struct Mfma16<double> {
-  typedef d4_t vec;
-  static __device__ inline vec fma(double a, double b, vec c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
-  static __device__ inline int row(int lane, int i) { return (lane >> 4) + 4 * i; }
-};
-
-template <typename R> struct TileLds {
-  R a[16][68], b[16][68];
-};
-
-template <typename R> struct TileAcc {
-  typename Mfma16<R>::vec v[2][2];
-  __device__ inline void zero() {
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) v[i][j] = typename Mfma16<R>::vec{R(0), R(0), R(0), R(0)};
-  }
-  // f(row, col, value&) for the 16 elements of this thread
-  template <class F> __device__ inline void each(F f) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          R x = v[i][j][q];
-          f((w >> 1) * 32 + i * 16 + Mfma16<R>::row(lane, q), (w & 1) * 32 + j * 16 + (lane & 15), x);
-          v[i][j][q] = x;
-        }
-  }
-};
-
-template <bool CA, bool CB, typename R, class FA, class FB>
-__device__ inline void tile_product(TileLds<R>& s, TileAcc<R>& acc, int C, FA fa, FB fb) {
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int ar = CA ? tid >> 4 : tid & 63, ac = CA ? tid & 15 : tid >> 6;
-  const int br = CB ? tid >> 4 : tid & 63, bc = CB ? tid & 15 : tid >> 6;
-  R ra[4], rb[4];
-  auto fetch = [&](int c0) {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int c = c0 + (CA ? ac : ac + 4 * q);
-      ra[q] = c < C ? fa(CA ? ar + 16 * q : ar, c) : R(0);
-      const int d = c0 + (CB ? bc : bc + 4 * q);
-      rb[q] = d < C ? fb(CB ? br + 16 * q : br, d) : R(0);
-    }
-  };
-  if (C > 0) fetch(0);
-  for (int c0 = 0; c0 < C; c0 += 16) {
-    __syncthreads();
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      s.a[CA ? ac : ac + 4 * q][CA ? ar + 16 * q : ar] = ra[q];
-      s.b[CB ? bc : bc + 4 * q][CB ? br + 16 * q : br] = rb[q];
-    }
-    __syncthreads();
-    if (c0 + 16 < C) fetch(c0 + 16);
-#pragma unroll
-    for (int k = 0; k < 16; k += 4) {
-      R x[2], y[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        x[i] = s.a[k + (lane >> 4)][(w >> 1) * 32 + i * 16 + (lane & 15)];
-        y[i] = s.b[k + (lane >> 4)][(w & 1) * 32 + i * 16 + (lane & 15)];
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc.v[i][j] = Mfma16<R>::fma(x[i], y[j], acc.v[i][j]);
-    }
-  }
-  __syncthreads();
-}

@@ -84,7 +84,7 @@ struct LowArgs {
 int lora_low(const LowArgs* sets, int n, hipStream_t st);
 
 // y[t*ldy + n] = alpha (sum_c x[t*ldx + c] W(n, c) + sum_j low(t, j) F[(l*N + n)*ldf + j]) + beta y[t*ldy + n];
-// nt: W(n, c) = W[n*ldw + c], else W[c*ldw + n] (h and b only)
+// nt: W(n, c) = W[n*ldw + c], else W[c*ldw + n]
 struct TileArgs {
   const void *x, *W, *F, *hi, *lo;
   const int* ids;
@@ -95,6 +95,6 @@ struct TileArgs {
 };
 int lora_tile(const TileArgs& a, bool nt, hipStream_t st);
 
-// Gradient in h and b (lora_grad.hip).
+// Gradient (lora_grad.hip).
 size_t lora_grad_ws(const LoraArgs& g);
-int lora_grad_half(const LoraArgs& g, hipStream_t st);
+int lora_grad(const LoraArgs& g, hipStream_t st);

@@ -1,4 +1,4 @@
-// Gradient of gemm_lora in the half precisions.
+// Gradient of gemm_lora.
 //
 //   P = s B dy, S = s A^T x per token (lora_low);  dX by the shared product with A's part added (lora_tile);
 //   dA_l = alpha sum_t x_t p_t^T and dB_l = alpha sum_t s_t dy_t^T by k_outer, over an adapter's tokens in order.
@@ -19,7 +19,7 @@ struct PrepareArgs {
   const int* ids;
   int *off, *perm, *pos;
   int4* zero;
-  __bf16* low[4];  // places after an adapter's last token, up to a multiple of 8, are zeroed here (null: not in use)
+  void* low[4];  // places after an adapter's last token, up to a multiple of 8, are zeroed here (null: not in use)
   long long tp;
   int nt, L, r;
   struct Turn {
@@ -54,7 +54,7 @@ template <typename T> __device__ inline void turn_tile(const PrepareArgs::Turn& 
 }
 
 // One workgroup per adapter reads all ids, each thread a run of them, so the order never depends on timing.
-__device__ inline void sort_one(const PrepareArgs& a, int l) {
+template <typename M> __device__ inline void sort_one(const PrepareArgs& a, int l) {
   __shared__ int sums[2][4];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   if (l == 0 && tid == 0) *a.zero = int4{0, 0, 0, 0};
@@ -92,12 +92,12 @@ __device__ inline void sort_one(const PrepareArgs& a, int l) {
   const int end = begin + count, pad = (8 - count % 8) % 8;
   for (int k = 0; k < 4; ++k)
     if (a.low[k])
-      for (int i = tid; i < a.r * pad; i += 256) a.low[k][(i / pad) * a.tp + end + i % pad] = (__bf16)0.f;
+      for (int i = tid; i < a.r * pad; i += 256) ((M*)a.low[k])[(i / pad) * a.tp + end + i % pad] = (M)0;
 }
 
 template <typename T> __global__ __launch_bounds__(256) void k_prepare(PrepareArgs a) {
   int b = blockIdx.x;
-  if (b < a.L) return sort_one(a, b);
+  if (b < a.L) return sort_one<typename Mid<T>::elem>(a, b);
   b -= a.L;
   if (b < a.turn[0].wgs * a.L) return turn_tile<T>(a.turn[0], b);
   turn_tile<T>(a.turn[1], b - a.turn[0].wgs * a.L);
@@ -108,12 +108,11 @@ template <typename T> __global__ __launch_bounds__(256) void k_prepare(PrepareAr
 // window of `win`; the items of windows and adapters are counted through (window + adapter).  An adapter inside one window
 // is finished here (one without tokens gets its zeros), others leave 32-bit parts that k_join adds in the order of the
 // windows: slot 2 w for the adapter that came in from window w - 1, 2 w + 1 for one that begins in w and goes on.
-// COLS columns per workgroup, 16 JF rows j.  Steps of 64 tokens go through a ring of LDS buffers: z as [token][column],
-// read by the transposing LDS read, low as [j][token] in its two parts (both laid out as in k_tile).
+// COLS columns per workgroup, 16 JF rows j.  Steps of 128 bytes of tokens go through a ring of LDS buffers: z as
+// [token][column], read across as W is in k_tile, low as [j][token] in its parts (both laid out as there).
 struct OuterSet {
   const void *z, *thi, *tlo;
-  void* out;
-  float* part;
+  void *out, *part;
   long long ldz, ldo;
   int C, win, items, jc;  // jc: g is stored [j][c] (dA), else [c][j] (dB)
 };
@@ -129,10 +128,15 @@ struct OuterArgs {
 constexpr int COLS = 256, WIN_MAX = 2048;
 
 template <typename T, int JF, bool DMA> __global__ __launch_bounds__(256, 1) void k_outer(OuterArgs a) {
+  typedef typename Num<T>::acc R;
   typedef typename Op<T>::vec V;
-  constexpr int FN = COLS / 64, CH = COLS / 8, J = 64 * CH / 256;  // 4 waves of 64 columns; chunks of a row; per thread
-  constexpr int ZB = 64 * COLS * 2, PB = JF * 16 * 128, STAGE = ZB + 2 * PB, RING = DMA ? (JF == 1 ? 4 : 3) : 2;
-  constexpr int PJ = 2 * PB / 4096, LOADS = J + PJ;
+  typedef typename Mid<T>::elem M;
+  typedef typename Op<M>::vec MV;
+  constexpr int E = Op<T>::E, STEP = 2 * Op<T>::KS;  // tokens of a step
+  constexpr int FN = COLS / 64, CH = COLS / E, J = STEP * CH / 256;  // 4 waves of 64 columns; chunks of a row; per thread
+  constexpr int PARTS = JF == 1 ? 2 : Mid<T>::PARTS;  // (one part of 16 rows is half a load of the workgroup: taken twice)
+  constexpr int ZB = STEP * COLS * (int)sizeof(T), PB = JF * 16 * 128, STAGE = ZB + PARTS * PB, RING = DMA ? (JF == 1 ? 4 : 3) : 2;
+  constexpr int PJ = PARTS * PB / 4096, LOADS = J + PJ;
   __shared__ __attribute__((aligned(1024))) char sm[RING * STAGE];
   __shared__ int rows[WIN_MAX];
   const bool second = (int)blockIdx.x >= a.wgs0;
@@ -164,25 +168,26 @@ template <typename T, int JF, bool DMA> __global__ __launch_bounds__(256, 1) voi
   for (int k = tid; k < n; k += 256) rows[k] = a.perm[p0 + k];
   __syncthreads();
   const T* z = (const T*)g.z;
-  auto turn = [](int step) { return (step & 3) + 4 * ((step >> 3) & 1); };
+  auto chunk = [](int row, int pc) {
+    const int turn = (row & 3) + 4 * ((row >> 3) & 1);
+    return sizeof(T) == 2 ? 2 * ((pc >> 1) ^ turn) + (pc & 1) : pc ^ (16 / E * (row / E & 3));
+  };
   const int sr = tid / CH, pc = tid % CH;
   V v[DMA ? 1 : J];
   auto stage_low = [&](char* b, int s) {
 #pragma unroll
     for (int k = 0; k < PJ; ++k) {
-      const int part = k >= PJ / 2, half = k % (PJ / 2 ? PJ / 2 : 1);
-      const int id = PJ / 2 ? tid + 256 * half : tid & 127, pt = PJ / 2 ? part : tid >> 7;
-      const int row = id >> 3, at = s + 8 * ((id & 7) ^ (row & 7));
-      const __bf16* src = (const __bf16*)(pt ? g.tlo : g.thi) + min(j0 + row, a.r - 1) * a.tp + p0 + at;
+      const int id = tid + 256 * k, pt = id / (PB / 16), row = id % (PB / 16) >> 3, at = s + E * ((id & 7) ^ (row & 7));
+      const M* src = (const M*)(Mid<T>::PARTS == 2 && pt ? g.tlo : g.thi) + min(j0 + row, a.r - 1) * a.tp + p0 + at;
       dma_global(at < n ? (const void*)src : (const void*)a.zero, b + ZB + wave * 1024 + k * 4096);
     }
   };
   auto stage = [&](int s) {
-    char* b = &sm[(s / 64) % RING * STAGE];
+    char* b = &sm[s / STEP % RING * STAGE];
 #pragma unroll
     for (int k = 0; k < J; ++k) {
       const int row = sr + k * (256 / CH), t = s + row;
-      const int c = c0 + (2 * ((pc >> 1) ^ turn(row)) + (pc & 1)) * 8;
+      const int c = c0 + chunk(row, pc) * E;
       if constexpr (DMA) {
         const void* p = t < n && c < g.C ? (const void*)(z + (long long)rows[min(t, n - 1)] * g.ldz + c) : (const void*)a.zero;
         dma_global(p, b + wave * 1024 + k * 4096);
@@ -193,7 +198,7 @@ template <typename T, int JF, bool DMA> __global__ __launch_bounds__(256, 1) voi
     stage_low(b, s);
   };
   auto put = [&](int s) {
-    char* b = &sm[(s / 64) % RING * STAGE];
+    char* b = &sm[s / STEP % RING * STAGE];
 #pragma unroll
     for (int k = 0; k < J; ++k) *(V*)(b + (tid + 256 * k) * 16) = v[k];
   };
@@ -201,29 +206,36 @@ template <typename T, int JF, bool DMA> __global__ __launch_bounds__(256, 1) voi
 #pragma unroll
   for (int i = 0; i < JF; ++i)
 #pragma unroll
-    for (int f = 0; f < FN; ++f) acc[i][f] = f4_t{0, 0, 0, 0};
+    for (int f = 0; f < FN; ++f) acc[i][f] = typename Op<T>::out{R(0), R(0), R(0), R(0)};
   const int ftr = (8 * q + (c16 >> 2)) * (COLS * 2) + (c16 & 3) * 8;
   const int tw = (c16 >> 2) + 4 * (q & 1);
   const int fp = ZB + c16 * 128 + ((q ^ (c16 & 7)) << 4);
   auto multiply = [&](int s) {
-    const char* b = &sm[(s / 64) % RING * STAGE];
+    const char* b = &sm[s / STEP % RING * STAGE];
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
-      b8_t hi[JF], lw[JF];
+      MV hi[JF], lw[JF];
 #pragma unroll
       for (int i = 0; i < JF; ++i) {
-        hi[i] = *(const b8_t*)(b + (fp ^ (64 * kk)) + i * 2048);
-        lw[i] = *(const b8_t*)(b + (fp ^ (64 * kk)) + PB + i * 2048);
+        hi[i] = *(const MV*)(b + (fp ^ (64 * kk)) + i * 2048);
+        lw[i] = Mid<T>::PARTS == 2 ? *(const MV*)(b + (fp ^ (64 * kk)) + PB + i * 2048) : hi[i];
       }
 #pragma unroll
       for (int f = 0; f < FN; ++f) {
-        typedef short s8_t __attribute__((ext_vector_type(8)));
-        const char* p = b + ftr + (((wave * FN + f) ^ tw) << 5) + kk * 32 * COLS * 2;
-        const s4_t v0 = read_turned(p);
-        const s4_t v1 = read_turned(p + 4 * COLS * 2);
-        const s8_t both = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+        V across;
+        if constexpr (sizeof(T) == 2) {
+          typedef short s8_t __attribute__((ext_vector_type(8)));
+          const char* p = b + ftr + (((wave * FN + f) ^ tw) << 5) + kk * 32 * COLS * 2;
+          const s4_t v0 = read_turned(p), v1 = read_turned(p + 4 * COLS * 2);
+          const s8_t both = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+          across = __builtin_bit_cast(V, both);
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            across[e] = *(const T*)(b + ((kk * Op<T>::KS + q * E + e) * COLS + ((wave * FN + f) ^ q) * 16 + c16) * (int)sizeof(T));
+        }
         MidOp<T> x;
-        x.set(__builtin_bit_cast(V, both));
+        x.set(across);
 #pragma unroll
         for (int i = 0; i < JF; ++i) acc[i][f] = x.mma_first(hi[i], lw[i], acc[i][f]);
       }
@@ -236,30 +248,30 @@ template <typename T, int JF, bool DMA> __global__ __launch_bounds__(256, 1) voi
   };
   if constexpr (DMA) {
 #pragma unroll
-    for (int k = 0; k < RING - 1; ++k) stage(64 * k);  // past the last token: zeros
-    for (int s = 0; s < n; s += 64) {
+    for (int k = 0; k < RING - 1; ++k) stage(STEP * k);  // past the last token: zeros
+    for (int s = 0; s < n; s += STEP) {
       // this step has arrived, and every wave has read the one before, whose buffer is filled next
       asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS * (RING - 2)) : "memory");
       meet();
-      stage(s + 64 * (RING - 1));
+      stage(s + STEP * (RING - 1));
       multiply(s);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing is on its way to LDS when the workgroup ends
   } else {
     stage(0);
     put(0);
-    for (int s = 0; s < n; s += 64) {
+    for (int s = 0; s < n; s += STEP) {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       meet();
-      if (s + 64 < n) stage(s + 64);
+      if (s + STEP < n) stage(s + STEP);
       multiply(s);
-      if (s + 64 < n) put(s + 64);
+      if (s + STEP < n) put(s + STEP);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
   const bool whole = lo / g.win == (end - 1) / g.win;
-  const float alpha = (float)a.alpha;
-  float* part = g.part + (long long)(2 * w + (lo >= w * g.win)) * a.r * g.C;
+  const R alpha = (R)a.alpha;
+  R* part = (R*)g.part + (long long)(2 * w + (lo >= w * g.win)) * a.r * g.C;
 #pragma unroll
   for (int f = 0; f < FN; ++f) {
     const int c = c0 + (wave * FN + f) * 16 + c16;
@@ -268,9 +280,9 @@ template <typename T, int JF, bool DMA> __global__ __launch_bounds__(256, 1) voi
     for (int i = 0; i < JF; ++i)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int j = j0 + 16 * i + 4 * q + k;
+        const int j = j0 + 16 * i + out_row<T>(lane, k);
         if (j >= a.r) continue;
-        if (whole) out[where(j, c)] = (T)(alpha == 0.f ? 0.f : alpha * acc[i][f][k]);
+        if (whole) out[where(j, c)] = (T)(alpha == R(0) ? R(0) : alpha * acc[i][f][k]);
         else part[g.jc ? (long long)j * g.C + c : (long long)c * a.r + j] = acc[i][f][k];
       }
   }
@@ -278,6 +290,7 @@ template <typename T, int JF, bool DMA> __global__ __launch_bounds__(256, 1) voi
 
 // Parts of the adapters that go over several windows, added in the windows' order.
 template <typename T> __global__ __launch_bounds__(256) void k_join(OuterArgs a) {
+  typedef typename Num<T>::acc R;
   const OuterSet& g = a.set[blockIdx.z];
   const int l = blockIdx.y, lo = begin_of(a.off, l), count = a.off[l + 1] - a.off[l];
   if (!g.out || count == 0) return;
@@ -285,12 +298,12 @@ template <typename T> __global__ __launch_bounds__(256) void k_join(OuterArgs a)
   if (w0 == w1) return;
   const long long n = (long long)a.r * g.C;
   const int width = g.jc ? g.C : a.r;
-  const float alpha = (float)a.alpha;
+  const R alpha = (R)a.alpha;
   for (long long e = blockIdx.x * 256ll + threadIdx.x; e < n; e += gridDim.x * 256ll) {
-    float v = 0;
+    R v = 0;
 #pragma unroll 4
-    for (int w = w0; w <= w1; ++w) v += g.part[(2 * w + (w == w0)) * n + e];
-    ((T*)g.out)[((long long)l * (n / width) + e / width) * g.ldo + e % width] = (T)(alpha == 0.f ? 0.f : alpha * v);
+    for (int w = w0; w <= w1; ++w) v += ((const R*)g.part)[(2 * w + (w == w0)) * n + e];
+    ((T*)g.out)[((long long)l * (n / width) + e / width) * g.ldo + e % width] = (T)(alpha == R(0) ? R(0) : alpha * v);
   }
 }
 
@@ -305,10 +318,12 @@ int window(const LoraArgs& g, int C) {
 
 template <typename T> struct GradWs {
   int *off, *perm, *pos;
-  __bf16 *hi = nullptr, *lo = nullptr, *pthi = nullptr, *ptlo = nullptr, *sthi = nullptr, *stlo = nullptr;
+  typedef typename Num<T>::acc R;
+  typedef typename Mid<T>::elem M;
+  M *hi = nullptr, *lo = nullptr, *pthi = nullptr, *ptlo = nullptr, *sthi = nullptr, *stlo = nullptr;
   T *At = nullptr, *Bt = nullptr;
   int4* zeros;
-  float *pa = nullptr, *pb = nullptr;
+  R *pa = nullptr, *pb = nullptr;
   bool dx, da, db;
   int rp, ldb, wa, wb;
   long long tp;
@@ -328,20 +343,20 @@ template <typename T> struct GradWs {
     perm = c.take<int>(places(g));
     pos = c.take<int>(g.T);
     if (dx) {
-      hi = c.take<__bf16>((size_t)g.T * rp);
-      lo = c.take<__bf16>((size_t)g.T * rp);
+      hi = c.take<M>((size_t)g.T * rp);
+      if (Mid<T>::PARTS == 2) lo = c.take<M>((size_t)g.T * rp);
       At = c.take<T>((size_t)g.L * g.K * rp);
     }
     if (dx || da) Bt = c.take<T>((size_t)g.L * g.r * ldb);
     if (da) {
-      pthi = c.take<__bf16>(g.r * tp);
-      ptlo = c.take<__bf16>(g.r * tp);
-      pa = c.take<float>((size_t)2 * (places(g) / wa + 1) * g.r * g.K);
+      pthi = c.take<M>(g.r * tp);
+      if (Mid<T>::PARTS == 2) ptlo = c.take<M>(g.r * tp);
+      pa = c.take<R>((size_t)2 * (places(g) / wa + 1) * g.r * g.K);
     }
     if (db) {
-      sthi = c.take<__bf16>(g.r * tp);
-      stlo = c.take<__bf16>(g.r * tp);
-      pb = c.take<float>((size_t)2 * (places(g) / wb + 1) * g.r * g.N);
+      sthi = c.take<M>(g.r * tp);
+      if (Mid<T>::PARTS == 2) stlo = c.take<M>(g.r * tp);
+      pb = c.take<R>((size_t)2 * (places(g) / wb + 1) * g.r * g.N);
     }
     bytes = c.used;
   }
@@ -378,7 +393,7 @@ template <typename T> int run(const LoraArgs& g, hipStream_t st) {
   if (w.da) a.set[0] = {g.X, w.pthi, w.ptlo, g.dA, w.pa, g.ldx, g.ldda, g.K, w.wa, (int)(places(g) / w.wa) + g.L, 1};
   if (w.db) a.set[1] = {g.dY, w.sthi, w.stlo, g.dB, w.pb, g.ldy, g.lddb, g.N, w.wb, (int)(places(g) / w.wb) + g.L, 0};
   a.wgs0 = wgs(a.set[0]);
-  auto aligned = [&](const OuterSet& o) { return !o.out || (((uintptr_t)o.z | (uintptr_t)(o.ldz * sizeof(T))) % 16 == 0 && o.C % 8 == 0); };
+  auto aligned = [&](const OuterSet& o) { return !o.out || (((uintptr_t)o.z | (uintptr_t)(o.ldz * sizeof(T))) % 16 == 0 && o.C % Op<T>::E == 0); };
   const bool dma = aligned(a.set[0]) && aligned(a.set[1]);
   const int jf = g.r <= 16 ? 1 : g.r <= 32 ? 2 : 4;
   const dim3 grid((unsigned)(a.wgs0 + wgs(a.set[1])), cdiv(g.r, 16 * jf));
@@ -395,8 +410,20 @@ template <typename T> int run(const LoraArgs& g, hipStream_t st) {
 
 }  // namespace
 
-size_t lora_grad_ws(const LoraArgs& g) { return g.prec == DPL_H ? GradWs<_Float16>(g, nullptr).bytes : GradWs<__bf16>(g, nullptr).bytes; }
+size_t lora_grad_ws(const LoraArgs& g) {
+  switch (g.prec) {
+    case DPL_S: return GradWs<float>(g, nullptr).bytes;
+    case DPL_D: return GradWs<double>(g, nullptr).bytes;
+  }
+  return GradWs<__bf16>(g, nullptr).bytes;
+}
 
-int lora_grad_half(const LoraArgs& g, hipStream_t st) {
-  return g.prec == DPL_H ? run<_Float16>(g, st) : run<__bf16>(g, st);
+int lora_grad(const LoraArgs& g, hipStream_t st) {
+  switch (g.prec) {
+    case DPL_S: return run<float>(g, st);
+    case DPL_D: return run<double>(g, st);
+    case DPL_H: return run<_Float16>(g, st);
+    case DPL_B: return run<__bf16>(g, st);
+  }
+  return -1;
 }

@@ -213,6 +213,8 @@ template <typename T> int run_low(const LowSets& sets, hipStream_t st) {
 // the same chunk of lie in different banks (no conflicts by the counter).  W stored with its features contiguous (NT false) is kept as it comes,
 // [step][features], and read through the transposing LDS read: a group of 16 lanes takes 4 steps x 16 features; the
 // 32-byte pair of such a read is displaced by the step's place in the instruction (16 steps of one instruction: 8 pairs).
+// s and d read element by element there, a lane group q its own E steps, with the 16 features of a fragment displaced by q
+// (their matrix instructions take 4 and 8 times as long per byte, which hides the reads).
 // The result has the tokens in its columns: a lane holds one token and 4 neighbouring features.
 template <typename T, int B, int WT, int WN, int SLOTS, bool NT, bool DMA>
 __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
@@ -222,7 +224,6 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
   constexpr int FT = B / WT / 16, FN = B / WN / 16;
   constexpr int J = B * 8 / THREADS, CH = B / E;  // CH: chunks of a [step][features] row
   static_assert(SLOTS >= 4 && (DMA || SLOTS == 4), "without DMA the step after next is in registers");
-  static_assert(NT || sizeof(T) == 2, "the transposing LDS read is for 16-bit elements");
   __shared__ __attribute__((aligned(1024))) char sm[SLOTS * SLOT];
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, c16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wt = wave / WN, wn = wave % WN;
@@ -241,7 +242,7 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
   const int wr = NT ? xr : tid / CH;
   const int wmask = CH / 2 - 1;
   auto turn = [&](int step) { return ((step & 3) + 4 * ((step >> 3) & 1)) & wmask; };
-  auto wchunk = [&](int row, int pc) { return 2 * ((pc >> 1) ^ turn(row)) + (pc & 1); };
+  auto wchunk = [&](int row, int pc) { return sizeof(T) == 2 ? 2 * ((pc >> 1) ^ turn(row)) + (pc & 1) : pc ^ (16 / E * (row / E & 3)); };
   V gx[DMA ? 1 : J], gw[DMA ? 1 : J];
   unsigned ox[DMA ? J : 1], ow[DMA ? J : 1];
   constexpr unsigned NOWHERE = 0x80000000u;
@@ -322,6 +323,10 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
     for (int i = 0; i < FN; ++i) {
       if constexpr (NT) {
         r.w[i] = *(const V*)(sw + (fw ^ (64 * half)) + i * 2048);
+      } else if constexpr (sizeof(T) > 2) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          r.w[i][e] = *(const T*)(sw + ((half * Op<T>::KS + q * E + e) * B + ((wn * FN + i) ^ q) * 16 + c16) * (int)sizeof(T));
       } else {
         typedef short s8_t __attribute__((ext_vector_type(8)));
         const char* p = sw + ftr + (((wn * FN + i) ^ tw) << 5) + half * 32 * B * 2;
@@ -527,7 +532,7 @@ template <typename T, bool NT> int run_tile(const TileArgs& a, hipStream_t st) {
   };
   // W with its features contiguous also needs whole chunks of them within a row, and offsets in 32 bits over all of it
   const bool dma = wide(a.x, a.ldx, 256) && wide(a.W, a.ldw, 256) && a.C % Op<T>::E == 0 &&
-                   (NT || (a.N % 8 == 0 && (a.C + 1024ll) * a.ldw * size < (1ll << 32)));
+                   (NT || (a.N % Op<T>::E == 0 && (a.C + 1024ll) * a.ldw * size < (1ll << 32)));
   auto tiles = [&](int b) { return (long long)cdiv(a.T, b) * cdiv(a.N, b); };
   if constexpr (sizeof(T) == 2)
     if (dma && tiles(256) >= 160) {
@@ -537,9 +542,11 @@ template <typename T, bool NT> int run_tile(const TileArgs& a, hipStream_t st) {
   // 8 buffers where they leave every workgroup a CU, and 8 waves on a 128 tile (T x K x N, us with 4 and 8 buffers: bf16
   // 256 x 4096 x 4096 38.5, 22.4; 1024 x 4096 x 4096 56.9, 49.1 with 4 waves, 42.1 with 8; with W's features contiguous
   // 67.9 with 4 and 4 waves, 61.4 with 8 and 8; fp64 1000 x 1000 x 2000 143, 175, with 4 and 8 waves 137)
-  if (tiles(128) >= 160 || sizeof(T) == 8) {
-    if (!dma) launch<T, 128, 2, sizeof(T) == 8 ? 4 : 2, 4, NT, false>(a, st);
-    else if (sizeof(T) < 8 && tiles(128) <= 256) launch<T, 128, 2, 4, 8, NT, true>(a, st);
+  if constexpr (sizeof(T) == 8) {
+    dma ? launch<T, 128, 2, 4, 4, NT, true>(a, st) : launch<T, 128, 2, 4, 4, NT, false>(a, st);
+  } else if (tiles(128) >= 160) {
+    if (!dma) launch<T, 128, 2, 2, 4, NT, false>(a, st);
+    else if (tiles(128) <= 256) launch<T, 128, 2, 4, 8, NT, true>(a, st);
     else launch<T, 128, 2, 4, 4, NT, true>(a, st);
   } else {
     if (!dma) launch<T, 64, 2, 2, 4, NT, false>(a, st);
@@ -566,8 +573,8 @@ int lora_low(const LowArgs* sets, int n, hipStream_t st) {
 
 int lora_tile(const TileArgs& a, bool nt, hipStream_t st) {
   switch (a.prec) {
-    case DPL_S: return nt ? run_tile<float, true>(a, st) : -1;
-    case DPL_D: return nt ? run_tile<double, true>(a, st) : -1;
+    case DPL_S: return nt ? run_tile<float, true>(a, st) : run_tile<float, false>(a, st);
+    case DPL_D: return nt ? run_tile<double, true>(a, st) : run_tile<double, false>(a, st);
     case DPL_H: return nt ? run_tile<_Float16, true>(a, st) : run_tile<_Float16, false>(a, st);
     case DPL_B: return nt ? run_tile<__bf16, true>(a, st) : run_tile<__bf16, false>(a, st);
   }
