@@ -539,13 +539,12 @@ template <typename T, bool NT> int run_tile(const TileArgs& a, hipStream_t st) {
       launch<T, 256, 2, 4, 5, NT, true>(a, st);
       return (int)hipGetLastError();
     }
-  // 8 buffers where they leave every workgroup a CU, and 8 waves on a 128 tile (T x K x N, us with 4 and 8 buffers: bf16
-  // 256 x 4096 x 4096 38.5, 22.4; 1024 x 4096 x 4096 56.9, 49.1 with 4 waves, 42.1 with 8; with W's features contiguous
-  // 67.9 with 4 and 4 waves, 61.4 with 8 and 8; fp64 1000 x 1000 x 2000 143, 175, with 4 and 8 waves 137)
-  if constexpr (sizeof(T) == 8) {
-    dma ? launch<T, 128, 2, 4, 4, NT, true>(a, st) : launch<T, 128, 2, 4, 4, NT, false>(a, st);
-  } else if (tiles(128) >= 160) {
-    if (!dma) launch<T, 128, 2, 2, 4, NT, false>(a, st);
+  // 128 tiles where they reach most CUs (fp64, 1000 x 1000 x 2000: 148 us with 128 of them, 93 with 512 of 64; 300 x 1000
+  // x 2000: 150, 59).  8 buffers where they leave every workgroup a CU or two, and 8 waves on a 128 tile (T x K x N, us
+  // with 4 and 8 buffers: bf16 100 x 4096 x 4096 38.0, 21.3; 512 x 4096 x 4096 39.7, 31.5; 1024 x 4096 x 4096 51.5, 39.8,
+  // with W's features contiguous 55.8, 43.5)
+  if (tiles(128) >= 160) {
+    if (!dma) launch<T, 128, 2, sizeof(T) == 8 ? 4 : 2, 4, NT, false>(a, st);  // (fp64 spills with 4 waves)
     else if (tiles(128) <= 256) launch<T, 128, 2, 4, 8, NT, true>(a, st);
     else launch<T, 128, 2, 4, 4, NT, true>(a, st);
   } else {
