@@ -23,6 +23,8 @@ import torch
 
 PRECS = {"s": torch.float32, "d": torch.float64, "c": torch.complex64, "z": torch.complex128}
 EPS = {"s": 5.96e-08, "d": 1.11e-16, "c": 5.96e-08, "z": 1.11e-16}
+# the products whose matrix depends on the column, and their precisions
+INDEXED = {"s": torch.float32, "d": torch.float64, "h": torch.float16, "b": torch.bfloat16}
 
 
 def _parse(argv):
@@ -115,10 +117,11 @@ class Harness:
             if a.verbose:
                 print(f"#+++++ scheduler {a.scheduler}: native ready-queue issue order", flush=True)
         self.prec = a.op[0]
-        if self.prec not in PRECS:
-            raise SystemExit(f"operation must start with a precision letter s/d/c/z: {a.op}")
         self.name = a.op[1:]
-        self.dt = PRECS[self.prec]
+        precs = INDEXED if self.name in INDEXED_OPS else PRECS
+        if self.prec not in precs:
+            raise SystemExit(f"operation must start with a precision letter {'/'.join(precs)}: {a.op}")
+        self.dt = precs[self.prec]
         self.ok = True
         self.mats = []   # operands made by mat(): restored before every run after the first
         if a.dot:
@@ -744,6 +747,83 @@ def t_pivgen(h):
     h.check("invalid trees", float(bad), 0.5)
 
 
+def _normal(h, m, n, nb, std, seed, name):
+    """m x n of normal numbers in tiles that span all rows, nb columns wide."""
+    X = h.mat(m, n, mb=max(m, 1), nb=max(nb, 1), name=name)
+    gen = torch.Generator().manual_seed(seed)
+    return X.from_dense((torch.randn(m, n, generator=gen, dtype=torch.float64) * std).to(h.dt))
+
+
+def _indexed_check(h, what, X, ref, terms):
+    """One rounding of the result, and that of sums of ``terms`` products (32 bits for h and b)."""
+    out = torch.finfo(h.dt).eps / 2
+    eps = out + terms * min(out, 2.0 ** -24)
+    got = _dense(h, X).double()
+    h.check(f"||{what} - ref|| / (||ref|| eps)", float((got - ref).abs().max() / (ref.abs().max() * eps + 1e-300)), 10.0)
+
+
+def t_gemm_lora(h, grad=False):
+    """-M tokens (default N), -N features out, -K features in (default N), -i rank (default 16); 4 adapters, and tokens
+    without one."""
+    dp, a, ctx = h.dp, h.a, h.ctx
+    if ctx.world > 1:
+        raise SystemExit(f"{h.name} runs on one process")
+    T, N, K, r, L = a.M or a.N, a.N, a.K or a.N, a.IB or 16, 4
+    W, X, A = _normal(h, K, N, N, K ** -0.5, a.seed, "A"), _normal(h, K, T, T, 1.0, a.seed + 1, "B"), \
+        _normal(h, K, L * r, r, K ** -0.5, a.seed + 2, "F")
+    B, Y = _normal(h, r, L * N, N, r ** -0.5, a.seed + 3, "G"), _normal(h, N, T, T, 1.0, a.seed + 4, "C")
+    gen = torch.Generator().manual_seed(a.seed + 5)
+    ids = torch.randint(-1, L, (T,), generator=gen, dtype=torch.int32).to(ctx.device)
+    scale = (torch.rand(L, generator=gen, dtype=torch.float64) + 0.5).to(torch.float64 if h.prec == "d" else torch.float32)
+    w, x, fa, fb, y = (_dense(h, M).double() for M in (W, X, A, B, Y))
+    if not grad:
+        h.run_tp("gemm_lora", lambda: dp.gemm_lora_New(ctx, a.alpha, W, X, A, B, ids, scale.to(ctx.device), 0.5, Y))
+    else:
+        dX, dA, dB = (_normal(h, M.m, M.n, M.nb, 0.0, 0, "D") for M in (X, A, B))
+        h.run_tp("gemm_lora_grad", lambda: dp.gemm_lora_grad_New(ctx, a.alpha, W, X, A, B, ids, scale.to(ctx.device), Y,
+                                                                 dX, dA, dB))
+    if not a.check:
+        return
+    fa, fb, ids = fa.view(K, L, r), fb.view(r, L, N), ids.cpu()
+    dx, da, db = w @ y, torch.zeros_like(fa), torch.zeros_like(fb)
+    ref = w.t() @ x
+    for l in range(L):
+        t, s = torch.nonzero(ids == l).flatten(), float(scale[l])
+        low, up = s * (fa[:, l].t() @ x[:, t]), s * (fb[:, l] @ y[:, t])
+        ref[:, t] += fb[:, l].t() @ low
+        dx[:, t] += fa[:, l] @ up
+        da[:, l], db[:, l] = x[:, t] @ up.t(), low @ y[:, t].t()
+    if not grad:
+        _indexed_check(h, "Y", Y, a.alpha * ref + 0.5 * y, K + r)
+        return
+    _indexed_check(h, "dX", dX, a.alpha * dx, N + r)
+    _indexed_check(h, "dA", dA, a.alpha * da.reshape(K, L * r), N + T)
+    _indexed_check(h, "dB", dB, a.alpha * db.reshape(r, L * N), K + T)
+
+
+def t_moe(h):
+    """-M tokens (default 16), -N features, -K features of an expert (default N); 8 experts, 2 of them for a token."""
+    dp, a, ctx = h.dp, h.a, h.ctx
+    if ctx.world > 1:
+        raise SystemExit(f"{h.name} runs on one process")
+    T, H, I, E, k = a.M or 16, a.N, a.K or a.N, 8, 2
+    G, X, Y = _normal(h, H, E, E, H ** -0.5, a.seed, "A"), _normal(h, H, T, T, 1.0, a.seed + 1, "B"), \
+        _normal(h, H, T, T, 1.0, a.seed + 2, "C")
+    W1, W2 = _normal(h, H, E * 2 * I, 2 * I, H ** -0.5, a.seed + 3, "F"), _normal(h, I, E * H, H, I ** -0.5, a.seed + 4, "G")
+    y = _dense(h, Y).double()
+    h.run_tp("moe", lambda: dp.moe_New(ctx, k, True, G, W1, W2, a.alpha, X, 0.5, Y))
+    if a.check:
+        g, x, w1, w2 = (_dense(h, M).double() for M in (G, X, W1, W2))
+        z = g.t() @ x
+        weight, chosen = torch.topk(torch.softmax(z, 0), k, dim=0)
+        ref, w1, w2 = torch.zeros_like(x), w1.view(H, E, 2 * I), w2.view(I, E, H)
+        for t in range(T):
+            for e, p in zip(chosen[:, t].tolist(), (weight[:, t] / weight[:, t].sum()).tolist()):
+                v = w1[:, e].t() @ x[:, t]
+                ref[:, t] += p * (w2[:, e].t() @ (torch.nn.functional.silu(v[:I]) * v[I:]))
+        _indexed_check(h, "Y", Y, a.alpha * ref + 0.5 * y, H + I)
+
+
 def _inf(x) -> float:
     """Infinity norm (max row sum of |x|) -- the norm of the reference's solve checks
     (tests/testing_zgetrf_incpiv.c:176-203, src/dplasma_zcheck.c check_zaxmb)."""
@@ -790,6 +870,8 @@ OPS = {
     "unmlq_systolic": lambda h: t_unmqr(h, True, "systolic"),
     "gesv_incpiv": t_gesv_incpiv, "gesvd": t_gesvd, "hbrdt": t_hbrdt, "pivgen": t_pivgen,
 }
+INDEXED_OPS = {"gemm_lora": t_gemm_lora, "gemm_lora_grad": lambda h: t_gemm_lora(h, grad=True), "moe": t_moe}
+OPS.update(INDEXED_OPS)
 
 
 def main(argv=None):

@@ -195,3 +195,33 @@ def test_columns_side_by_side_in_one_buffer(ctx):
     dp.gemm_lora(ctx, 1.0, W, X, A, Bd, c.ids, c.scale, 0.0, Y)
     within(both[:5, 8:], *c.plain())
     assert torch.equal(both[:5, :8], c.x) and not both[5].any()
+
+
+DRIVER = ["bgemm_lora -N 96 -M 70 -K 64 -i 8 -x", "dgemm_lora -N 50 -M 9 -x --nruns 2", "hgemm_lora_grad -N 96 -M 70 -K 64 -x",
+          "sgemm_lora_grad -N 40 -M 30 -K 64 -x -a 0.5", "bmoe -N 64 -K 48 -x", "dmoe -N 40 -M 5 -x"]
+
+
+@pytest.mark.parametrize("args", DRIVER)
+def test_testing_driver(args, capsys):
+    from dplasma_amd import testing
+    assert testing.main(args.split() + ["-g", "0"]) == 0
+    out = capsys.readouterr().out
+    assert "[****] TIME(s)" in out and "CORRECT" in out and "SUSPICIOUS" not in out
+
+
+@pytest.mark.parametrize("args", ["bpotrf -N 40", "hgemm -N 40", "zmoe -N 40", "cgemm_lora -N 40"])
+def test_testing_driver_refuses_other_precisions(args):
+    from dplasma_amd import testing
+    with pytest.raises(SystemExit):
+        testing.main(args.split() + ["-g", "0"])
+
+
+def test_run_of_a_lone_task_is_traced(ctx, tmp_path):
+    """A taskpool of one task leaves its spans where tracing is on."""
+    c = Lora(D, 5, 8, 8, 4, 2)
+    tr = dp.profiling_start(ctx)
+    try:
+        c.forward(ctx)
+    finally:
+        dp.profiling_stop(ctx, str(tmp_path / "t.json"))
+    assert "GEMM_LORA" in (tmp_path / "t.json").read_text()

@@ -414,3 +414,24 @@ def test_storage_on_another_device_is_refused(ctx):
         dp.gemm_lora(ctx, 1.0, matrix(c.w.cpu()), X, A, Bd, c.ids, None, 0.0, Y)
     with pytest.raises(ValueError):
         dp.gemm_lora(ctx, 1.0, W, X, A, Bd, c.ids.cpu(), None, 0.0, Y)
+
+
+@pytest.mark.parametrize("args", ["bgemm_lora -N 2048 -M 300 -K 1024 -x", "hgemm_lora_grad -N 512 -M 700 -K 640 -x",
+                                  "sgemm_lora_grad -N 300 -M 200 -x", "dgemm_lora -N 200 -M 20 -x", "bmoe -N 512 -K 256 -x --nruns 2"])
+def test_testing_driver(args, capsys):
+    from dplasma_amd import testing
+    assert testing.main(args.split()) == 0
+    out = capsys.readouterr().out
+    assert "[****] TIME(s)" in out and "CORRECT" in out and "SUSPICIOUS" not in out
+
+
+def test_traced_run(ctx, tmp_path):
+    """A lone task's run with tracing on: the same result, and its span in the trace."""
+    c = lora(B, 9, 256, 128, 8, 3, "tokens")
+    plain = c.forward(ctx)
+    dp.profiling_start(ctx)
+    try:
+        assert torch.equal(plain, c.forward(ctx))
+    finally:
+        dp.profiling_stop(ctx, str(tmp_path / "t.json"))
+    assert "GEMM_LORA" in (tmp_path / "t.json").read_text()
