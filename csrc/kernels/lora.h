@@ -4,6 +4,8 @@
 
 // 16 bytes per lane from memory to LDS (lane i to lds + 16 i; lds is the same for the whole wave).  The buffer form reads
 // base[off + soff ..], zeros where that is past `bytes`.
+// The kernels that use these have all their LDS in one object: with two the compiler tells their accesses apart, and then
+// waits for every load to LDS that is under way before it reads the object that they go to.  The waits are the kernels'.
 __device__ inline void dma_buffer(const void* base, unsigned bytes, void* lds, unsigned off, int soff) {
 #ifdef __HIP_DEVICE_COMPILE__
   __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void*)base, 0, bytes, 0x00020000),

@@ -145,7 +145,7 @@ __global__ __launch_bounds__(1024) void k_one(const T* __restrict__ x, const T* 
 // workgroup per CU allow; what the adapters' parts need is asked for before and beside them.
 constexpr int S_MAX = 64;  // r up to which the low-rank vectors go through LDS
 
-template <typename T, int G, int NF>
+template <typename T, int G, int NF, bool LINES>
 __global__ __launch_bounds__(512) void k_few_apply(const T* __restrict__ x, long long ldx, const T* __restrict__ W,
                                                    long long ldw, const T* __restrict__ B, long long ldb,
                                                    const int* __restrict__ ids,
@@ -156,10 +156,14 @@ __global__ __launch_bounds__(512) void k_few_apply(const T* __restrict__ x, long
   typedef typename Op<T>::vec V;
   constexpr int E = Op<T>::E, KS = Op<T>::KS, ROW = 16 * NF, LANES = 512 / ROW;  // tokens finished at a time
   constexpr int TI = (16 * G + LANES - 1) / LANES, SI = 16 * G * S_MAX / 512;
-  __shared__ R red[8][16 * G][ROW + 1], low[16 * G * S_MAX];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, q = lane >> 4, c = lane & 15;
+  constexpr int RING = G == 4 ? 2 : 3, SLOT = G * 2048, RED = 8 * 16 * G * (ROW + 1) * (int)sizeof(R);
+  constexpr int MAIN = LINES && 8 * RING * SLOT > RED ? 8 * RING * SLOT : RED;
+  __shared__ __attribute__((aligned(1024))) char sm[MAIN + 16 * G * S_MAX * sizeof(R)];
+  R* low = (R*)(sm + MAIN);
+  R(*red)[16 * G][ROW + 1] = (R(*)[16 * G][ROW + 1])sm;
+  const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, c = lane & 15;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n0 = blockIdx.x * ROW;
-  const int steps = (K + KS - 1) / KS, s0 = steps * w / 8, s1 = steps * (w + 1) / 8, whole = min(s1, K / KS);
   typename Op<T>::out acc[NF][G];
 #pragma unroll
   for (int f = 0; f < NF; ++f)
@@ -185,43 +189,121 @@ __global__ __launch_bounds__(512) void k_few_apply(const T* __restrict__ x, long
     for (int k = 0; k < SI; ++k)
       if (tid + 512 * k < nt * r) sv[k] = S[tid + 512 * k];
   }
-  int s = s0;
-  auto run = [&](auto width) {
-    constexpr int U = decltype(width)::value;
-    V a[U][NF], b[U][G];
+  if constexpr (LINES) {
+    constexpr int BK = 2 * KS, WL = 2 * NF, XL = 2 * G;  // loads of a step
+    constexpr unsigned NOWHERE = 0x80000000u;
+    const int units = (K + 4 * BK - 1) / (4 * BK), d0 = units * w / 8 * 4, d1 = units * (w + 1) / 8 * 4;
+    char* ring = sm + w * RING * SLOT;
+    const int xr = lane >> 3, xc = (lane & 7) ^ xr;
+    unsigned ox[XL];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int k = 0; k < XL; ++k) ox[k] = (unsigned)(min(8 * k + xr, nt - 1) * (int)ldx + xc * E) * sizeof(T);
+    const unsigned xbytes = (unsigned)(((nt - 1) * ldx + K) * (long long)sizeof(T));
+    auto stage = [&](int d) {  // past K: zeros
+      const bool in = d * BK + xc * E < K;
+      char* b = ring + d % RING * SLOT;
 #pragma unroll
-      for (int f = 0; f < NF; ++f) a[u][f] = load_vec(pw[f] + (long long)(s + u) * KS);
+      for (int k = 0; k < XL; ++k) dma_buffer(x, xbytes, b + k * 1024, in ? ox[k] : NOWHERE, d * BK * (int)sizeof(T));
+    };
+    V a[4][2][NF];
+    auto weights = [&](V(*v)[NF], int d) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int g = 0; g < G; ++g) b[u][g] = load_vec(px[g] + (long long)(s + u) * KS);
+        for (int f = 0; f < NF; ++f) v[h][f] = load_vec(pw[f] + min((2 * d + h) * KS, K - E - q * E));
+    };
+    const int fx = c * 128 + ((q ^ (c & 7)) << 4);
+    auto step = [&](const V(*v)[NF], int d) {
+      const char* b = ring + d % RING * SLOT;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+      for (int h = 0; h < 2; ++h) {
+        const bool in = (2 * d + h) * KS + q * E < K;
+        V z[G];
 #pragma unroll
-      for (int g = 0; g < G; ++g)
+        for (int g = 0; g < G; ++g) z[g] = *(const V*)(b + (fx ^ 64 * h) + g * 2048);
 #pragma unroll
-        for (int f = 0; f < NF; ++f) acc[f][g] = Op<T>::mma(a[u][f], b[u][g], acc[f][g]);
-    s += U;
-  };
-  if constexpr (G == 1)
-    while (s + 16 <= whole) run(Int<16>());
-  if constexpr (sizeof(T) < 8)
-    while (s + 8 <= whole) run(Int<8>());
-  while (s + 4 <= whole) run(Int<4>());
-  while (s + 2 <= whole) run(Int<2>());
-  if (s < whole) run(Int<1>());
-  for (; s < s1; ++s) {
-    const int left = K - s * KS - q * E;
-    V a[NF];
+        for (int f = 0; f < NF; ++f) {
+          V m = v[h][f];
 #pragma unroll
-    for (int f = 0; f < NF; ++f) a[f] = load_part(pw[f] + (long long)s * KS, left);
+          for (int i = 0; i < E; ++i) m[i] = in ? m[i] : (T)0;
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const V b = load_part(px[g] + (long long)s * KS, left);
+          for (int g = 0; g < G; ++g) acc[f][g] = Op<T>::mma(m, z[g], acc[f][g]);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    if (d0 < d1) {
+      // A step's x is asked for RING - 1 steps ahead, its weights four, and a wait is for the step's x: for all but what
+      // was asked for after it.  The first requests come in the order that the counts of the loop expect.
 #pragma unroll
-      for (int f = 0; f < NF; ++f) acc[f][g] = Op<T>::mma(a[f], b, acc[f][g]);
+      for (int u = 0; u < 4; ++u) {
+        if (u >= 5 - RING) stage(d0 + u - (5 - RING));
+        weights(a[u], d0 + u);
+      }
+      int d = d0;
+      for (; d + 8 <= d1; d += 4) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(WL + (RING - 2) * (XL + WL)) : "memory");
+          step(a[u], d + u);
+          stage(d + u + RING - 1);
+          weights(a[u], d + u + 4);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      auto last = [&](auto at) {
+        constexpr int U = decltype(at)::value;
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(XL * ((U + RING - 2 < 3 ? U + RING - 2 : 3) - U) + WL * (RING - 1 > U ? RING - 1 - U : 0)) : "memory");
+        step(a[U], d + U);
+        if (U + RING - 1 < 4) stage(d + U + RING - 1);
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      last(Int<0>());
+      last(Int<1>());
+      last(Int<2>());
+      last(Int<3>());
+    }
+    __syncthreads();  // the rings give way to the join
+  } else {
+    const int steps = (K + KS - 1) / KS, s0 = steps * w / 8, s1 = steps * (w + 1) / 8, whole = min(s1, K / KS);
+    int s = s0;
+    auto run = [&](auto width) {
+      constexpr int U = decltype(width)::value;
+      V a[U][NF], b[U][G];
+  #pragma unroll
+      for (int u = 0; u < U; ++u)
+  #pragma unroll
+        for (int f = 0; f < NF; ++f) a[u][f] = load_vec(pw[f] + (long long)(s + u) * KS);
+  #pragma unroll
+      for (int u = 0; u < U; ++u)
+  #pragma unroll
+        for (int g = 0; g < G; ++g) b[u][g] = load_vec(px[g] + (long long)(s + u) * KS);
+  #pragma unroll
+      for (int u = 0; u < U; ++u)
+  #pragma unroll
+        for (int g = 0; g < G; ++g)
+  #pragma unroll
+          for (int f = 0; f < NF; ++f) acc[f][g] = Op<T>::mma(a[u][f], b[u][g], acc[f][g]);
+      s += U;
+    };
+    if constexpr (G == 1)
+      while (s + 16 <= whole) run(Int<16>());
+    if constexpr (sizeof(T) < 8)
+      while (s + 8 <= whole) run(Int<8>());
+    while (s + 4 <= whole) run(Int<4>());
+    while (s + 2 <= whole) run(Int<2>());
+    if (s < whole) run(Int<1>());
+    for (; s < s1; ++s) {
+      const int left = K - s * KS - q * E;
+      V a[NF];
+  #pragma unroll
+      for (int f = 0; f < NF; ++f) a[f] = load_part(pw[f] + (long long)s * KS, left);
+  #pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const V b = load_part(px[g] + (long long)s * KS, left);
+  #pragma unroll
+        for (int f = 0; f < NF; ++f) acc[f][g] = Op<T>::mma(a[f], b, acc[f][g]);
+      }
     }
   }
   // the first two vectors of the adapters' rows, on their way during the join
@@ -303,17 +385,22 @@ template <typename T> int run(const LoraArgs& g, hipStream_t st) {
     kernel<<<cdiv(g.N, 16 * nf), 512, 0, st>>>(X, g.ldx, W, g.ldw, B, g.ldb, ids, S, g.T, g.K, g.N, g.r, g.L, (R)g.alpha, (R)g.beta,
                                           (T*)g.Y, g.ldy);
   };
-  if constexpr (sizeof(T) < 8)
-    if (nf == 2) {
-      if (g.T <= 32) apply(k_few_apply<T, 2, 2>);
-      else if (g.T <= 48) apply(k_few_apply<T, 3, 2>);
-      else apply(k_few_apply<T, 4, 2>);
-      return (int)hipGetLastError();
-    }
-  if (g.T <= 16) apply(k_few_apply<T, 1, 1>);
-  else if (g.T <= 32) apply(k_few_apply<T, 2, 1>);
-  else if (g.T <= 48) apply(k_few_apply<T, 3, 1>);
-  else apply(k_few_apply<T, 4, 1>);
+  const int groups = cdiv(g.T, 16);
+  if constexpr (sizeof(T) < 8) {
+    const bool lines = ((uintptr_t)X | (uintptr_t)(g.ldx * sizeof(T))) % 16 == 0 && g.K % Op<T>::E == 0 && g.K >= 64 * Op<T>::KS &&
+                       g.ldx * (long long)sizeof(T) * 64 < (1ll << 30);
+    auto pick = [&](auto f, auto l) {
+      constexpr int F = decltype(f)::value;
+      constexpr bool L = decltype(l)::value;
+      if constexpr (F == 1) if (groups == 1) return apply(k_few_apply<T, 1, F, L>);
+      groups <= 2 ? apply(k_few_apply<T, 2, F, L>) : groups == 3 ? apply(k_few_apply<T, 3, F, L>) : apply(k_few_apply<T, 4, F, L>);
+    };
+    if (nf == 2) lines ? pick(Int<2>(), Int<1>()) : pick(Int<2>(), Int<0>());
+    else lines ? pick(Int<1>(), Int<1>()) : pick(Int<1>(), Int<0>());
+  } else {
+    groups == 1 ? apply(k_few_apply<T, 1, 1, false>) : groups == 2 ? apply(k_few_apply<T, 2, 1, false>)
+    : groups == 3 ? apply(k_few_apply<T, 3, 1, false>) : apply(k_few_apply<T, 4, 1, false>);
+  }
   return (int)hipGetLastError();
 }
 

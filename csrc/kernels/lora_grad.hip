@@ -137,8 +137,8 @@ template <typename T, int JF, bool DMA> __global__ __launch_bounds__(256, 1) voi
   constexpr int PARTS = JF == 1 ? 2 : Mid<T>::PARTS;  // (one part of 16 rows is half a load of the workgroup: taken twice)
   constexpr int ZB = STEP * COLS * (int)sizeof(T), PB = JF * 16 * 128, STAGE = ZB + PARTS * PB, RING = DMA ? (JF == 1 ? 4 : 3) : 2;
   constexpr int PJ = PARTS * PB / 4096, LOADS = J + PJ;
-  __shared__ __attribute__((aligned(1024))) char sm[RING * STAGE];
-  __shared__ int rows[WIN_MAX];
+  __shared__ __attribute__((aligned(1024))) char sm[RING * STAGE + WIN_MAX * sizeof(int)];
+  int* rows = (int*)(sm + RING * STAGE);
   const bool second = (int)blockIdx.x >= a.wgs0;
   const OuterSet& g = a.set[second];
   const int block = second ? blockIdx.x - a.wgs0 : blockIdx.x;
@@ -154,6 +154,12 @@ template <typename T, int JF, bool DMA> __global__ __launch_bounds__(256, 1) voi
   }
   const int w = item - l, lo = begin_of(a.off, l), count = a.off[l + 1] - a.off[l], end = lo + count;
   T* out = (T*)g.out;
+  // (copies: a pointer chosen per lane from the arguments would be loaded again, and waited for, in every step)
+  const T* z = (const T*)g.z;
+  const M *thi = (const M*)g.thi, *tlo = Mid<T>::PARTS == 2 ? (const M*)g.tlo : thi;
+  const void* zero = a.zero;
+  const long long ldz = g.ldz, tp = a.tp;
+  const int C = g.C, r = a.r;
   auto where = [&](int j, int c) { return g.jc ? ((long long)l * a.r + j) * g.ldo + c : ((long long)l * g.C + c) * g.ldo + j; };
   if (count == 0) {
     if (w == lo / g.win)
@@ -167,7 +173,6 @@ template <typename T, int JF, bool DMA> __global__ __launch_bounds__(256, 1) voi
   if (n <= 0) return;
   for (int k = tid; k < n; k += 256) rows[k] = a.perm[p0 + k];
   __syncthreads();
-  const T* z = (const T*)g.z;
   auto chunk = [](int row, int pc) {
     const int turn = (row & 3) + 4 * ((row >> 3) & 1);
     return sizeof(T) == 2 ? 2 * ((pc >> 1) ^ turn) + (pc & 1) : pc ^ (16 / E * (row / E & 3));
@@ -178,10 +183,16 @@ template <typename T, int JF, bool DMA> __global__ __launch_bounds__(256, 1) voi
 #pragma unroll
     for (int k = 0; k < PJ; ++k) {
       const int id = tid + 256 * k, pt = id / (PB / 16), row = id % (PB / 16) >> 3, at = s + E * ((id & 7) ^ (row & 7));
-      const M* src = (const M*)(Mid<T>::PARTS == 2 && pt ? g.tlo : g.thi) + min(j0 + row, a.r - 1) * a.tp + p0 + at;
-      dma_global(at < n ? (const void*)src : (const void*)a.zero, b + ZB + wave * 1024 + k * 4096);
+      const M* src = (pt ? tlo : thi) + min(j0 + row, r - 1) * tp + p0 + at;
+      dma_global(at < n ? (const void*)src : zero, b + ZB + wave * 1024 + k * 4096);
     }
   };
+  int token[J];  // of the next step's rows
+  auto look = [&](int s) {
+#pragma unroll
+    for (int k = 0; k < J; ++k) token[k] = rows[min(s + sr + k * (256 / CH), n - 1)];
+  };
+  look(0);
   auto stage = [&](int s) {
     char* b = &sm[s / STEP % RING * STAGE];
 #pragma unroll
@@ -189,13 +200,14 @@ template <typename T, int JF, bool DMA> __global__ __launch_bounds__(256, 1) voi
       const int row = sr + k * (256 / CH), t = s + row;
       const int c = c0 + chunk(row, pc) * E;
       if constexpr (DMA) {
-        const void* p = t < n && c < g.C ? (const void*)(z + (long long)rows[min(t, n - 1)] * g.ldz + c) : (const void*)a.zero;
+        const void* p = t < n && c < C ? (const void*)(z + (long long)token[k] * ldz + c) : zero;
         dma_global(p, b + wave * 1024 + k * 4096);
       } else {
-        v[k] = load_part(z + (t < n ? (long long)rows[t] * g.ldz + c : 0), t < n ? g.C - c : 0);
+        v[k] = load_part(z + (t < n ? (long long)token[k] * ldz + c : 0), t < n ? C - c : 0);
       }
     }
     stage_low(b, s);
+    look(s + STEP);
   };
   auto put = [&](int s) {
     char* b = &sm[s / STEP % RING * STAGE];

@@ -47,9 +47,10 @@ __global__ __launch_bounds__(DMA && JF * TF >= 4 ? 256 : 512) void k_low_tile(Lo
   constexpr int WAVES = DMA && JF * TF >= 4 ? 4 : 8, E = Op<T>::E, KS = Op<T>::KS;
   constexpr int RING = JF == 4 || JF + TF == 3 ? 3 : 4, LOADS = 2 * TF + 2 * JF, STAGE = LOADS * 1024;
   constexpr int JOIN = WAVES * 16 * (16 * TF + 1) * (int)sizeof(R);
-  __shared__ __attribute__((aligned(1024))) char sm[DMA ? WAVES * RING * STAGE : JOIN];
-  static_assert(!DMA || JOIN <= WAVES * RING * STAGE, "the join's place");
-  __shared__ int sid[16 * TF];
+  constexpr int MAIN = DMA ? WAVES * RING * STAGE : JOIN;
+  static_assert(JOIN <= MAIN, "the join's place");
+  __shared__ __attribute__((aligned(1024))) char sm[MAIN + 16 * TF * sizeof(int)];
+  int* sid = (int*)(sm + MAIN);
   const LowArgs& a = sets.set[blockIdx.z];
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, c = lane & 15;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
