@@ -40,6 +40,7 @@ struct MoeArgs {
 //   h, b: one 16x16x32 instruction;   s: four 16x16x4;   d: two 16x16x4
 typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
+typedef int i4_t __attribute__((ext_vector_type(4)));
 typedef double d2_t __attribute__((ext_vector_type(2)));
 
 template <typename T> struct Op;
@@ -93,6 +94,14 @@ template <typename T> __device__ inline typename Op<T>::vec load_part(const T* p
 #pragma unroll
   for (int i = 0; i < Op<T>::E; ++i) v[i] = i < m ? p[i] : (T)0;
   return v;
+}
+
+// the vector, or zeros
+template <typename V> __device__ inline V keep(V v, bool in) {
+  i4_t b = __builtin_bit_cast(i4_t, v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) b[i] = in ? b[i] : 0;
+  return __builtin_bit_cast(V, b);
 }
 
 // ---------------------------------------------------------------- intermediates between two products

@@ -223,9 +223,7 @@ __global__ __launch_bounds__(512) void k_few_apply(const T* __restrict__ x, long
         for (int g = 0; g < G; ++g) z[g] = *(const V*)(b + (fx ^ 64 * h) + g * 2048);
 #pragma unroll
         for (int f = 0; f < NF; ++f) {
-          V m = v[h][f];
-#pragma unroll
-          for (int i = 0; i < E; ++i) m[i] = in ? m[i] : (T)0;
+          const V m = keep(v[h][f], in);
 #pragma unroll
           for (int g = 0; g < G; ++g) acc[f][g] = Op<T>::mma(m, z[g], acc[f][g]);
         }

@@ -361,6 +361,24 @@ __global__ __launch_bounds__(64 * WAVES) void k_moe_up(const T* __restrict__ x, 
   }
 }
 
+// `left` steps in batches of MOST and one of what remains (in powers of two that would be up to three ways to memory: fp16,
+// 30 experts of 1000 x 728, 24 tokens: 48.7 us with those, 44.7 in one; nothing gained in the first product, whose
+// batches fill the registers)
+template <int MOST, class F> __device__ inline void in_batches(int left, F run) {
+  for (; left >= MOST; left -= MOST) run(Int<MOST>());
+  if constexpr (MOST > 4) {
+    if (left == 7) run(Int<7>());
+    if (left == 6) run(Int<6>());
+    if (left == 5) run(Int<5>());
+    if (left == 4) run(Int<4>());
+  }
+  if constexpr (MOST > 2) {
+    if (left == 3) run(Int<3>());
+    if (left == 2) run(Int<2>());
+  }
+  if (left == 1) run(Int<1>());
+}
+
 // ---------------------------------------------------------------- second product
 // y for 16 h and a batch of tokens.  A unit is one (expert in use, split of I); the units are divided evenly over the
 // workgroups that share these rows (blockIdx.z) and go round their 8 waves.  A unit leaves its slots' 16 values in LDS,
@@ -436,12 +454,7 @@ __global__ __launch_bounds__(512) void k_moe_down(const typename Mid<T>::elem* _
         }
         s += U;
       };
-      if constexpr (G == 1)
-        while (s + 8 <= whole) run(Int<8>());
-      if constexpr (G <= 2)
-        while (s + 4 <= whole) run(Int<4>());
-      while (s + 2 <= whole) run(Int<2>());
-      if (s < whole) run(Int<1>());
+      in_batches<G == 1 ? 8 : G == 2 ? 4 : 2>(whole - s, run);
       for (; s < s1; ++s) {
         const int left = I - s * KS - q * E;
         MidOp<T> f;
