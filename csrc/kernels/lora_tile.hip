@@ -39,7 +39,8 @@ template <typename T> __global__ __launch_bounds__(256) void k_low_dot(LowSets s
 //   DMA (rows begin at multiples of 16 bytes): each wave has a ring of LDS buffers of its own for steps of 128 bytes, laid
 //     out as in k_tile and filled straight from memory; no barrier before the join.  (Fragments read where they are used,
 //     16 rows x 64 bytes a load, come out of the L2 at 37 GB/s per CU, whole lines at 130.)
-//   else: fragments from any address.
+//   else: the same lines from any address through registers, two steps ahead (16 JF = 64, 3648 x 2015: 53.6 us with
+//     fragments straight from memory, 24 so).
 template <typename T, int JF, int TF, bool DMA>
 __global__ __launch_bounds__(DMA && JF * TF >= 4 ? 256 : 512) void k_low_tile(LowSets sets) {
   typedef typename Num<T>::acc R;
@@ -47,8 +48,7 @@ __global__ __launch_bounds__(DMA && JF * TF >= 4 ? 256 : 512) void k_low_tile(Lo
   constexpr int WAVES = DMA && JF * TF >= 4 ? 4 : 8, E = Op<T>::E, KS = Op<T>::KS;
   constexpr int RING = JF == 4 || JF + TF == 3 ? 3 : 4, LOADS = 2 * TF + 2 * JF, STAGE = LOADS * 1024;
   constexpr int JOIN = WAVES * 16 * (16 * TF + 1) * (int)sizeof(R);
-  constexpr int MAIN = DMA ? WAVES * RING * STAGE : JOIN;
-  static_assert(JOIN <= MAIN, "the join's place");
+  constexpr int BUFS = WAVES * (DMA ? RING : 1) * STAGE, MAIN = BUFS > JOIN ? BUFS : JOIN;
   __shared__ __attribute__((aligned(1024))) char sm[MAIN + 16 * TF * sizeof(int)];
   int* sid = (int*)(sm + MAIN);
   const LowArgs& a = sets.set[blockIdx.z];
@@ -122,30 +122,43 @@ __global__ __launch_bounds__(DMA && JF * TF >= 4 ? 256 : 512) void k_low_tile(Lo
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     } else {
       static_assert(TF == 1, "one fragment of tokens");
-      constexpr int U = JF <= 2 ? 4 : 2;
-      const T *px = x + min(c, rt - 1) * a.ldx + q * E, *pf[JF];
+      constexpr int BK = 2 * KS;
+      const int steps = (a.C + BK - 1) / BK, s0 = steps * w / WAVES, s1 = steps * (w + 1) / WAVES;
+      const int row = lane >> 3, chunk = (lane & 7) ^ row, fr = c * 128 + ((q ^ (c & 7)) << 4);
+      const T* p[LOADS];
 #pragma unroll
-      for (int i = 0; i < JF; ++i) pf[i] = f + min(16 * i + c, rj - 1) * a.ldf + q * E;
-      const int steps = (a.C + KS - 1) / KS, s0 = steps * w / WAVES, s1 = steps * (w + 1) / WAVES, whole = min(s1, a.C / KS);
-      int s = s0;
-      for (; s + U <= whole; s += U) {
-        V xv[U], fv[U][JF];
+      for (int k = 0; k < LOADS; ++k)
+        p[k] = (k < 2 ? x + min(row + 8 * k, rt - 1) * a.ldx : f + min(row + 8 * (k - 2), rj - 1) * a.ldf) + chunk * E;
+      V g[2][LOADS];
+      auto fetch = [&](V* v, int s) {
+        if (s >= s1) return;
+        const long long k0 = (long long)s * BK;
+        if (k0 + BK <= a.C) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          xv[u] = load_vec(px + (long long)(s + u) * KS);
+          for (int k = 0; k < LOADS; ++k) v[k] = load_vec(p[k] + k0);
+        } else {
 #pragma unroll
-          for (int i = 0; i < JF; ++i) fv[u][i] = load_vec(pf[i] + (long long)(s + u) * KS);
+          for (int k = 0; k < LOADS; ++k) v[k] = load_part(p[k] + k0, a.C - (int)k0 - chunk * E);
         }
+      };
+      char* b = sm + w * STAGE;
+      auto use = [&](const V* v) {
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int k = 0; k < LOADS; ++k) *(V*)(b + k * 1024 + lane * 16) = v[k];
 #pragma unroll
-          for (int i = 0; i < JF; ++i) acc[i][0] = Op<T>::mma(fv[u][i], xv[u], acc[i][0]);
-      }
-      for (; s < s1; ++s) {
-        const int left = a.C - s * KS - q * E;
-        const V xv = load_part(px + (long long)s * KS, left);
+        for (int half = 0; half < 2; ++half) {
+          const V xv = *(const V*)(b + (fr ^ (64 * half)));
 #pragma unroll
-        for (int i = 0; i < JF; ++i) acc[i][0] = Op<T>::mma(load_part(pf[i] + (long long)s * KS, left), xv, acc[i][0]);
+          for (int i = 0; i < JF; ++i) acc[i][0] = Op<T>::mma(*(const V*)(b + 2048 + (fr ^ (64 * half)) + i * 2048), xv, acc[i][0]);
+        }
+      };
+      fetch(g[0], s0);
+      for (int s = s0; s < s1; s += 2) {
+        fetch(g[1], s + 1);
+        use(g[0]);
+        if (s + 1 >= s1) break;
+        fetch(g[0], s + 2);
+        use(g[1]);
       }
     }
     const R scale = a.scale ? ((const R*)a.scale)[l] : R(1);
@@ -182,7 +195,7 @@ template <typename T> int run_low(const LowSets& sets, hipStream_t st) {
     auto wide = [](const void* q, long long ld) { return ((uintptr_t)q | (uintptr_t)(ld * sizeof(T))) % 16 == 0 && ld * (long long)sizeof(T) * 64 < (1ll << 30); };
     dma = dma && wide(s.x, s.ldx) && wide(s.F, s.ldf) && s.C % Op<T>::E == 0;
   }
-  const int jf = a.r <= 16 ? 1 : a.r <= 32 ? 2 : 4;
+  const int jf = a.r <= 16 ? 1 : a.r <= 32 || (!dma && sizeof(T) > 2) ? 2 : 4;  // (4 through registers spills in s and d)
   // two fragments of tokens, which halves the factors' traffic, where that leaves a workgroup for every CU
   const int tf = dma && sizeof(T) == 2 && a.nt >= 8192 ? 2 : 1;
   const dim3 grid(cdiv(a.nt, 16 * tf), cdiv(a.r, 16 * jf), sets.sets);
@@ -193,7 +206,9 @@ template <typename T> int run_low(const LowSets& sets, hipStream_t st) {
       return (int)hipGetLastError();
     }
   if (dma) jf == 1 ? go(k_low_tile<T, 1, 1, true>, 512) : jf == 2 ? go(k_low_tile<T, 2, 1, true>, 512) : go(k_low_tile<T, 4, 1, true>, 256);
-  else jf == 1 ? go(k_low_tile<T, 1, 1, false>, 512) : jf == 2 ? go(k_low_tile<T, 2, 1, false>, 512) : go(k_low_tile<T, 4, 1, false>, 512);
+  else if (jf == 1) go(k_low_tile<T, 1, 1, false>, 512);
+  else if (jf == 2) go(k_low_tile<T, 2, 1, false>, 512);
+  else if constexpr (sizeof(T) == 2) go(k_low_tile<T, 4, 1, false>, 512);
   return (int)hipGetLastError();
 }
 
@@ -209,7 +224,8 @@ template <typename T> int run_low(const LowSets& sets, hipStream_t st) {
 // features contiguous: 1.16 and 1.17).
 //   DMA: rows begin at multiples of 16 bytes and the tile's rows lie within 2^30 bytes: memory to LDS directly.
 //        A chunk past the rows' end is fetched from past the buffer descriptor's end, which reads as zero.
-//   else: through registers, 16 bytes from any address, with zeros past the rows' end.
+//   else: through registers, 16 bytes from any address, with zeros past the rows' end, one step ahead of the buffers on a
+//     128 tile and two on a 64 tile (bf16, 184 x 4429 x 704: 38.3 us with 4, 36.5 with 2; 4097^3: 302 with 2, 292 with 1).
 // LDS rows are 8 chunks of 16 bytes; chunk c of row i lies at c ^ (i & 7), so that the rows that a fragment read takes
 // the same chunk of lie in different banks (no conflicts by the counter).  W stored with its features contiguous (NT false) is kept as it comes,
 // [step][features], and read through the transposing LDS read: a group of 16 lanes takes 4 steps x 16 features; the
@@ -224,7 +240,8 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
   constexpr int THREADS = 64 * WT * WN, E = Op<T>::E, BK = 2 * Op<T>::KS, SLOT = B * 128;
   constexpr int FT = B / WT / 16, FN = B / WN / 16;
   constexpr int J = B * 8 / THREADS, CH = B / E;  // CH: chunks of a [step][features] row
-  static_assert(SLOTS >= 4 && (DMA || SLOTS == 4), "without DMA the step after next is in registers");
+  static_assert(SLOTS >= 4 && (DMA || SLOTS == 4), "without DMA the steps after next are in registers");
+  constexpr int SETS = DMA || B == 128 ? 1 : 2;  // of registers, a step each
   __shared__ __attribute__((aligned(1024))) char sm[SLOTS * SLOT];
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, c16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wt = wave / WN, wn = wave % WN;
@@ -244,7 +261,7 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
   const int wmask = CH / 2 - 1;
   auto turn = [&](int step) { return ((step & 3) + 4 * ((step >> 3) & 1)) & wmask; };
   auto wchunk = [&](int row, int pc) { return sizeof(T) == 2 ? 2 * ((pc >> 1) ^ turn(row)) + (pc & 1) : pc ^ (16 / E * (row / E & 3)); };
-  V gx[DMA ? 1 : J], gw[DMA ? 1 : J];
+  V gx[SETS][J], gw[SETS][J];  // (not in use with DMA)
   unsigned ox[DMA ? J : 1], ow[DMA ? J : 1];
   constexpr unsigned NOWHERE = 0x80000000u;
   if constexpr (DMA) {
@@ -286,25 +303,36 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
       for (int j = 0; j < J; ++j) dma_buffer(W, wbytes, slot + j * THREADS * 16, ow[j] + (unsigned)k0 * pitch, 0);
     }
   };
-  auto fetch = [&](int s) {
+  auto fetch = [&](V* vx, V* vw, int s) {
     const int k0 = place(s), left = a.C - k0 - xc * E;
+    auto px = [&](int j) { return x + (long long)min(xr + j * (THREADS / 8), rt - 1) * a.ldx + k0 + xc * E; };
+    auto pw = [&](int j) { return W + (long long)min(wr + j * (THREADS / 8), rn - 1) * a.ldw + k0 + xc * E; };
+    // inside the rows without a test per lane.  W's features past the tile are not used, but have to be there: what
+    // follows in the same row, or the row after it
+    if (NT ? k0 + BK <= a.C : k0 + BK < a.C && a.N >= E) {
 #pragma unroll
-    for (int j = 0; j < J; ++j) gx[j] = load_part(x + (long long)min(xr + j * (THREADS / 8), rt - 1) * a.ldx + k0 + xc * E, left);
+      for (int j = 0; j < J; ++j) vx[j] = load_vec(px(j));
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-      if (NT) {
-        gw[j] = load_part(W + (long long)min(wr + j * (THREADS / 8), rn - 1) * a.ldw + k0 + xc * E, left);
-      } else {
-        const int row = wr + j * (THREADS / CH), n = wchunk(row, tid % CH) * E;
-        gw[j] = load_part(W + (long long)(k0 + row) * a.ldw + n, k0 + row < a.C ? rn - n : 0);
+      for (int j = 0; j < J; ++j) {
+        const int row = wr + j * (THREADS / CH);
+        vw[j] = load_vec(NT ? pw(j) : W + (long long)(k0 + row) * a.ldw + min(wchunk(row, tid % CH), (rn - 1) / E) * E);
       }
+    } else {
+#pragma unroll
+      for (int j = 0; j < J; ++j) vx[j] = load_part(px(j), left);
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int row = wr + j * (THREADS / CH), n = wchunk(row, tid % CH) * E;
+        vw[j] = NT ? load_part(pw(j), left) : load_part(W + (long long)(k0 + row) * a.ldw + n, k0 + row < a.C ? rn - n : 0);
+      }
+      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): lets the compiler count the loads under way where the paths meet
     }
   };
-  auto put = [&](char* sx, char* sw) {
+  auto put = [&](const V* vx, const V* vw, char* sx, char* sw) {
 #pragma unroll
-    for (int j = 0; j < J; ++j) *(V*)(sx + tid * 16 + j * THREADS * 16) = gx[j];
+    for (int j = 0; j < J; ++j) *(V*)(sx + tid * 16 + j * THREADS * 16) = vx[j];
 #pragma unroll
-    for (int j = 0; j < J; ++j) *(V*)(sw + tid * 16 + j * THREADS * 16) = gw[j];
+    for (int j = 0; j < J; ++j) *(V*)(sw + tid * 16 + j * THREADS * 16) = vw[j];
   };
 
   typename Op<T>::out acc[FN][FT];
@@ -382,40 +410,46 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
       for (int k = 0; k < SLOTS; ++k) k & 1 ? stage_w(k / 2, own + k * SLOT) : stage_x(k / 2, own + k * SLOT);
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"(J * (SLOTS - 2)) : "memory");
     } else {
-      fetch(0);
-      put(sm, sm + SLOT);
-      fetch(1);
-      put(sm + 2 * SLOT, sm + 3 * SLOT);
-      fetch(2);
+      fetch(gx[0], gw[0], 0);
+      if (SETS == 1) put(gx[0], gw[0], sm, sm + SLOT);
+      fetch(gx[SETS - 1], gw[SETS - 1], 1);
+      if (SETS > 1) put(gx[0], gw[0], sm, sm + SLOT);
+      put(gx[SETS - 1], gw[SETS - 1], sm + 2 * SLOT, sm + 3 * SLOT);
+#pragma unroll
+      for (int u = 0; u < SETS; ++u) fetch(gx[u], gw[u], u + 2);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
     meet();
     read(one, sm + sx, sm + sw, 0);
-    for (int s = 0; s < steps; ++s) {
-      read(two, sm + sx, sm + sw, 1);
-      multiply(one);
-      pace(0);
-      // step s + 1 has arrived, and this step is in registers: its buffers are free
-      if constexpr (DMA) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(J * (SLOTS - 4)) : "memory");
-      else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      meet();
-      const int fx0 = sx, fw0 = sw;
-      sx = next(sx);
-      sw = next(sw);
-      read(one, sm + sx, sm + sw, 0);
-      if constexpr (!DMA) {
-        put(sm + fx0, sm + fw0);
-        fetch(s + 3);
-      } else if constexpr (SLOTS & 1) {  // an odd number: the operands change places
-        stage_w(s + SLOTS / 2, own + fx0);
-        stage_x(s + SLOTS / 2 + 1, own + fw0);
-      } else {
-        stage_x(s + SLOTS / 2, own + fx0);
-        stage_w(s + SLOTS / 2, own + fw0);
+    for (int s0 = 0; s0 < steps; s0 += SETS)
+#pragma unroll
+      for (int u = 0; u < SETS; ++u) {
+        const int s = s0 + u;
+        if (SETS > 1 && s >= steps) break;
+        read(two, sm + sx, sm + sw, 1);
+        multiply(one);
+        pace(0);
+        // step s + 1 has arrived, and this step is in registers: its buffers are free
+        if constexpr (DMA) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(J * (SLOTS - 4)) : "memory");
+        else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        meet();
+        const int fx0 = sx, fw0 = sw;
+        sx = next(sx);
+        sw = next(sw);
+        read(one, sm + sx, sm + sw, 0);
+        if constexpr (!DMA) {
+          put(gx[u], gw[u], sm + fx0, sm + fw0);
+          fetch(gx[u], gw[u], s + 2 + SETS);
+        } else if constexpr (SLOTS & 1) {  // an odd number: the operands change places
+          stage_w(s + SLOTS / 2, own + fx0);
+          stage_x(s + SLOTS / 2 + 1, own + fw0);
+        } else {
+          stage_x(s + SLOTS / 2, own + fx0);
+          stage_w(s + SLOTS / 2, own + fw0);
+        }
+        multiply(two);
+        pace(1);
       }
-      multiply(two);
-      pace(1);
-    }
     // nothing is on its way to LDS when the workgroup ends
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   }
