@@ -140,9 +140,16 @@ __global__ __launch_bounds__(1024) void k_one(const T* __restrict__ x, const T* 
 }
 
 // 16 NF output features per workgroup, the contraction split over 8 waves and joined in LDS; G groups of 16 tokens.
-// W's fragments go straight from memory to the matrix instruction (each element is used by one wave once); x comes
-// from the caches.  A wave has one batch of fragments under way after another, as large as the registers of one
-// workgroup per CU allow; what the adapters' parts need is asked for before and beside them.
+// W's fragments go straight from memory to the matrix instruction (each element is used by one wave once); what the
+// adapters' parts need is asked for before and beside them.  x comes from the caches, and that is what bounds more than
+// a few tokens: 16 rows x 64 bytes a load, as the matrix instruction takes it, come out of the L2 at 37 GB/s per CU, whole
+// lines at 115 to 130.
+//   LINES (x's rows begin at multiples of 16 bytes): x in steps of 128 bytes of a row through a ring of LDS buffers that
+//     each wave fills for itself, straight from memory (rows laid out as in k_tile); W four steps ahead in registers.
+//   else: x in fragments from any address, in batches as large as the registers of one workgroup per CU allow.
+// (T x K x N, us without and with LINES: 48 x 4096 x 8192 30.5, 27.3; 48 x 4096 x 4096 23.0, 16.4; 48 x 1024 x 4096 12.0,
+// 10.8; 16 x 4096 x 8192 24.5, 20.5; 16 x 1024 x 4096 9.0, 9.2.)  What is left at 48 x 4096 x 8192: the way through
+// memory of the low-rank vectors, 5 us, and the beginning and end of one round of workgroups around 67 MB at 4.4 TB/s.
 constexpr int S_MAX = 64;  // r up to which the low-rank vectors go through LDS
 
 template <typename T, int G, int NF, bool LINES>
@@ -375,9 +382,9 @@ template <typename T> int run(const LoraArgs& g, hipStream_t st) {
     return (int)hipGetLastError();
   }
   if (g.L > 0) k_few_low<T><<<dim3(g.T, cdiv(g.r, 4)), 256, 0, st>>>(X, g.ldx, A, g.lda, ids, (const R*)g.scale, g.K, g.r, g.L, S);
-  // two fragments of features for a fragment of tokens where that leaves a workgroup for every CU: x is read half as
-  // often, and what a CU can have under way is the bound (48 tokens, 4096 x 8192: 43.4 us with one, 30.6 with two; 48
-  // tokens, 4096 x 4096: 23.2 with one, 27.0 with two)
+  // two fragments of features for a fragment of tokens where that leaves a workgroup for every CU: x is read half as often
+  // (48 tokens, 4096 x 8192: 32.3 us with one, 27.3 with two; 48 tokens, 4096 x 4096: 16.4 with one, 20.7 with two; 16
+  // tokens, 4096 x 8192: 20.5 and 21.8)
   const int nf = sizeof(T) < 8 && g.T > 16 && g.N >= 32 * 256 ? 2 : 1;
   auto apply = [&](auto kernel) {
     kernel<<<cdiv(g.N, 16 * nf), 512, 0, st>>>(X, g.ldx, W, g.ldw, B, g.ldb, ids, S, g.T, g.K, g.N, g.r, g.L, (R)g.alpha, (R)g.beta,
@@ -385,7 +392,7 @@ template <typename T> int run(const LoraArgs& g, hipStream_t st) {
   };
   const int groups = cdiv(g.T, 16);
   if constexpr (sizeof(T) < 8) {
-    const bool lines = ((uintptr_t)X | (uintptr_t)(g.ldx * sizeof(T))) % 16 == 0 && g.K % Op<T>::E == 0 && g.K >= 64 * Op<T>::KS &&
+    const bool lines = ((uintptr_t)X | (uintptr_t)(g.ldx * sizeof(T))) % 16 == 0 && g.K % Op<T>::E == 0 && g.K >= (groups > 1 ? 16 : 64) * Op<T>::KS &&
                        g.ldx * (long long)sizeof(T) * 64 < (1ll << 30);
     auto pick = [&](auto f, auto l) {
       constexpr int F = decltype(f)::value;

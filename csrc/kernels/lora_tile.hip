@@ -215,13 +215,16 @@ template <typename T> int run_low(const LowSets& sets, hipStream_t st) {
 // ---------------------------------------------------------------- shared product
 // A workgroup owns B tokens x B features, WT x WN waves of (B / WT) x (B / WN).  The contraction goes in steps of 128
 // bytes of a row (whole cache lines: with 64-byte steps the same lines were asked for twice, 1.12 against 1.13 PFLOP/s at
-// 16384 x 4096 x 16384, and 1.26 against 1.38 where all of it lies in the L2) through a ring of LDS buffers, each step in two halves of one fragment.  While a half is multiplied
-// from registers the fragments of the next one are read from LDS; when a step's second half is in registers its buffers
-// take a later step.  So neither latency is waited for, and a step has one barrier.  SLOTS buffers, each of one
-// operand's part of a step, X and W in turn: 4 (a step ahead) where several workgroups share a CU, 8 where few share the
-// chip and a step's products are much shorter than the way from memory, and 5, all of the LDS, with the largest tile: X
-// then has two steps to arrive (16384 x 4096 x 16384: 1.28 PFLOP/s with 4, 1.37 with 5; W two steps: the same; W's
-// features contiguous: 1.16 and 1.17).
+// 16384 x 4096 x 16384, and 1.26 against 1.38 where all of it lies in the L2) through LDS buffers, each step in two
+// halves of one fragment.  While a half is multiplied from registers the fragments of the next one are read from LDS;
+// when a step's second half is in registers its buffers take a later step.  So neither latency is waited for, and a step
+// has one barrier.  SLOTS buffers, each of one operand's part of a step, X and W in turn: 4 (a step ahead) where several
+// workgroups share a CU, 8 where few share the chip and a step's products are much shorter than the way from memory, and
+// 5, all of the LDS, with the largest tile: X then has two steps to arrive (16384 x 4096 x 16384: 1.25 PFLOP/s with 4,
+// 1.31 with 5, W's features contiguous 1.20 and 1.37; W two steps instead of X: the same).
+// What bounds the largest tile: half a step reads 96 KB of fragments from LDS in the 1024 cycles that its products take,
+// and the waits for loads.  (4 waves of 128 x 128 would read a third less, but with 256 accumulators a lane the compiler
+// moves them about: 1.04 PFLOP/s.)
 //   DMA: rows begin at multiples of 16 bytes and the tile's rows lie within 2^30 bytes: memory to LDS directly.
 //        A chunk past the rows' end is fetched from past the buffer descriptor's end, which reads as zero.
 //   else: through registers, 16 bytes from any address, with zeros past the rows' end, one step ahead of the buffers on a
