@@ -319,12 +319,15 @@ template <typename T> __global__ __launch_bounds__(256) void k_join(OuterArgs a)
   }
 }
 
-// places in all, and a window's length: about 512 workgroups, in whole steps, a window's tokens in LDS; few tokens stay
-// in one window, which needs no join
+// places in all, and a window's length: about 96 workgroups for each factor, so that both together are one round of the
+// CUs with the ends of adapters (one each: the buffers take most of a CU's LDS), and few parts to join, in whole steps, a
+// window's tokens in LDS; few tokens stay in one window, which needs no join.  (Both factors, us with 96 and with 512:
+// 8192 tokens, 4096 and 16384 features, r 64, 8 adapters 277, 325; 4096 tokens, 4096 features, r 16 47.4, 52.5; 2048
+// tokens, 2048 features, r 32 35.4, 34.8.)
 long long places(const LoraArgs& g) { return cdiv(g.T, 8) * 8ll + 8ll * (g.L + 1); }
 int window(const LoraArgs& g, int C) {
   if (places(g) <= 512) return 512;
-  const int tiles = cdiv(C, COLS) * cdiv(g.r, 64), parts = max(1, 512 / max(1, tiles));
+  const int tiles = cdiv(C, COLS) * cdiv(g.r, 64), parts = max(1, 96 / max(1, tiles));
   return min(WIN_MAX, max(256, cdiv(cdiv(g.T, parts), 64) * 64));
 }
 

@@ -222,9 +222,10 @@ template <typename T> int run_low(const LowSets& sets, hipStream_t st) {
 // workgroups share a CU, 8 where few share the chip and a step's products are much shorter than the way from memory, and
 // 5, all of the LDS, with the largest tile: X then has two steps to arrive (16384 x 4096 x 16384: 1.25 PFLOP/s with 4,
 // 1.31 with 5, W's features contiguous 1.20 and 1.37; W two steps instead of X: the same).
-// What bounds the largest tile: half a step reads 96 KB of fragments from LDS in the 1024 cycles that its products take,
-// and the waits for loads.  (4 waves of 128 x 128 would read a third less, but with 256 accumulators a lane the compiler
-// moves them about: 1.04 PFLOP/s.)
+// What bounds the largest tile: power.  At 16384 x 4096 x 16384 (1.67 ms) the matrix pipes are busy 71 % of the time (W's
+// features contiguous: 80 %) at the 1.77 (1.72) GHz that the card's limit leaves; the library's product runs at 85 % and
+// 1.50 GHz, 1.64 to 1.70 ms.  (4 waves of 128 x 128 would read a third less from LDS, but with 256 accumulators a lane the
+// compiler moves them about: 1.04 PFLOP/s.)
 //   DMA: rows begin at multiples of 16 bytes and the tile's rows lie within 2^30 bytes: memory to LDS directly.
 //        A chunk past the rows' end is fetched from past the buffer descriptor's end, which reads as zero.
 //   else: through registers, 16 bytes from any address, with zeros past the rows' end, one step ahead of the buffers on a
