@@ -31,11 +31,11 @@ struct PrepareArgs {
 };
 
 // dst[l][c][r] = src[l][r][c], rows of dst padded with zeros to ldd; 64 x 64 elements per workgroup
-template <typename T> __device__ inline void turn_tile(const PrepareArgs::Turn& a, int block) {
+template <typename T> __device__ inline void turn_tile(const PrepareArgs::Turn& a, long long block) {
   __shared__ T s[64][66];
   const int tr = (a.ldd + 63) / 64;
   const long long m = block / a.wgs;
-  const int in = block % a.wgs, r0 = in % tr * 64, c0 = in / tr * 64, tid = threadIdx.x;
+  const int in = (int)(block % a.wgs), r0 = in % tr * 64, c0 = in / tr * 64, tid = threadIdx.x;
   const T* src = (const T*)a.src;
   T v[16];
 #pragma unroll
@@ -96,11 +96,13 @@ template <typename M> __device__ inline void sort_one(const PrepareArgs& a, int 
 }
 
 template <typename T> __global__ __launch_bounds__(256) void k_prepare(PrepareArgs a) {
-  int b = blockIdx.x;
-  if (b < a.L) return sort_one<typename Mid<T>::elem>(a, b);
-  b -= a.L;
-  if (b < a.turn[0].wgs * a.L) return turn_tile<T>(a.turn[0], b);
-  turn_tile<T>(a.turn[1], b - a.turn[0].wgs * a.L);
+  const long long first = (long long)a.turn[0].wgs * a.L, all = a.L + first + (long long)a.turn[1].wgs * a.L;
+  for (long long b = blockIdx.x; b < all; b += gridDim.x) {
+    if (b < a.L) sort_one<typename Mid<T>::elem>(a, (int)b);
+    else if (b - a.L < first) turn_tile<T>(a.turn[0], b - a.L);
+    else turn_tile<T>(a.turn[1], b - a.L - first);
+    __syncthreads();
+  }
 }
 
 // ---------------------------------------------------------------- gradients of the factors
@@ -386,7 +388,7 @@ template <typename T> int run(const LoraArgs& g, hipStream_t st) {
     PrepareArgs a{ids, w.off, w.perm, w.pos, w.zeros, {w.pthi, w.ptlo, w.sthi, w.stlo}, w.tp, g.T, g.L, g.r, {}};
     if (p && g.N > 0) a.turn[0] = {g.B, w.Bt, g.ldb, w.ldb, g.N, g.r, cdiv(w.ldb, 64) * cdiv(g.r, 64)};
     if (low && w.dx) a.turn[1] = {g.A, w.At, g.lda, w.rp, g.r, g.K, cdiv(w.rp, 64) * cdiv(g.K, 64)};
-    k_prepare<T><<<(unsigned)(g.L * (1ll + a.turn[0].wgs + a.turn[1].wgs)), 256, 0, st>>>(a);
+    k_prepare<T><<<(unsigned)min(1ll << 20, g.L * (1ll + a.turn[0].wgs + a.turn[1].wgs)), 256, 0, st>>>(a);
   }
   int rc = 0;
   if (p || s) {

@@ -17,7 +17,8 @@ are multiplied by the 16-bit matrix instructions and summed in 32 bits; each res
 A taskpool runs on the stream that is current when it is run, takes the operands' and indices' values of that moment,
 makes no allocation and no host synchronisation, and may be captured into a HIP graph.  It owns its workspace, so one
 taskpool (and every graph that captured it) has one run in flight at a time, and it lives as long as those graphs.
-Outputs must not overlap inputs.
+Outputs must not overlap inputs.  An infinity or NaN in one adapter, expert, token or output's weights makes what it meets
+infinite or NaN (in h and b an infinity of a factor may come out as NaN) and nothing else.
 """
 from __future__ import annotations
 
@@ -29,6 +30,8 @@ from ..runtime import Taskpool
 
 _LIMIT = 4194240      # tokens or features: 65535 tiles of 64 along one grid axis
 _FAMILY = 65535       # adapters: one grid axis
+_RANK = 262140        # 65535 groups of 4 along one grid axis
+_FACTORS = 2 ** 23    # adapters times tiles of 256 features: the workgroups of the factors' gradients
 
 
 def _matrix(op, ctx, name, M, m, n, dtype):
@@ -124,6 +127,8 @@ def _lora_checks(op, ctx, W, X, A, B, ids, scale, N, outputs, others):
     if max(T, K, N, r) > _LIMIT or L > _FAMILY:
         raise ValueError(f"{op}: at most {_LIMIT} tokens or features and {_FAMILY} adapters, got T = {T}, K = {K}, "
                          f"N = {N}, r = {r}, L = {L}")
+    if r > _RANK:
+        raise ValueError(f"{op}: at most rank {_RANK}, got {r}")
     _vector(op, ctx, "ids", ids, T, torch.int32)
     if scale is not None:
         _vector(op, ctx, "scale", scale, L, torch.float64 if dtype is torch.float64 else torch.float32)
@@ -181,6 +186,8 @@ def gemm_lora_grad_New(ctx, alpha, W, X, A, B, ids, scale, dY, dX, dA, dB) -> Ta
             if nb:
                 _family(op, name, M, nb)
     _lora_checks(op, ctx, W, X, A, B, ids, scale, N, [o[:2] for o in outputs if o[1] is not None], [("dY", dY)])
+    if A.n // r * -(-max(K, N) // 256) > _FACTORS:
+        raise ValueError(f"{op}: {A.n // r} adapters of {max(K, N)} features are more than {_FACTORS} tiles of 256")
     return _pool(ctx, op,
                  lambda: ops.lora_call(ctx.device, float(alpha), W, X, A, B, ids, scale, dY=dY, dX=dX, dA=dA, dB=dB),
                  lambda: ops.lora_grad_cpu(float(alpha), W, X, A, B, ids, scale, dY, dX, dA, dB),

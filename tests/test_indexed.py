@@ -225,3 +225,17 @@ def test_run_of_a_lone_task_is_traced(ctx, tmp_path):
     finally:
         dp.profiling_stop(ctx, str(tmp_path / "t.json"))
     assert "GEMM_LORA" in (tmp_path / "t.json").read_text()
+
+
+def test_extents_past_a_launch_are_refused(ctx):
+    """Ranks and families that no grid holds (storage that is never touched)."""
+    r = 262144
+    W, X, Y = matrix(torch.zeros(1, 1)), matrix(torch.zeros(2, 1)), matrix(torch.zeros(2, 1))
+    A, Bd, ids = matrix(torch.empty(r, 1), r), matrix(torch.empty(1, r), 1), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="rank"):
+        dp.gemm_lora(ctx, 1.0, W, X, A, Bd, ids, None, 0.0, Y)
+    L, K = 65535, 33000
+    W, X, Y = matrix(torch.empty(1, K, dtype=H)), matrix(torch.empty(2, K, dtype=H)), matrix(torch.empty(2, 1, dtype=H))
+    A, Bd = matrix(torch.empty(L, K, dtype=H), 1), matrix(torch.empty(L, 1, dtype=H), 1)
+    with pytest.raises(ValueError, match="tiles of 256"):
+        dp.gemm_lora_grad(ctx, 1.0, W, X, A, Bd, ids, None, Y, matrix(torch.empty(2, K, dtype=H)), None, None)

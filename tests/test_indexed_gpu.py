@@ -435,3 +435,28 @@ def test_traced_run(ctx, tmp_path):
     finally:
         dp.profiling_stop(ctx, str(tmp_path / "t.json"))
     assert "GEMM_LORA" in (tmp_path / "t.json").read_text()
+
+
+def test_lora_grad_of_many_adapters(ctx):
+    """More than 2^20 pieces of preparation, so that a workgroup takes several."""
+    c = lora(B, 70, 1024, 8, 1, 60000, "tokens")
+    c.ids[:] = torch.randint(0, 60000, (70,), generator=torch.Generator().manual_seed(2)).to(torch.int32)
+    c.ids[:3] = torch.tensor([59999, 0, 59999], dtype=torch.int32)
+    x, w, a, b, dy = (v.double() for v in (c.x, c.w, c.a, c.b, c.dy))
+    dx, da, db = c.backward(ctx, 0.5)
+    lid = c.ids.long()
+    s = c.scale.double()[lid, None, None]
+    p, q = s * dy[:, None, :] @ b[lid], s * x[:, None, :] @ a[lid].transpose(1, 2)
+    # one rounding of the result, and within 2^-13 of the magnitudes: sums of at most 1024 + 70 + 8 + 16 products
+    # in 32 bits (1118 2^-24 < 2^-13.8), the split intermediate (2^-16) and the rounding of these errors with the result
+    want = 0.5 * (dy @ w + (p @ a[lid])[:, 0])
+    room = 0.5 * (dy.abs() @ w.abs() + (p.abs() @ a[lid].abs())[:, 0])
+    assert ((dx.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -13 * room).all()
+    da_, db_ = torch.zeros_like(a), torch.zeros_like(b)
+    da_.index_add_(0, lid, 0.5 * p.transpose(1, 2) * x[:, None, :])
+    db_.index_add_(0, lid, 0.5 * dy[:, :, None] * q)
+    room_a, room_b = torch.zeros_like(a), torch.zeros_like(b)
+    room_a.index_add_(0, lid, 0.5 * (s * dy[:, None, :].abs() @ b[lid].abs()).transpose(1, 2) * x[:, None, :].abs())
+    room_b.index_add_(0, lid, 0.5 * dy[:, :, None].abs() * (s * x[:, None, :].abs() @ a[lid].abs().transpose(1, 2)))
+    assert ((da.double() - da_).abs() <= 2.0 ** -8 * da_.abs() + 2.0 ** -13 * room_a).all()
+    assert ((db.double() - db_).abs() <= 2.0 ** -8 * db_.abs() + 2.0 ** -13 * room_b).all()
