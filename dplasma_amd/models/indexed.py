@@ -15,8 +15,9 @@ Precisions: s and d, and the half precisions h (fp16) and b (bf16), which the ot
 are multiplied by the 16-bit matrix instructions and summed in 32 bits; each result is rounded once.
 
 A taskpool runs on the stream that is current when it is run, takes the operands' and indices' values of that moment,
-makes no allocation and no host synchronisation, and may be captured into a HIP graph.  It owns its workspace, so one
-taskpool (and every graph that captured it) has one run in flight at a time, and it lives as long as those graphs.
+makes no allocation and no host synchronisation, and may be captured into a HIP graph (moe's is built before the
+capture).  It owns its workspace, so one taskpool (and every graph that captured it) has one run in flight at a time, and
+it lives as long as those graphs.
 Outputs must not overlap inputs.  An infinity or NaN in one adapter, expert, token or output's weights makes what it meets
 infinite or NaN (in h and b an infinity of a factor may come out as NaN) and nothing else.
 """

@@ -47,6 +47,9 @@ class _Call:
         self.name, self.args = name, args
         self.index = torch.cuda.current_device() if device.index is None else device.index
         self.keep = keep  # tensors whose addresses the record holds
+        if zero and torch.cuda.is_current_stream_capturing():
+            # the zeros would be written by the graph's replays, and a run before the first one would read what was there
+            raise RuntimeError(f"{name[4:]}: build the taskpool before the capture that runs it")
         self.ws = torch.empty(max(256, ws_bytes), dtype=torch.uint8, device=device)
         self.ws[:zero].zero_()
         self.home = torch.cuda.current_stream(device).cuda_stream

@@ -460,3 +460,11 @@ def test_lora_grad_of_many_adapters(ctx):
     room_b.index_add_(0, lid, 0.5 * dy[:, :, None].abs() * (s * x[:, None, :].abs() @ a[lid].abs().transpose(1, 2)))
     assert ((da.double() - da_).abs() <= 2.0 ** -8 * da_.abs() + 2.0 ** -13 * room_a).all()
     assert ((db.double() - db_).abs() <= 2.0 ** -8 * db_.abs() + 2.0 ** -13 * room_b).all()
+
+
+def test_moe_is_built_before_a_capture(ctx, monkeypatch):
+    m = moe(B, 3, 64, 32, 4, 2)
+    G, W1, W2, X = m.descriptors()
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="before the capture"):
+        dp.moe_New(ctx, 2, True, G, W1, W2, 1.0, X, 0.0, matrix(m.y))
