@@ -331,16 +331,16 @@ template <typename T> __global__ __launch_bounds__(256) void k_join(OuterArgs a)
   }
 }
 
-// places in all, and a window's length: about 96 workgroups for each factor, so that both together are one round of the
-// CUs with the ends of adapters (one each: the buffers take most of a CU's LDS), and few parts to join, in whole steps, a
-// window's tokens in LDS; few tokens stay in one window, which needs no join.  (Both factors, us with 96 and with 512:
-// 8192 tokens, 4096 and 16384 features, r 64, 8 adapters 277, 325; 4096 tokens, 4096 features, r 16 47.4, 52.5; 2048
-// tokens, 2048 features, r 32 35.4, 34.8.)
+// places in all, and a window's length: about 192 workgroups for both factors, which with the ends of adapters is one
+// round of the CUs (one each: the buffers take most of a CU's LDS) and leaves few parts to join, in whole steps, a window's
+// tokens in LDS; few tokens stay in one window, which needs no join.  (Both factors, us so and with 512 workgroups for
+// each: 8192 tokens, 4096 and 16384 features, r 64, 8 adapters 271, 325; 4096 tokens, 4096 features, r 16 43.0, 48; 2048
+// tokens, 2048 features, r 32 35.2, 34.8.)
 long long places(const LoraArgs& g) { return cdiv(g.T, 8) * 8ll + 8ll * (g.L + 1); }
-int window(const LoraArgs& g, int C) {
+int window(const LoraArgs& g) {
   if (places(g) <= 512) return 512;
-  const int tiles = cdiv(C, COLS) * cdiv(g.r, 64), parts = max(1, 96 / max(1, tiles));
-  return min(WIN_MAX, max(256, cdiv(cdiv(g.T, parts), 64) * 64));
+  const long long tiles = (long long)(cdiv(g.K, COLS) + cdiv(g.N, COLS)) * cdiv(g.r, 64);
+  return (int)min((long long)WIN_MAX, max(256ll, (g.T * tiles / 192 + 63) / 64 * 64));
 }
 
 template <typename T> struct GradWs {
@@ -352,7 +352,7 @@ template <typename T> struct GradWs {
   int4* zeros;
   R *pa = nullptr, *pb = nullptr;
   bool dx, da, db;
-  int rp, ldb, wa, wb;
+  int rp, ldb, win;
   long long tp;
   size_t bytes;
   GradWs(const LoraArgs& g, void* ws) {
@@ -362,8 +362,7 @@ template <typename T> struct GradWs {
     rp = low_pitch(g.prec, g.r);
     ldb = cdiv(g.N, 8) * 8;
     tp = (places(g) + 63) / 64 * 64 + 64;
-    wa = window(g, g.K);
-    wb = window(g, g.N);
+    win = window(g);
     Carve c{(char*)ws};
     zeros = c.take<int4>(1);
     off = c.take<int>(g.L + 1);
@@ -378,12 +377,12 @@ template <typename T> struct GradWs {
     if (da) {
       pthi = c.take<M>(g.r * tp);
       if (Mid<T>::PARTS == 2) ptlo = c.take<M>(g.r * tp);
-      pa = c.take<R>((size_t)2 * (places(g) / wa + 1) * g.r * g.K);
+      pa = c.take<R>((size_t)2 * (places(g) / win + 1) * g.r * g.K);
     }
     if (db) {
       sthi = c.take<M>(g.r * tp);
       if (Mid<T>::PARTS == 2) stlo = c.take<M>(g.r * tp);
-      pb = c.take<R>((size_t)2 * (places(g) / wb + 1) * g.r * g.N);
+      pb = c.take<R>((size_t)2 * (places(g) / win + 1) * g.r * g.N);
     }
     bytes = c.used;
   }
@@ -417,8 +416,8 @@ template <typename T> int run(const LoraArgs& g, hipStream_t st) {
   if (rc || !(w.da || w.db)) return rc;
   OuterArgs a{{}, w.off, w.perm, w.zeros, w.tp, g.alpha, g.r, g.L, 0};
   auto wgs = [&](const OuterSet& o) { return o.out ? cdiv(o.C, COLS) * o.items : 0; };
-  if (w.da) a.set[0] = {g.X, w.pthi, w.ptlo, g.dA, w.pa, g.ldx, g.ldda, g.K, w.wa, (int)(places(g) / w.wa) + g.L, 1};
-  if (w.db) a.set[1] = {g.dY, w.sthi, w.stlo, g.dB, w.pb, g.ldy, g.lddb, g.N, w.wb, (int)(places(g) / w.wb) + g.L, 0};
+  if (w.da) a.set[0] = {g.X, w.pthi, w.ptlo, g.dA, w.pa, g.ldx, g.ldda, g.K, w.win, (int)(places(g) / w.win) + g.L, 1};
+  if (w.db) a.set[1] = {g.dY, w.sthi, w.stlo, g.dB, w.pb, g.ldy, g.lddb, g.N, w.win, (int)(places(g) / w.win) + g.L, 0};
   a.wgs0 = wgs(a.set[0]);
   auto aligned = [&](const OuterSet& o) { return !o.out || (((uintptr_t)o.z | (uintptr_t)(o.ldz * sizeof(T))) % 16 == 0 && o.C % Op<T>::E == 0); };
   const bool dma = aligned(a.set[0]) && aligned(a.set[1]);
@@ -428,7 +427,7 @@ template <typename T> int run(const LoraArgs& g, hipStream_t st) {
   if (jf == 1) dma ? go(k_outer<T, 1, true>) : go(k_outer<T, 1, false>);
   else if (jf == 2) dma ? go(k_outer<T, 2, true>) : go(k_outer<T, 2, false>);
   else dma ? go(k_outer<T, 4, true>) : go(k_outer<T, 4, false>);
-  if ((w.da && places(g) > w.wa) || (w.db && places(g) > w.wb)) {
+  if (places(g) > w.win) {
     const long long most = (long long)g.r * max(w.da ? g.K : 0, w.db ? g.N : 0);
     k_join<T><<<dim3((unsigned)min(512ll, (most + 255) / 256), g.L, 2), 256, 0, st>>>(a);
   }
