@@ -185,7 +185,10 @@ __global__ __launch_bounds__(DMA && JF * TF >= 4 ? 256 : 512) void k_low_tile(Lo
 
 template <typename T> int run_low(const LowSets& sets, hipStream_t st) {
   const LowArgs& a = sets.set[0];
-  if (a.nt <= 256) {
+  // one wave per (token, j) for few tokens, and up to 512 where a tile's tokens would go through several adapters one after
+  // the other (us in all, by tiles and so: 300 x 4096 x 1024, r 32, 16 adapters 36.1, 31.0; 413 x 2040 x 5001, r 12, 9
+  // adapters 38.6, 36.0; 512 x 4096 x 4096, r 16, one adapter 37.9, 38.9; 500 x 4096 x 1024, r 64, 16 adapters 42.0, 44.0)
+  if (a.nt <= 256 || (a.nt <= 512 && a.r <= 32 && a.L > 1)) {
     k_low_dot<T><<<dim3(a.nt, cdiv(a.r, 4), sets.sets), 256, 0, st>>>(sets);
     return (int)hipGetLastError();
   }
