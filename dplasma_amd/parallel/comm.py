@@ -199,6 +199,11 @@ def bcast(t: torch.Tensor, src_global: int, group, world: bool = False) -> None:
     _rec_coll("bcast", t, group)
     if world and not (dist.is_initialized() and dist.get_world_size() > 1):
         return
+    if _staged(t):
+        h = t.cpu()
+        dist.broadcast(h, src=src_global, group=group)
+        t.copy_(h)
+        return
     w = dist.broadcast(t, src=src_global, group=group, async_op=True)
     w.wait()
 
@@ -219,6 +224,12 @@ def _nccl() -> bool:
     return dist.get_backend() == "nccl"
 
 
+def _staged(t: torch.Tensor) -> bool:
+    """Whether a collective on ``t`` goes through host memory: gloo's own collectives on device tensors are not used
+    (with several ranks on one GPU they have hung)."""
+    return t.device.type == "cuda" and not _nccl()
+
+
 def allgather_inplace(out: torch.Tensor, my_index: int, group) -> None:
     """out is [n_in_group, ...] contiguous; slot my_index already holds my contribution."""
     if _BACKEND is not None and hasattr(_BACKEND, "sync"):
@@ -231,6 +242,12 @@ def allgather_inplace(out: torch.Tensor, my_index: int, group) -> None:
         w = dist.all_gather_into_tensor(out.view(-1), inp.reshape(-1),
                                         group=group, async_op=True)
         w.wait()
+    elif _staged(out):
+        mine = inp.cpu()
+        parts = [torch.empty_like(mine) for _ in range(out.shape[0])]
+        dist.all_gather(parts, mine, group=group)
+        for slot, h in zip(out.unbind(0), parts):
+            slot.copy_(h)
     else:
         parts = list(out.unbind(0))
         mine = inp.clone()
@@ -244,6 +261,11 @@ def allreduce(t: torch.Tensor, op=dist.ReduceOp.SUM, group=None) -> None:
     if not (dist.is_available() and dist.is_initialized()) or dist.get_world_size() == 1:
         return
     _rec_coll("allreduce", t, group)
+    if _staged(t):
+        h = t.cpu()
+        dist.all_reduce(h, op=op, group=group)
+        t.copy_(h)
+        return
     dist.all_reduce(t, op=op, group=group)
 
 
