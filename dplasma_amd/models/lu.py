@@ -1117,8 +1117,7 @@ def _permute_rows_2d(ctx, A, dst_rows, src_rows, coltiles):
                 for w, pr in pairs(src_rows[sends[q]], slot, True).items():
                     ops.row_gather(sbuf, A.data, pr, w, 1, A.ld)
             slot += len(sends[q]) * nct
-        dist.all_to_all_single(rbuf, sbuf, output_split_sizes=rcount, input_split_sizes=scount,
-                               group=ctx.col_group)
+        comm.alltoall(rbuf, sbuf, rcount, scount, group=ctx.col_group)
     if len(local) and nct:
         for w, pr in pairs(dst_rows[local], 0, False).items():
             ops.row_gather(A.data, tmp, pr, w, A.ld, 1)

@@ -19,6 +19,7 @@ import torch
 from ..constants import dplasmaLeft, dplasmaNoTrans, dplasmaNonUnit, dplasmaUpper
 from ..descriptor import TiledMatrix
 from ..ops import lu_incpiv_ops
+from ..parallel import comm
 from ..runtime.dag import TileDAG
 from ..runtime.taskpool import Taskpool
 from ..utils.flops import flops
@@ -79,9 +80,8 @@ def getrf_incpiv_New(ctx, A, L, IPIV, info_out=None) -> Taskpool:
     def _done():
         v = info.clone()
         if ctx.world > 1:
-            import torch.distributed as dist
             vv = v.to(ctx.device)
-            dist.all_reduce(vv, op=dist.ReduceOp.MAX)
+            comm.allreduce(vv, op=torch.distributed.ReduceOp.MAX)
             v = vv
         return int(v.item())
     tp.on_complete(_done)

@@ -255,6 +255,16 @@ def allgather_inplace(out: torch.Tensor, my_index: int, group) -> None:
         w.wait()
 
 
+def alltoall(recv: torch.Tensor, send: torch.Tensor, recv_splits, send_splits, group=None) -> None:
+    """dist.all_to_all_single of one-dimensional tensors, waited for by the current stream."""
+    if _staged(recv):
+        h = torch.empty(recv.shape, dtype=recv.dtype)
+        dist.all_to_all_single(h, send.cpu(), recv_splits, send_splits, group=group)
+        recv.copy_(h)
+        return
+    dist.all_to_all_single(recv, send, recv_splits, send_splits, group=group, async_op=True).wait()
+
+
 def allreduce(t: torch.Tensor, op=dist.ReduceOp.SUM, group=None) -> None:
     if _BACKEND is not None and hasattr(_BACKEND, "sync"):
         return _BACKEND.sync("allreduce", 2 * _nbytes(t), group)

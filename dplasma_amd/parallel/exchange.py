@@ -17,7 +17,6 @@ from __future__ import annotations
 from typing import Dict, List, Sequence, Tuple
 
 import torch
-import torch.distributed as dist
 
 from . import comm
 
@@ -114,6 +113,4 @@ class ExchangePlan:
         out_splits = [c * nbe for c in self.recv_counts]
         in_splits = [c * nbe for c in self.send_counts]
         comm._rec_coll("alltoall", None, None)
-        w = dist.all_to_all_single(recv[: self.nremote * nbe], sendbuf[: self.nsend * nbe], out_splits,
-                                   in_splits, async_op=True)
-        w.wait()
+        comm.alltoall(recv[: self.nremote * nbe], sendbuf[: self.nsend * nbe], out_splits, in_splits)
