@@ -32,6 +32,58 @@ __device__ inline s4_t read_turned(const char* __restrict__ p) {
 #endif
 }
 
+template <int N> struct Int {
+  static constexpr int value = N;
+};
+
+// The rows p[0 .. ROWS) against x by one wave, its lanes along the rows; every lane gets the sums.  4 loads of a row are
+// under way at a time (with 8 the low-rank vectors of 48 tokens, K = 4096, took 2.5 us longer: more code to fetch).
+template <int ROWS, typename T>
+__device__ inline void wave_dots(const T* const* p, const T* x, int K, typename Num<T>::acc* out) {
+  typedef typename Num<T>::acc R;
+  typedef typename Op<T>::vec V;
+  constexpr int E = Op<T>::E, STEP = 64 * E;
+  R s[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) s[i] = 0;
+  int k = (threadIdx.x & 63) * E, left = K / STEP;
+  auto run = [&](auto width) {
+    constexpr int U = decltype(width)::value;
+    V a[U][ROWS], b[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) a[u][i] = load_vec(p[i] + k + u * STEP);
+      b[u] = load_vec(x + k + u * STEP);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+        for (int e = 0; e < E; ++e) s[i] = fma((R)a[u][i][e], (R)b[u][e], s[i]);
+    k += U * STEP;
+    left -= U;
+  };
+  while (left >= 4) run(Int<4>());
+  if (left >= 2) run(Int<2>());
+  if (left) run(Int<1>());
+  if (k < K) {
+    const V b = load_part(x + k, K - k);
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const V a = load_part(p[i] + k, K - k);
+#pragma unroll
+      for (int e = 0; e < E; ++e) s[i] = fma((R)a[e], (R)b[e], s[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    for (int o = 32; o; o >>= 1) s[i] += __shfl_xor(s[i], o);
+    out[i] = s[i];
+  }
+}
+
 // T <= 64, forward (lora_few.hip)
 size_t lora_few_ws(const LoraArgs& g);
 int lora_few(const LoraArgs& g, hipStream_t st);

@@ -10,29 +10,17 @@ __global__ __launch_bounds__(256) void k_few_low(const T* __restrict__ x, long l
                                                  const typename Num<T>::acc* __restrict__ scale, int K, int r, int L,
                                                  typename Num<T>::acc* __restrict__ S) {
   typedef typename Num<T>::acc R;
-  constexpr int E = Op<T>::E;
   const int t = blockIdx.x, j = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int l = ids[t];
   if (j >= r) return;
   R s = 0;
   if ((unsigned)l < (unsigned)L) {
     const T* a = A + ((long long)l * r + j) * lda;
-    const T* p = x + (long long)t * ldx;
-#pragma unroll 4
-    for (int k = lane * E; k < K; k += 64 * E) {
-      const typename Op<T>::vec u = load_part(a + k, K - k), v = load_part(p + k, K - k);
-#pragma unroll
-      for (int i = 0; i < E; ++i) s = fma((R)u[i], (R)v[i], s);
-    }
-    for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
+    wave_dots<1>(&a, x + (long long)t * ldx, K, &s);
     s *= scale ? scale[l] : R(1);
   }
   if (lane == 0) S[(long long)t * r + j] = s;
 }
-
-template <int N> struct Int {
-  static constexpr int value = N;
-};
 
 // One token: rows of W and of its adapter's A against x, one wave per row with its lanes along K (whole lines).  8 waves
 // take the workgroup's 8 M features (M: 1 or 2) while 8 others make the low-rank vector, every workgroup for itself: A
@@ -50,55 +38,10 @@ __global__ __launch_bounds__(1024) void k_one(const T* __restrict__ x, const T* 
                                               int M, typename Num<T>::acc alpha, typename Num<T>::acc beta,
                                               T* __restrict__ y) {
   typedef typename Num<T>::acc R;
-  typedef typename Op<T>::vec V;
-  constexpr int E = Op<T>::E, STEP = 64 * E;
   __shared__ R low[ONE_R];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int l = L > 0 ? ids[0] : -1;
   const bool has = (unsigned)l < (unsigned)L;
-  // the rows p[0 .. ROWS) against x, in every lane
-  auto dots = [&](auto rows, const T* const* p, R* out) {
-    constexpr int ROWS = decltype(rows)::value;
-    R s[ROWS];
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) s[i] = 0;
-    int k = lane * E, left = K / STEP;
-    auto run = [&](auto width) {
-      constexpr int U = decltype(width)::value;
-      V a[U][ROWS], b[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-#pragma unroll
-        for (int i = 0; i < ROWS; ++i) a[u][i] = load_vec(p[i] + k + u * STEP);
-        b[u] = load_vec(x + k + u * STEP);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int i = 0; i < ROWS; ++i)
-#pragma unroll
-          for (int e = 0; e < E; ++e) s[i] = fma((R)a[u][i][e], (R)b[u][e], s[i]);
-      k += U * STEP;
-      left -= U;
-    };
-    while (left >= 4) run(Int<4>());
-    if (left >= 2) run(Int<2>());
-    if (left) run(Int<1>());
-    if (k < K) {
-      const V b = load_part(x + k, K - k);
-#pragma unroll
-      for (int i = 0; i < ROWS; ++i) {
-        const V a = load_part(p[i] + k, K - k);
-#pragma unroll
-        for (int e = 0; e < E; ++e) s[i] = fma((R)a[e], (R)b[e], s[i]);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-      for (int o = 32; o; o >>= 1) s[i] += __shfl_xor(s[i], o);
-      out[i] = s[i];
-    }
-  };
   if (w >= 8) {
     if (has) {
       const T* a = A + (long long)l * r * lda;
@@ -106,7 +49,7 @@ __global__ __launch_bounds__(1024) void k_one(const T* __restrict__ x, const T* 
       for (int j = w - 8; j < r; j += 16) {
         const T* p[2] = {a + j * lda, a + min(j + 8, r - 1) * lda};
         R v[2];
-        dots(Int<2>(), p, v);
+        wave_dots<2>(p, x, K, v);
         if (lane == 0) {
           low[j] = f * v[0];
           if (j + 8 < r) low[j + 8] = f * v[1];
@@ -119,8 +62,8 @@ __global__ __launch_bounds__(1024) void k_one(const T* __restrict__ x, const T* 
   const int n = blockIdx.x * M * 8 + w, n2 = M > 1 ? n + 8 : N;
   R v[2] = {0, 0}, f[2] = {0, 0};
   const T* p[2] = {W + min(n, N - 1) * ldw, W + min(n2, N - 1) * ldw};
-  if (n2 < N) dots(Int<2>(), p, v);
-  else if (n < N) dots(Int<1>(), p, v);
+  if (n2 < N) wave_dots<2>(p, x, K, v);
+  else if (n < N) wave_dots<1>(p, x, K, v);
   if (has && lane < r) {
     if (n < N) f[0] = widen(B[((long long)l * N + n) * ldb + lane]);
     if (n2 < N) f[1] = widen(B[((long long)l * N + n2) * ldb + lane]);

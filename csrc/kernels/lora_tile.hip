@@ -14,22 +14,14 @@ struct LowSets {
 // One wave per (token, j): for few tokens, where the tokens of a workgroup's rows would mostly have adapters of their own.
 template <typename T> __global__ __launch_bounds__(256) void k_low_dot(LowSets sets) {
   typedef typename Num<T>::acc R;
-  constexpr int E = Op<T>::E;
   const LowArgs& a = sets.set[blockIdx.z];
   const int t = blockIdx.x, j = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int l = a.ids[t];
   if (j >= a.r || (unsigned)l >= (unsigned)a.L) return;
   if (j == 0 && lane < a.out.rp - a.r) pad_low<T>(a.out, t, a.r + lane);
-  R s = 0;
+  R s;
   const T* f = (const T*)a.F + ((long long)l * a.r + j) * a.ldf;
-  const T* p = (const T*)a.x + (long long)t * a.ldx;
-#pragma unroll 4
-  for (int c = lane * E; c < a.C; c += 64 * E) {
-    const typename Op<T>::vec u = load_part(f + c, a.C - c), v = load_part(p + c, a.C - c);
-#pragma unroll
-    for (int i = 0; i < E; ++i) s = fma((R)u[i], (R)v[i], s);
-  }
-  for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
+  wave_dots<1>(&f, (const T*)a.x + (long long)t * a.ldx, a.C, &s);
   s *= a.scale ? ((const R*)a.scale)[l] : R(1);
   if (lane == 0) put_low<T>(a.out, t, j, s);
 }
