@@ -37,7 +37,7 @@ template <int N> struct Int {
 };
 
 // The rows p[0 .. ROWS) against x by one wave, its lanes along the rows; every lane gets the sums.  4 loads of a row are
-// under way at a time (with 8 the low-rank vectors of 48 tokens, K = 4096, took 2.5 us longer: more code to fetch).
+// under way at a time (with 8 the low-rank vectors of 48 tokens, K = 4096, took 2.5 us longer).
 template <int ROWS, typename T>
 __device__ inline void wave_dots(const T* const* p, const T* x, int K, typename Num<T>::acc* out) {
   typedef typename Num<T>::acc R;
