@@ -105,50 +105,89 @@ template <typename V> __device__ inline V keep(V v, bool in) {
 }
 
 // ---------------------------------------------------------------- intermediates between two products
-// A 32-bit result that is the next product's operand.  For h and b it goes to the 16-bit matrix instructions as two
-// bf16 numbers, hi + lo: 16 bits of it (off by at most 2^-16 of itself) over the whole range of 32-bit numbers -- one
-// 16-bit number would keep 8 bits, or overflow past 65504 in fp16 where the plain 32-bit intermediate does not.  The
-// second product's own operand is exact in one bf16 (b) or two (h); of the four products of an h pair the smallest
-// (lo lo, below 2^-16) is left out.  s and d keep their own type.
+// A 32-bit result that is the next product's operand.  It lies in memory as it is (64 bits in d).  For h and b it goes to
+// the 16-bit matrix instructions as three bf16 numbers of 8 bits each whose sum it is, over the whole range of 32-bit
+// numbers: nothing is rounded between the two products.  The second product's own operand is exact in one bf16 (b) or two
+// (h); of the six products of an h pair the smallest, below 2^-24 of the whole and so below the rounding of a 32-bit
+// product, is left out.  s and d take it as it is.
+//
+// Mem: a lane's intermediates as they come from memory, Op<T>::E of them.
+template <typename T> struct Mem {  // h, b
+  f4_t v[2];
+  __device__ inline void load(const float* p) {
+    v[0] = load_vec(p);
+    v[1] = load_vec(p + 4);
+  }
+  // zeros from the m-th on
+  __device__ inline void load_to(const float* p, int m) {
+    v[0] = load_part(p, m);
+    v[1] = load_part(p + 4, m - 4);
+  }
+};
+template <> struct Mem<float> {
+  f4_t v;
+  __device__ inline void load(const float* p) { v = load_vec(p); }
+  __device__ inline void load_to(const float* p, int m) { v = load_part(p, m); }
+};
+template <> struct Mem<double> {
+  d2_t v;
+  __device__ inline void load(const double* p) { v = load_vec(p); }
+  __device__ inline void load_to(const double* p, int m) { v = load_part(p, m); }
+};
+// Mid: the same as operands.
 template <typename T> struct Mid {  // h, b
-  typedef __bf16 elem;
-  static constexpr int PARTS = 2;
-  static __device__ inline void put(elem* hi, elem* lo, float v) {
-    const __bf16 h = (__bf16)v;
-    // an infinity has no remainder (inf - inf would make it NaN)
-    const float rest = v - (float)h;
-    *hi = h;
-    *lo = (__bf16)(__builtin_isfinite(rest) ? rest : 0.f);
+  b8_t part[3];
+  __device__ inline void set(const Mem<T>& m) {
+    i4_t w[3];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      unsigned u[3][2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        // by truncation: 8 bits, then the exact rest's 8, then the last 8.  An infinity has no rest (inf - inf would make
+        // it NaN)
+        const float x = m.v[i / 2][i % 2 * 2 + e];
+        u[0][e] = __float_as_uint(x);
+        float rest = x - __uint_as_float(u[0][e] & 0xffff0000u);
+        rest = rest == rest ? rest : 0.f;
+        u[1][e] = __float_as_uint(rest);
+        u[2][e] = __float_as_uint(rest - __uint_as_float(u[1][e] & 0xffff0000u));
+      }
+#pragma unroll
+      for (int p = 0; p < 3; ++p) w[p][i] = (int)__builtin_amdgcn_perm(u[p][1], u[p][0], 0x07060302);  // both upper halves
+    }
+#pragma unroll
+    for (int p = 0; p < 3; ++p) part[p] = __builtin_bit_cast(b8_t, w[p]);
   }
 };
 template <> struct Mid<float> {
-  typedef float elem;
-  static constexpr int PARTS = 1;
-  static __device__ inline void put(elem* hi, elem*, float v) { *hi = v; }
+  f4_t part;
+  __device__ inline void set(const Mem<float>& m) { part = m.v; }
 };
 template <> struct Mid<double> {
-  typedef double elem;
-  static constexpr int PARTS = 1;
-  static __device__ inline void put(elem* hi, elem*, double v) { *hi = v; }
+  d2_t part;
+  __device__ inline void set(const Mem<double>& m) { part = m.v; }
 };
-// The other operand of a Mid product: one vector, or hi and lo for h.
-template <typename T> struct MidOp {
-  typedef typename Op<typename Mid<T>::elem>::vec vec;
-  vec f;
+// The other operand of a Mid product, which is a sum of N of the instruction's: product k adds the k-th (product_first: with
+// the intermediate as the instruction's first operand).  One after the other on the same accumulators they would wait for
+// each other, so kernels with several accumulators put the loop over k outside.
+template <typename T> struct MidOp {  // s, d
+  static constexpr int N = 1;
+  typename Op<T>::vec f;
   __device__ inline void set(typename Op<T>::vec v) { f = v; }
-  __device__ inline typename Op<T>::out mma(vec hi, vec lo, typename Op<T>::out c) const {
-    c = Op<T>::mma(f, hi, c);
-    return Mid<T>::PARTS == 2 ? Op<T>::mma(f, lo, c) : c;
-  }
-  // the intermediate as the first operand
-  __device__ inline typename Op<T>::out mma_first(vec hi, vec lo, typename Op<T>::out c) const {
-    c = Op<T>::mma(hi, f, c);
-    return Mid<T>::PARTS == 2 ? Op<T>::mma(lo, f, c) : c;
-  }
+  __device__ inline typename Op<T>::out product(int, const Mid<T>& m, typename Op<T>::out c) const { return Op<T>::mma(f, m.part, c); }
+  __device__ inline typename Op<T>::out product_first(int, const Mid<T>& m, typename Op<T>::out c) const { return Op<T>::mma(m.part, f, c); }
+};
+template <> struct MidOp<__bf16> {
+  static constexpr int N = 3;
+  b8_t f;
+  __device__ inline void set(b8_t v) { f = v; }
+  __device__ inline f4_t product(int k, const Mid<__bf16>& m, f4_t c) const { return Op<__bf16>::mma(f, m.part[k], c); }
+  __device__ inline f4_t product_first(int k, const Mid<__bf16>& m, f4_t c) const { return Op<__bf16>::mma(m.part[k], f, c); }
 };
 template <> struct MidOp<_Float16> {
-  typedef b8_t vec;
-  vec f, g;
+  static constexpr int N = 5;
+  b8_t f, g;
   // 11 bits: the upper 8 by truncation, the rest exactly in the second number (none beside an infinity)
   __device__ inline void set(h8_t v) {
 #pragma unroll
@@ -158,16 +197,8 @@ template <> struct MidOp<_Float16> {
       g[i] = (__bf16)(rest == rest ? rest : 0.f);
     }
   }
-  __device__ inline f4_t mma(vec hi, vec lo, f4_t c) const {
-    c = Op<__bf16>::mma(f, hi, c);
-    c = Op<__bf16>::mma(f, lo, c);
-    return Op<__bf16>::mma(g, hi, c);
-  }
-  __device__ inline f4_t mma_first(vec hi, vec lo, f4_t c) const {
-    c = Op<__bf16>::mma(hi, f, c);
-    c = Op<__bf16>::mma(lo, f, c);
-    return Op<__bf16>::mma(hi, g, c);
-  }
+  __device__ inline f4_t product(int k, const Mid<_Float16>& m, f4_t c) const { return Op<__bf16>::mma(k < 3 ? f : g, m.part[k % 3], c); }
+  __device__ inline f4_t product_first(int k, const Mid<_Float16>& m, f4_t c) const { return Op<__bf16>::mma(m.part[k % 3], k < 3 ? f : g, c); }
 };
 
 // ---------------------------------------------------------------- workspace cursor

@@ -88,44 +88,32 @@ __device__ inline void wave_dots(const T* const* p, const T* x, int K, typename 
 size_t lora_few_ws(const LoraArgs& g);
 int lora_few(const LoraArgs& g, hipStream_t st);
 
-// Low-rank vectors of every token as the operand of the next product (Mid<T>::elem, hi and lo parts).
-//   by token:    hi[t * rp + j], zeros for j in r .. rp (rp: r in whole matrix steps)
-//   by adapter:  thi[j * tp + pos[t]], the tokens of an adapter next to each other (the gradients of its factors)
+// Low-rank vectors of every token, 32-bit numbers (64 in d) for the next product (Mem<T>).
+//   by_token:    [t * rp + j], zeros for j in r .. rp (rp: r in whole matrix steps)
+//   by_adapter:  [j * tp + pos[t]], the tokens of an adapter next to each other (the gradients of its factors)
 // Nothing is written for a token without an adapter, and nothing of it is used.
 struct LowOut {
-  void *hi, *lo;    // null: not asked for
-  void *thi, *tlo;  // null: not asked for
+  void *by_token, *by_adapter;  // null: not asked for
   const int* pos;
   long long tp;
   int rp;
 };
 
 template <typename T> __device__ inline void put_low(const LowOut& o, int t, int j, typename Num<T>::acc v) {
-  typedef typename Mid<T>::elem M;
-  M h, l;
-  Mid<T>::put(&h, &l, v);
-  if (o.hi) {
-    ((M*)o.hi)[(long long)t * o.rp + j] = h;
-    if (Mid<T>::PARTS == 2) ((M*)o.lo)[(long long)t * o.rp + j] = l;
-  }
-  if (o.thi) {
-    const long long at = j * o.tp + o.pos[t];
-    ((M*)o.thi)[at] = h;
-    if (Mid<T>::PARTS == 2) ((M*)o.tlo)[at] = l;
-  }
+  typedef typename Num<T>::acc R;
+  if (o.by_token) ((R*)o.by_token)[(long long)t * o.rp + j] = v;
+  if (o.by_adapter) ((R*)o.by_adapter)[j * o.tp + o.pos[t]] = v;
 }
 template <typename T> __device__ inline void pad_low(const LowOut& o, int t, int j) {
-  typedef typename Mid<T>::elem M;
-  if (!o.hi) return;
-  ((M*)o.hi)[(long long)t * o.rp + j] = (M)0;
-  if (Mid<T>::PARTS == 2) ((M*)o.lo)[(long long)t * o.rp + j] = (M)0;
+  typedef typename Num<T>::acc R;
+  if (o.by_token) ((R*)o.by_token)[(long long)t * o.rp + j] = R(0);
 }
 
 static inline int low_pitch(int prec, int r) {
   const int ks = prec == DPL_D ? 8 : prec == DPL_S ? 16 : 32;
   return cdiv(r, ks) * ks;
 }
-static inline size_t mid_bytes(int prec) { return prec == DPL_D ? 8 : prec == DPL_S ? 4 : 2; }
+static inline size_t mid_bytes(int prec) { return prec == DPL_D ? 8 : 4; }
 
 // out(t, j) = s_l sum_c x[t*ldx + c] F[(l*r + j)*ldf + c],  l = ids[t], for one or two sets of the same tokens.
 struct LowArgs {
@@ -140,7 +128,7 @@ int lora_low(const LowArgs* sets, int n, hipStream_t st);
 // y[t*ldy + n] = alpha (sum_c x[t*ldx + c] W(n, c) + sum_j low(t, j) F[(l*N + n)*ldf + j]) + beta y[t*ldy + n];
 // nt: W(n, c) = W[n*ldw + c], else W[c*ldw + n]
 struct TileArgs {
-  const void *x, *W, *F, *hi, *lo;
+  const void *x, *W, *F, *low;  // low: by token
   const int* ids;
   void* y;
   long long ldx, ldw, ldf, ldy;

@@ -19,15 +19,14 @@ namespace {
 
 // T > 64: the low-rank vectors, then the shared product that adds the adapters' parts
 struct ForwardWs {
-  char *hi, *lo;
+  char* low;
   int rp;
   size_t bytes;
   ForwardWs(const LoraArgs& g, void* ws) {
     rp = low_pitch(g.prec, g.r);
     const size_t n = (size_t)g.T * rp * mid_bytes(g.prec);
     Carve c{(char*)ws};
-    hi = c.take<char>(n);
-    lo = c.take<char>(n);
+    low = c.take<char>(n);
     bytes = c.used;
   }
 };
@@ -38,11 +37,11 @@ int forward(const LoraArgs& g, hipStream_t st) {
   if ((size_t)g.ws_bytes < w.bytes) return -2;
   const int* ids = (const int*)g.ids;
   if (g.L > 0) {
-    const LowArgs a{g.X, g.A, g.scale, ids, g.ldx, g.lda, g.prec, g.T, g.K, g.r, g.L, {w.hi, w.lo, nullptr, nullptr, nullptr, 0, w.rp}};
+    const LowArgs a{g.X, g.A, g.scale, ids, g.ldx, g.lda, g.prec, g.T, g.K, g.r, g.L, {w.low, nullptr, nullptr, 0, w.rp}};
     const int rc = lora_low(&a, 1, st);
     if (rc) return rc;
   }
-  return lora_tile({g.X, g.W, g.B, w.hi, w.lo, ids, g.Y, g.ldx, g.ldw, g.ldb, g.ldy, g.alpha, g.beta, g.prec, g.T, g.K, g.N, g.r, w.rp, g.L}, true, st);
+  return lora_tile({g.X, g.W, g.B, w.low, ids, g.Y, g.ldx, g.ldw, g.ldb, g.ldy, g.alpha, g.beta, g.prec, g.T, g.K, g.N, g.r, w.rp, g.L}, true, st);
 }
 
 }  // namespace

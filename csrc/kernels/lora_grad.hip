@@ -19,7 +19,7 @@ struct PrepareArgs {
   const int* ids;
   int *off, *perm, *pos;
   int4* zero;
-  void* low[4];  // places after an adapter's last token, up to a multiple of 8, are zeroed here (null: not in use)
+  void* low[2];  // places after an adapter's last token, up to a multiple of 8, are zeroed here (null: not in use)
   long long tp;
   int nt, L, r;
   struct Turn {
@@ -55,7 +55,7 @@ template <typename T> __device__ inline void turn_tile(const PrepareArgs::Turn& 
 
 // One workgroup per adapter reads all ids, each wave a run of them, so the order never depends on timing.  64 ids at a time,
 // 16 times that under way (the launch with 13416 ids: 23 us with a run for each thread, 12 so).
-template <typename M> __device__ inline void sort_one(const PrepareArgs& a, int l) {
+template <typename R> __device__ inline void sort_one(const PrepareArgs& a, int l) {
   __shared__ int sums[2][4];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   if (l == 0 && tid == 0) *a.zero = int4{0, 0, 0, 0};
@@ -100,15 +100,15 @@ template <typename M> __device__ inline void sort_one(const PrepareArgs& a, int 
       at += __popcll(m);
     });
   const int end = begin + count, pad = (8 - count % 8) % 8;
-  for (int k = 0; k < 4; ++k)
+  for (int k = 0; k < 2; ++k)
     if (a.low[k])
-      for (int i = tid; i < a.r * pad; i += 256) ((M*)a.low[k])[(i / pad) * a.tp + end + i % pad] = (M)0;
+      for (int i = tid; i < a.r * pad; i += 256) ((R*)a.low[k])[(i / pad) * a.tp + end + i % pad] = R(0);
 }
 
 template <typename T> __global__ __launch_bounds__(256) void k_prepare(PrepareArgs a) {
   const long long first = (long long)a.turn[0].wgs * a.L, all = a.L + first + (long long)a.turn[1].wgs * a.L;
   for (long long b = blockIdx.x; b < all; b += gridDim.x) {
-    if (b < a.L) sort_one<typename Mid<T>::elem>(a, (int)b);
+    if (b < a.L) sort_one<typename Num<T>::acc>(a, (int)b);
     else if (b - a.L < first) turn_tile<T>(a.turn[0], b - a.L);
     else turn_tile<T>(a.turn[1], b - a.L - first);
     __syncthreads();
@@ -121,9 +121,10 @@ template <typename T> __global__ __launch_bounds__(256) void k_prepare(PrepareAr
 // is finished here (one without tokens gets its zeros), others leave 32-bit parts that k_join adds in the order of the
 // windows: slot 2 w for the adapter that came in from window w - 1, 2 w + 1 for one that begins in w and goes on.
 // COLS columns per workgroup, 16 JF rows j.  Steps of 128 bytes of tokens go through a ring of LDS buffers: z as
-// [token][column], read across as W is in k_tile, low as [j][token] in its parts (both laid out as there).
+// [token][column], read across as W is in k_tile, low as [j][token] (both laid out as there; a step of h and b holds twice
+// 128 bytes of low, one such block for each of its two products).
 struct OuterSet {
-  const void *z, *thi, *tlo;
+  const void *z, *low;  // low: by adapter
   void *out, *part;
   long long ldz, ldo;
   int C, win, items, jc;  // jc: g is stored [j][c] (dA), else [c][j] (dB)
@@ -142,11 +143,15 @@ constexpr int COLS = 256, WIN_MAX = 2048;
 template <typename T, int JF, bool DMA> __global__ __launch_bounds__(256, 1) void k_outer(OuterArgs a) {
   typedef typename Num<T>::acc R;
   typedef typename Op<T>::vec V;
-  typedef typename Mid<T>::elem M;
-  typedef typename Op<M>::vec MV;
   constexpr int E = Op<T>::E, STEP = 2 * Op<T>::KS;  // tokens of a step
-  constexpr int FN = COLS / 64, CH = COLS / E, J = STEP * CH / 256;  // 4 waves of 64 columns; chunks of a row; per thread
-  constexpr int PARTS = JF == 1 ? 2 : Mid<T>::PARTS;  // (one part of 16 rows is half a load of the workgroup: taken twice)
+  constexpr int EL = 16 / (int)sizeof(R);            // tokens of a chunk of low
+  constexpr int CH = COLS / E, J = STEP * CH / 256;  // chunks of a row of z; of them per thread
+  // WJ x 4 / WJ waves of 16 JW rows j x 16 FN columns.  Every wave takes the numbers of low that it uses apart for itself,
+  // which with all of 64 rows is the longest part of a step in b: there two waves along j halve it (the whole gradient of
+  // 8192 tokens, 4096 and 16384 features, 8 adapters: 1103 us with one, 1083 with two).  In h z's numbers are taken apart
+  // too, and no division saves anything
+  constexpr int WJ = JF == 4 && __is_same(T, __bf16) ? 2 : 1, JW = JF / WJ, FN = COLS / 64 * WJ;
+  constexpr int BLOCKS = STEP / (8 * EL), PARTS = JF == 1 ? 2 : BLOCKS;  // (one of 16 rows is half a load of the workgroup: taken twice)
   constexpr int ZB = STEP * COLS * (int)sizeof(T), PB = JF * 16 * 128, STAGE = ZB + PARTS * PB, RING = DMA ? (JF == 1 ? 4 : 3) : 2;
   constexpr int PJ = PARTS * PB / 4096, LOADS = J + PJ;
   __shared__ __attribute__((aligned(1024))) char sm[RING * STAGE + WIN_MAX * sizeof(int)];
@@ -157,7 +162,7 @@ template <typename T, int JF, bool DMA> __global__ __launch_bounds__(256, 1) voi
   const int ct = (g.C + COLS - 1) / COLS, item = block / ct;
   const int c0 = block % ct * COLS, j0 = blockIdx.y * 16 * JF;
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, c16 = lane & 15;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wj = WJ > 1 ? wave & 1 : 0, wc = WJ > 1 ? wave >> 1 : wave;
   int l = 0;
   for (int hi = a.L - 1; l < hi;) {  // the largest adapter whose first item is not past this one
     const int mid = (l + hi + 1) >> 1;
@@ -168,7 +173,7 @@ template <typename T, int JF, bool DMA> __global__ __launch_bounds__(256, 1) voi
   T* out = (T*)g.out;
   // (copies: a pointer chosen per lane from the arguments would be loaded again, and waited for, in every step)
   const T* z = (const T*)g.z;
-  const M *thi = (const M*)g.thi, *tlo = Mid<T>::PARTS == 2 ? (const M*)g.tlo : thi;
+  const R* low = (const R*)g.low;
   const void* zero = a.zero;
   const long long ldz = g.ldz, tp = a.tp;
   const int C = g.C, r = a.r;
@@ -194,8 +199,9 @@ template <typename T, int JF, bool DMA> __global__ __launch_bounds__(256, 1) voi
   auto stage_low = [&](char* b, int s) {
 #pragma unroll
     for (int k = 0; k < PJ; ++k) {
-      const int id = tid + 256 * k, pt = id / (PB / 16), row = id % (PB / 16) >> 3, at = s + E * ((id & 7) ^ (row & 7));
-      const M* src = (pt ? tlo : thi) + min(j0 + row, r - 1) * tp + p0 + at;
+      const int id = tid + 256 * k, pt = BLOCKS > 1 ? id / (PB / 16) : 0, row = id % (PB / 16) >> 3;
+      const int at = s + 8 * EL * pt + EL * ((id & 7) ^ (row & 7));
+      const R* src = low + min(j0 + row, r - 1) * tp + p0 + at;
       dma_global(at < n ? (const void*)src : zero, b + ZB + wave * 1024 + k * 4096);
     }
   };
@@ -226,43 +232,53 @@ template <typename T, int JF, bool DMA> __global__ __launch_bounds__(256, 1) voi
 #pragma unroll
     for (int k = 0; k < J; ++k) *(V*)(b + (tid + 256 * k) * 16) = v[k];
   };
-  typename Op<T>::out acc[JF][FN];
+  typename Op<T>::out acc[JW][FN];
 #pragma unroll
-  for (int i = 0; i < JF; ++i)
+  for (int i = 0; i < JW; ++i)
 #pragma unroll
     for (int f = 0; f < FN; ++f) acc[i][f] = typename Op<T>::out{R(0), R(0), R(0), R(0)};
   const int ftr = (8 * q + (c16 >> 2)) * (COLS * 2) + (c16 & 3) * 8;
   const int tw = (c16 >> 2) + 4 * (q & 1);
-  const int fp = ZB + c16 * 128 + ((q ^ (c16 & 7)) << 4);
+  const int fp = ZB + wj * JW * 2048 + c16 * 128 + (((BLOCKS > 1 ? 2 * q : q) ^ (c16 & 7)) << 4);
   auto multiply = [&](int s) {
     const char* b = &sm[s / STEP % RING * STAGE];
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
-      MV hi[JF], lw[JF];
+      Mid<T> part[JW];
 #pragma unroll
-      for (int i = 0; i < JF; ++i) {
-        hi[i] = *(const MV*)(b + (fp ^ (64 * kk)) + i * 2048);
-        lw[i] = Mid<T>::PARTS == 2 ? *(const MV*)(b + (fp ^ (64 * kk)) + PB + i * 2048) : hi[i];
+      for (int i = 0; i < JW; ++i) {
+        Mem<T> mem;
+        if constexpr (BLOCKS > 1) {
+          mem.v[0] = *(const f4_t*)(b + fp + kk * PB + i * 2048);
+          mem.v[1] = *(const f4_t*)(b + (fp ^ 16) + kk * PB + i * 2048);
+        } else {
+          mem.v = *(const V*)(b + (fp ^ (64 * kk)) + i * 2048);
+        }
+        part[i].set(mem);
       }
+      MidOp<T> x[FN];
 #pragma unroll
       for (int f = 0; f < FN; ++f) {
         V across;
         if constexpr (sizeof(T) == 2) {
           typedef short s8_t __attribute__((ext_vector_type(8)));
-          const char* p = b + ftr + (((wave * FN + f) ^ tw) << 5) + kk * 32 * COLS * 2;
+          const char* p = b + ftr + (((wc * FN + f) ^ tw) << 5) + kk * 32 * COLS * 2;
           const s4_t v0 = read_turned(p), v1 = read_turned(p + 4 * COLS * 2);
           const s8_t both = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
           across = __builtin_bit_cast(V, both);
         } else {
 #pragma unroll
           for (int e = 0; e < E; ++e)
-            across[e] = *(const T*)(b + ((kk * Op<T>::KS + q * E + e) * COLS + ((wave * FN + f) ^ q) * 16 + c16) * (int)sizeof(T));
+            across[e] = *(const T*)(b + ((kk * Op<T>::KS + q * E + e) * COLS + ((wc * FN + f) ^ q) * 16 + c16) * (int)sizeof(T));
         }
-        MidOp<T> x;
-        x.set(across);
-#pragma unroll
-        for (int i = 0; i < JF; ++i) acc[i][f] = x.mma_first(hi[i], lw[i], acc[i][f]);
+        x[f].set(across);
       }
+#pragma unroll
+      for (int k = 0; k < MidOp<T>::N; ++k)
+#pragma unroll
+        for (int f = 0; f < FN; ++f)
+#pragma unroll
+          for (int i = 0; i < JW; ++i) acc[i][f] = x[f].product_first(k, part[i], acc[i][f]);
     }
   };
   auto meet = [&]() {
@@ -298,13 +314,13 @@ template <typename T, int JF, bool DMA> __global__ __launch_bounds__(256, 1) voi
   R* part = (R*)g.part + (long long)(2 * w + (lo >= w * g.win)) * a.r * g.C;
 #pragma unroll
   for (int f = 0; f < FN; ++f) {
-    const int c = c0 + (wave * FN + f) * 16 + c16;
+    const int c = c0 + (wc * FN + f) * 16 + c16;
     if (c >= g.C) continue;
 #pragma unroll
-    for (int i = 0; i < JF; ++i)
+    for (int i = 0; i < JW; ++i)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int j = j0 + 16 * i + out_row<T>(lane, k);
+        const int j = j0 + 16 * (wj * JW + i) + out_row<T>(lane, k);
         if (j >= a.r) continue;
         if (whole) out[where(j, c)] = (T)(alpha == R(0) ? R(0) : alpha * acc[i][f][k]);
         else part[g.jc ? (long long)j * g.C + c : (long long)c * a.r + j] = acc[i][f][k];
@@ -346,8 +362,7 @@ int window(const LoraArgs& g) {
 template <typename T> struct GradWs {
   int *off, *perm, *pos;
   typedef typename Num<T>::acc R;
-  typedef typename Mid<T>::elem M;
-  M *hi = nullptr, *lo = nullptr, *pthi = nullptr, *ptlo = nullptr, *sthi = nullptr, *stlo = nullptr;
+  R *p = nullptr, *pt = nullptr, *st = nullptr;  // P by token, P and S by adapter
   T *At = nullptr, *Bt = nullptr;
   int4* zeros;
   R *pa = nullptr, *pb = nullptr;
@@ -369,19 +384,16 @@ template <typename T> struct GradWs {
     perm = c.take<int>(places(g));
     pos = c.take<int>(g.T);
     if (dx) {
-      hi = c.take<M>((size_t)g.T * rp);
-      if (Mid<T>::PARTS == 2) lo = c.take<M>((size_t)g.T * rp);
+      p = c.take<R>((size_t)g.T * rp);
       At = c.take<T>((size_t)g.L * g.K * rp);
     }
     if (dx || da) Bt = c.take<T>((size_t)g.L * g.r * ldb);
     if (da) {
-      pthi = c.take<M>(g.r * tp);
-      if (Mid<T>::PARTS == 2) ptlo = c.take<M>(g.r * tp);
+      pt = c.take<R>(g.r * tp);
       pa = c.take<R>((size_t)2 * (places(g) / win + 1) * g.r * g.K);
     }
     if (db) {
-      sthi = c.take<M>(g.r * tp);
-      if (Mid<T>::PARTS == 2) stlo = c.take<M>(g.r * tp);
+      st = c.take<R>(g.r * tp);
       pb = c.take<R>((size_t)2 * (places(g) / win + 1) * g.r * g.N);
     }
     bytes = c.used;
@@ -394,7 +406,7 @@ template <typename T> int run(const LoraArgs& g, hipStream_t st) {
   const int* ids = (const int*)g.ids;
   const bool low = g.L > 0 && g.T > 0, p = low && (w.dx || w.da), s = low && w.db;
   if (g.L > 0) {
-    PrepareArgs a{ids, w.off, w.perm, w.pos, w.zeros, {w.pthi, w.ptlo, w.sthi, w.stlo}, w.tp, g.T, g.L, g.r, {}};
+    PrepareArgs a{ids, w.off, w.perm, w.pos, w.zeros, {w.pt, w.st}, w.tp, g.T, g.L, g.r, {}};
     if (p && g.N > 0) a.turn[0] = {g.B, w.Bt, g.ldb, w.ldb, g.N, g.r, cdiv(w.ldb, 64) * cdiv(g.r, 64)};
     if (low && w.dx) a.turn[1] = {g.A, w.At, g.lda, w.rp, g.r, g.K, cdiv(w.rp, 64) * cdiv(g.K, 64)};
     k_prepare<T><<<(unsigned)min(1ll << 20, g.L * (1ll + a.turn[0].wgs + a.turn[1].wgs)), 256, 0, st>>>(a);
@@ -405,19 +417,19 @@ template <typename T> int run(const LoraArgs& g, hipStream_t st) {
     int n = 0;
     if (p)
       a[n++] = {g.dY, w.Bt, g.scale, ids, g.ldy, w.ldb, g.prec, g.T, g.N, g.r, g.L,
-                {w.dx ? w.hi : nullptr, w.lo, w.da ? w.pthi : nullptr, w.ptlo, w.pos, w.tp, w.rp}};
+                {w.p, w.pt, w.pos, w.tp, w.rp}};
     if (s)
       a[n++] = {g.X, g.A, g.scale, ids, g.ldx, g.lda, g.prec, g.T, g.K, g.r, g.L,
-                {nullptr, nullptr, w.sthi, w.stlo, w.pos, w.tp, g.r}};
+                {nullptr, w.st, w.pos, w.tp, g.r}};
     rc = lora_low(a, n, st);
   }
   if (!rc && w.dx)
-    rc = lora_tile({g.dY, g.W, w.At, w.hi, w.lo, ids, g.dX, g.ldy, g.ldw, w.rp, g.lddx, g.alpha, 0.0, g.prec, g.T, g.N, g.K, g.r, w.rp, g.L}, false, st);
+    rc = lora_tile({g.dY, g.W, w.At, w.p, ids, g.dX, g.ldy, g.ldw, w.rp, g.lddx, g.alpha, 0.0, g.prec, g.T, g.N, g.K, g.r, w.rp, g.L}, false, st);
   if (rc || !(w.da || w.db)) return rc;
   OuterArgs a{{}, w.off, w.perm, w.zeros, w.tp, g.alpha, g.r, g.L, 0};
   auto wgs = [&](const OuterSet& o) { return o.out ? cdiv(o.C, COLS) * o.items : 0; };
-  if (w.da) a.set[0] = {g.X, w.pthi, w.ptlo, g.dA, w.pa, g.ldx, g.ldda, g.K, w.win, (int)(places(g) / w.win) + g.L, 1};
-  if (w.db) a.set[1] = {g.dY, w.sthi, w.stlo, g.dB, w.pb, g.ldy, g.lddb, g.N, w.win, (int)(places(g) / w.win) + g.L, 0};
+  if (w.da) a.set[0] = {g.X, w.pt, g.dA, w.pa, g.ldx, g.ldda, g.K, w.win, (int)(places(g) / w.win) + g.L, 1};
+  if (w.db) a.set[1] = {g.dY, w.st, g.dB, w.pb, g.ldy, g.lddb, g.N, w.win, (int)(places(g) / w.win) + g.L, 0};
   a.wgs0 = wgs(a.set[0]);
   auto aligned = [&](const OuterSet& o) { return !o.out || (((uintptr_t)o.z | (uintptr_t)(o.ldz * sizeof(T))) % 16 == 0 && o.C % Op<T>::E == 0); };
   const bool dma = aligned(a.set[0]) && aligned(a.set[1]);

@@ -463,8 +463,6 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
     if ((unsigned)l >= (unsigned)a.L) l = -1;
     lid[f] = l;
   }
-  typedef typename Mid<T>::elem M;
-  typedef typename Op<M>::vec MV;
   constexpr int NONE = 0x7fffffff;
   auto after = [&](int l) {  // the next larger adapter of this wave's tokens
     int next = NONE;
@@ -491,13 +489,18 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
         __builtin_amdgcn_sched_barrier(0);
         if (m == 0) continue;
         const long long at = (long long)min(t0 + (wt * FT + f) * 16 + c16, a.T - 1) * a.rp + j;
-        const MV hi = load_vec((const M*)a.hi + at), lo = Mid<T>::PARTS == 2 ? load_vec((const M*)a.lo + at) : hi;
+        Mem<T> mem;
+        mem.load((const R*)a.low + at);
+        Mid<T> low;
+        low.set(mem);
+        const typename Op<T>::out none = {R(0), R(0), R(0), R(0)};
+        typename Op<T>::out d[FN];
 #pragma unroll
-        for (int i = 0; i < FN; ++i) {
-          const typename Op<T>::out d = F[i].mma(hi, lo, typename Op<T>::out{R(0), R(0), R(0), R(0)});
-          const typename Op<T>::out none = {R(0), R(0), R(0), R(0)};
-          acc[i][f] += lid[f] == l ? d : none;
-        }
+        for (int k = 0; k < MidOp<T>::N; ++k)
+#pragma unroll
+          for (int i = 0; i < FN; ++i) d[i] = F[i].product(k, low, k ? d[i] : none);
+#pragma unroll
+        for (int i = 0; i < FN; ++i) acc[i][f] += lid[f] == l ? d[i] : none;
       }
     }
     j0 += Op<T>::KS;

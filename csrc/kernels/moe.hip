@@ -230,12 +230,10 @@ __global__ __launch_bounds__(256) void k_moe_route(const T* __restrict__ x, long
 
 template <typename T> struct MoeWs {
   typedef typename Num<T>::acc R;
-  typedef typename Mid<T>::elem M;
   int *arrived, *done, *joined, *ids;
-  R *wt, *part;
+  R *wt, *part, *act;
   double* zs;
   Used* used;
-  M *hi, *lo = nullptr;
   int batch, batches, tiles, shares;
   size_t zero, bytes;
   MoeWs(const MoeArgs& g, void* ws) {
@@ -255,8 +253,7 @@ template <typename T> struct MoeWs {
     zs = c.take<double>((size_t)g.T * g.E);
     used = c.take<Used>(batches);
     part = c.take<R>(shares > 1 ? (size_t)shares * g.T * tiles * 16 : 0);
-    hi = c.take<M>(n * g.I);
-    if (Mid<T>::PARTS == 2) lo = c.take<M>(n * g.I);
+    act = c.take<R>(n * g.I);
     bytes = c.used;
   }
 };
@@ -267,8 +264,7 @@ template <typename T> struct MoeWs {
 template <typename T, int G, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void k_moe_up(const T* __restrict__ x, long long ldx, const T* __restrict__ W1,
                                                 long long ld1, const Used* __restrict__ used, int batch, int topk, int H,
-                                                int I, typename Mid<T>::elem* __restrict__ hi0,
-                                                typename Mid<T>::elem* __restrict__ lo0) {
+                                                int I, typename Num<T>::acc* __restrict__ act) {
   typedef typename Num<T>::acc R;
   typedef typename Op<T>::vec V;
   constexpr int E = Op<T>::E, KS = Op<T>::KS;
@@ -354,7 +350,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_moe_up(const T* __restrict__ x, 
           gate[p] = v;
         } else if (i0 + i < I) {
           const long long at = ((long long)t0 * topk + out[p]) * I + i0 + i;
-          Mid<T>::put(hi0 + at, lo0 + at, v * (gate[p] / (R(1) + exp(-gate[p]))));
+          act[at] = v * (gate[p] / (R(1) + exp(-gate[p])));
         }
       }
     }
@@ -385,8 +381,7 @@ template <int MOST, class F> __device__ inline void in_batches(int left, F run) 
 // each output adds its slots' splits in a fixed order, and the last workgroup of a row tile to arrive adds the shares in
 // theirs: which one that is does not change the sum.
 template <typename T, int G>
-__global__ __launch_bounds__(512) void k_moe_down(const typename Mid<T>::elem* __restrict__ hi0,
-                                                  const typename Mid<T>::elem* __restrict__ lo0,
+__global__ __launch_bounds__(512, 4) void k_moe_down(const typename Num<T>::acc* __restrict__ act,
                                                   const T* __restrict__ W2, long long ld2,
                                                   const Used* __restrict__ used,
                                                   const typename Num<T>::acc* __restrict__ wt0, int T_, int batch,
@@ -394,9 +389,7 @@ __global__ __launch_bounds__(512) void k_moe_down(const typename Mid<T>::elem* _
                                                   typename Num<T>::acc beta, T* __restrict__ y, long long ldy,
                                                   typename Num<T>::acc* share, int* joined) {
   typedef typename Num<T>::acc R;
-  typedef typename Mid<T>::elem M;
   typedef typename Op<T>::vec V;
-  typedef typename Op<M>::vec MV;
   constexpr int E = Op<T>::E, KS = Op<T>::KS;
   __shared__ R part[SLOTS][17], weight[SLOTS];
   __shared__ short at_of[SLOTS][2];  // a slot's place and expert in use
@@ -424,33 +417,34 @@ __global__ __launch_bounds__(512) void k_moe_down(const typename Mid<T>::elem* _
     for (int skip = 0; skip < total; skip += 16 * G) {
       const int m = min(16 * G, total - skip);
       typename Op<T>::out acc[G];
-      int slot[G];
+      const R* pa[G];  // a lane's slot's intermediates
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         acc[g] = typename Op<T>::out{R(0), R(0), R(0), R(0)};
-        slot[g] = us->slot[b0 + skip + min(16 * g + c16, m - 1)];
+        pa[g] = act + ((long long)t0 * topk + us->slot[b0 + skip + min(16 * g + c16, m - 1)]) * I + q * E;
       }
-      auto at = [&](int g) { return ((long long)t0 * topk + slot[g]) * I + q * E; };
       int s = s0;
       auto run = [&](auto width) {  // all loads of a batch before its products: loads are waited for in their order
         constexpr int U = decltype(width)::value;
         V wv[U];
-        MV h[U][G], l[U][G];
+        Mem<T> h[U][G];
 #pragma unroll
         for (int u = 0; u < U; ++u) wv[u] = load_vec(pw + (long long)(s + u) * KS);
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int g = 0; g < G; ++g) {
-            h[u][g] = load_vec(hi0 + at(g) + (s + u) * KS);
-            l[u][g] = Mid<T>::PARTS == 2 ? load_vec(lo0 + at(g) + (s + u) * KS) : h[u][g];
-          }
+          for (int g = 0; g < G; ++g) h[u][g].load(pa[g] + (s + u) * KS);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           MidOp<T> f;
           f.set(wv[u]);
 #pragma unroll
-          for (int g = 0; g < G; ++g) acc[g] = f.mma(h[u][g], l[u][g], acc[g]);
+          for (int g = 0; g < G; ++g) {
+            Mid<T> m;
+            m.set(h[u][g]);
+#pragma unroll
+            for (int k = 0; k < MidOp<T>::N; ++k) acc[g] = f.product(k, m, acc[g]);
+          }
         }
         s += U;
       };
@@ -461,8 +455,12 @@ __global__ __launch_bounds__(512) void k_moe_down(const typename Mid<T>::elem* _
         f.set(load_part(pw + (long long)s * KS, left));
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-          const MV h = load_part(hi0 + at(g) + s * KS, left);
-          acc[g] = f.mma(h, Mid<T>::PARTS == 2 ? load_part(lo0 + at(g) + s * KS, left) : h, acc[g]);
+          Mem<T> h;
+          h.load_to(pa[g] + s * KS, left);
+          Mid<T> m;
+          m.set(h);
+#pragma unroll
+          for (int k = 0; k < MidOp<T>::N; ++k) acc[g] = f.product(k, m, acc[g]);
         }
       }
 #pragma unroll
@@ -530,10 +528,10 @@ template <typename T> int run(const MoeArgs& g, hipStream_t st) {
   // 8 waves while each has 8 steps (30 experts of 1000 x 728 in fp16: 27.3 us with 8 waves, 27.1 with 4)
   const int waves = g.H >= 64 * Op<T>::KS ? 8 : 4;
   auto up = [&](auto kernel) {
-    kernel<<<dim3(cdiv(g.I, 16), most, w.batches), 64 * waves, 0, st>>>(X, g.ldx, W1, g.ld1, w.used, w.batch, g.topk, g.H, g.I, w.hi, w.lo);
+    kernel<<<dim3(cdiv(g.I, 16), most, w.batches), 64 * waves, 0, st>>>(X, g.ldx, W1, g.ld1, w.used, w.batch, g.topk, g.H, g.I, w.act);
   };
   auto down = [&](auto kernel) {
-    kernel<<<dim3(w.tiles, w.batches, w.shares), 512, 0, st>>>(w.hi, w.lo, W2, g.ld2, w.used, w.wt, g.T, w.batch, g.topk, g.H, g.I, (R)g.alpha,
+    kernel<<<dim3(w.tiles, w.batches, w.shares), 512, 0, st>>>(w.act, W2, g.ld2, w.used, w.wt, g.T, w.batch, g.topk, g.H, g.I, (R)g.alpha,
                                                              (R)g.beta, (T*)g.Y, g.ldy, w.part, w.joined);
   };
   if (g.I > 0 && waves == 8) groups == 1 ? up(k_moe_up<T, 1, 8>) : groups == 2 ? up(k_moe_up<T, 2, 8>) : up(k_moe_up<T, 4, 8>);

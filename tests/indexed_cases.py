@@ -1,8 +1,8 @@
 """Plain 64-bit forms of the products whose matrix depends on the column, with bounds on what a kernel may be off by.
 
 The bounds hold element by element.  u is the result type's half step; a sum of n products in 32 bits (64 for d) is off
-by at most n e times the sum of the products' magnitudes, e = 2^-24 (2^-53).  The kernels for h and b hand a 32-bit
-intermediate to the 16-bit matrix instructions as two bf16 numbers, which keeps it to 2^-16 of itself.
+by at most n e times the sum of the products' magnitudes, e = 2^-24 (2^-53).  For h and b there is room
+for an intermediate that is kept to 2^-16 of itself (the kernels keep all of its 32 bits).
 """
 import torch
 

@@ -468,3 +468,92 @@ def test_moe_is_built_before_a_capture(ctx, monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     with pytest.raises(RuntimeError, match="before the capture"):
         dp.moe_New(ctx, 2, True, G, W1, W2, 1.0, X, 0.0, matrix(m.y))
+
+
+def _third(n, *lead):
+    """Rows [1, 2^-5, 2^-9, 0 ..] and [1, 2^-5, 0 ..] of n: against [1, 2^-4, 2^-8, 0 ..] they give 1 + 2^-9 + 2^-17, which
+    takes 18 bits, and 1 + 2^-9."""
+    rows = torch.zeros(2, n, dtype=D)
+    rows[:, :3] = torch.tensor([[1, 2.0 ** -5, 2.0 ** -9], [1, 2.0 ** -5, 0]], dtype=D)
+    one = torch.tensor([1, 2.0 ** -4, 2.0 ** -8] + [0] * (n - 3), dtype=D)
+    return rows, one
+
+
+@pytest.mark.parametrize("T", [70, 600])
+@pytest.mark.parametrize("dtype,b", [(B, 1.0), (H, 1.0), (H, 1 + 2.0 ** -10), (S, 1.0)])
+def test_low_rank_vectors_keep_32_bits(ctx, T, dtype, b):
+    """Two low-rank numbers that differ in their 18th bit, subtracted by the second product."""
+    c = lora(dtype, T, 24, 72, 2, 1, "one")
+    rows, one = _third(24)
+    c.w.zero_()
+    c.x[:], c.a[0] = one.to(c.x), rows.to(c.a)
+    c.b[0, :, 0], c.b[0, :, 1] = b, -b
+    # S is exact.  Its product with B is a sum of at most 12 numbers whose partial sums stay below 1.01, each rounded by
+    # 2^-24 at most, and what is left out of an fp16 pair is below 2^-24: 13 2^-24 1.01, times alpha, below 2^-10
+    y = c.forward(ctx, 1024.0, scale=False).double()
+    want = b * 2.0 ** -7
+    assert ((y - want).abs() <= 2.0 ** -10 + 2.0 ** -8 * want).all(), float((y - want).abs().max())
+    # dX = alpha (p_0 - p_1), the same numbers
+    rows, one = _third(72)
+    c.dy[:], c.b[0] = one.to(c.dy), rows.t().to(c.b)
+    c.a[0, 0], c.a[0, 1] = b, -b
+    dx = c.backward(ctx, 1024.0, scale=False)[0].double()
+    assert ((dx - want).abs() <= 2.0 ** -10 + 2.0 ** -8 * want).all(), float((dx - want).abs().max())
+
+
+@pytest.mark.parametrize("T", [70, 600, 5000])
+@pytest.mark.parametrize("dtype,z", [(B, 1.0), (H, 1.0), (H, 1 + 2.0 ** -10), (S, 1.0)])
+@pytest.mark.parametrize("r", [2, 20, 40])
+def test_gradients_of_the_factors_keep_32_bits(ctx, T, dtype, z, r):
+    """The low-rank numbers of even tokens are those of odd ones plus 2^-17, and the two meet opposite signs."""
+    c = lora(dtype, T, 24, 72, r, 1, "one")
+    sign = torch.where(torch.arange(T) % 2 == 0, z, -z)[:, None]
+    # Every product of parts is a multiple of 2^-19, and no more than 16 tokens of one sign come one after the other (an
+    # instruction adds 32), so partial sums below 2^4.1 are exact in 32 bits in any order.  What is left out of an fp16
+    # pair is 2^-10 of 2^-17 each; the result is rounded once.  Ranks past the first are not looked at
+    room = 2.0 ** -8 + 2.0 ** -10
+    for n, what in ((72, "a"), (24, "b")):
+        rows, one = _third(n)
+        every = one.repeat(T, 1)
+        every[1::2, 2] = 0
+        if what == "a":
+            c.dy[:], c.b[0, :, 0] = every.to(c.dy), rows[0].to(c.b)
+            c.x[:] = sign.to(c.x)
+            got = c.backward(ctx, 1.0, scale=False, want="a")[1][0, 0]
+        else:
+            c.x[:], c.a[0, 0] = every.to(c.x), rows[0].to(c.a)
+            c.dy[:] = sign.to(c.dy)
+            got = c.backward(ctx, 1.0, scale=False, want="b")[2][0, :, 0]
+        want = z * (T // 2) * 2.0 ** -17
+        assert ((got.double() - want).abs() <= room * want).all(), (what, got[:4].tolist(), want)
+
+
+@pytest.mark.parametrize("T,I", [(3, 2), (3, 256), (20, 2), (20, 256), (60, 2), (60, 256)])
+@pytest.mark.parametrize("dtype,b", [(B, 1.0), (H, 1.0), (H, 1 + 2.0 ** -10), (S, 1.0)])
+def test_moe_activations_keep_32_bits(ctx, T, I, dtype, b):
+    """Two activations, 32 + 2^-4 + 2^-12 and 32 + 2^-4, subtracted by the down projection (silu(32) is 32 in 32 bits)."""
+    c = moe(dtype, T, 40, I, 1, 1)
+    rows, one = _third(40)
+    c.x[:] = one.to(c.x)
+    c.w1.zero_()
+    c.w1[0, :I, 0] = 32
+    c.w1[0, I:I + 2] = rows.to(c.w1)
+    c.w2.zero_()
+    c.w2[0, :, 0], c.w2[0, :, 1] = b, -b
+    # as for the low-rank vectors, with partial sums below 33: 13 2^-24 33 1024 < 2^-5
+    y = c.forward(ctx, True, 1024.0).double()
+    want = b * 2.0 ** -2
+    assert ((y - want).abs() <= 2.0 ** -5 + 2.0 ** -8 * want).all(), float((y - want).abs().max())
+
+
+@pytest.mark.parametrize("case", [(H, 300, 520, 264, 24, 3, "runs", 0), (B, 300, 520, 264, 24, 3, "runs", 0),
+                                  (B, 700, 264, 520, 64, 5, "runs", 0), (H, 900, 201, 333, 40, 4, "tokens", 1)], ids=str)
+def test_lora_without_room_for_short_intermediates(ctx, case, monkeypatch):
+    """The bounds of sums in 32 bits alone, nothing for an intermediate of fewer bits."""
+    import indexed_cases
+    monkeypatch.setattr(indexed_cases, "split_eps", lambda dtype: 0.0)
+    c = lora(*case)
+    within(c.forward(ctx)[:, :c.N], *c.plain(), "y")
+    got = c.backward(ctx)
+    for one, (want, bound), what in zip((got[0][:, :c.K], *got[1:]), c.plain_backward(), ("dx", "da", "db")):
+        within(one, want, bound, what)
