@@ -16,12 +16,15 @@ are multiplied by the 16-bit matrix instructions and summed in 32 bits; each res
 
 A taskpool runs on the stream that is current when it is run, takes the operands' and indices' values of that moment,
 makes no allocation and no host synchronisation, and may be captured into a HIP graph (moe's is built before the
-capture).  It owns its workspace, so one taskpool (and every graph that captured it) has one run in flight at a time, and
-it lives as long as those graphs.
+capture).  Its operands are the storages that the descriptors have when it is built, and it holds on to them: a tensor
+that is bound to a descriptor later is another matrix's.  It owns its workspace, so one taskpool (and every graph that
+captured it) has one run in flight at a time, and it lives as long as those graphs.
 Outputs must not overlap inputs.  An infinity or NaN in one adapter, expert, token or output's weights makes what it meets
 infinite or NaN (in h and b an infinity of a factor may come out as NaN) and nothing else.
 """
 from __future__ import annotations
+
+import copy
 
 import torch
 
@@ -56,6 +59,11 @@ def _matrix(op, ctx, name, M, m, n, dtype):
         if M.ld < M.m or M.data.numel() < last:
             raise ValueError(f"{op}: {name}'s storage holds {M.data.numel()} elements, {last} are needed")
     return M
+
+
+def _bound(*matrices):
+    """Descriptors of the taskpool's own, with the storages of this moment (None stays None)."""
+    return [copy.copy(M) for M in matrices]
 
 
 def _vector(op, ctx, name, v, n, dtype):
@@ -161,6 +169,7 @@ def gemm_lora_New(ctx, alpha, W, X, A, B, ids, scale, beta, Y) -> Taskpool:
     N = Y.m
     _matrix(op, ctx, "Y", Y, N, X.n, _precision(op, X))
     _lora_checks(op, ctx, W, X, A, B, ids, scale, N, [("Y", Y)], [])
+    W, X, A, B, Y = _bound(W, X, A, B, Y)
     return _pool(ctx, op, lambda: ops.lora_call(ctx.device, float(alpha), W, X, A, B, ids, scale, float(beta), Y),
                  lambda: ops.lora_cpu(float(alpha), W, X, A, B, ids, scale, float(beta), Y),
                  2 * X.n * (X.m * N + A.nb * (X.m + N)))
@@ -189,6 +198,7 @@ def gemm_lora_grad_New(ctx, alpha, W, X, A, B, ids, scale, dY, dX, dA, dB) -> Ta
     _lora_checks(op, ctx, W, X, A, B, ids, scale, N, [o[:2] for o in outputs if o[1] is not None], [("dY", dY)])
     if A.n // r * -(-max(K, N) // 256) > _FACTORS:
         raise ValueError(f"{op}: {A.n // r} adapters of {max(K, N)} features are more than {_FACTORS} tiles of 256")
+    W, X, A, B, dY, dX, dA, dB = _bound(W, X, A, B, dY, dX, dA, dB)
     return _pool(ctx, op,
                  lambda: ops.lora_call(ctx.device, float(alpha), W, X, A, B, ids, scale, dY=dY, dX=dX, dA=dA, dB=dB),
                  lambda: ops.lora_grad_cpu(float(alpha), W, X, A, B, ids, scale, dY, dX, dA, dB),
@@ -228,6 +238,7 @@ def moe_New(ctx, topk, norm, G, W1, W2, alpha, X, beta, Y) -> Taskpool:
         raise ValueError(f"{op}: at most 65535 tokens, got {T}")
     _extent(op, H=H, I=2 * width, E=E * 2 * width)
     _disjoint(op, [("Y", Y)], [("G", G), ("W1", W1), ("W2", W2), ("X", X)])
+    G, W1, W2, X, Y = _bound(G, W1, W2, X, Y)
     return _pool(ctx, op, lambda: ops.moe_call(ctx.device, int(topk), bool(norm), G, W1, W2, float(alpha), X,
                                                float(beta), Y),
                  lambda: ops.moe_cpu(int(topk), bool(norm), G, W1, W2, float(alpha), X, float(beta), Y),

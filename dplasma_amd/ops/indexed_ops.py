@@ -39,6 +39,11 @@ def pointer(M):
     return M.data.data_ptr() + M.offset(0, 0) * M.data.element_size() if M.m and M.n else M.data.data_ptr()
 
 
+def _storages(*matrices):
+    """What the addresses of a record belong to: the tensors, as the descriptors can be given others."""
+    return [M.data for M in matrices if M is not None]
+
+
 class _Call:
     """A kernel call with its argument record and workspace; ``__call__`` enqueues it on the current stream."""
 
@@ -46,7 +51,7 @@ class _Call:
         """zero: bytes at the workspace's beginning that start as zeros (every run leaves them so)."""
         self.name, self.args = name, args
         self.index = torch.cuda.current_device() if device.index is None else device.index
-        self.keep = keep  # tensors whose addresses the record holds
+        self.keep = keep  # the storages whose addresses the record holds
         if zero and torch.cuda.is_current_stream_capturing():
             # the zeros would be written by the graph's replays, and a run before the first one would read what was there
             raise RuntimeError(f"{name[4:]}: build the taskpool before the capture that runs it")
@@ -88,7 +93,7 @@ def lora_call(device, alpha, W, X, A, B, ids, scale, beta=0.0, Y=None, dY=None, 
         a.lddx, a.ldda, a.lddb = (0 if M is None else M.ld for M in (dX, dA, dB))
     else:
         a.Y = pointer(Y)
-    keep = [W, X, A, B, ids, scale, Y, dY, dX, dA, dB]
+    keep = _storages(W, X, A, B, Y, dY, dX, dA, dB) + [ids, scale]
     return _Call(device, "dpl_lora_grad" if grad else "dpl_lora", a, lib.dpl_lora_ws_bytes(ctypes.byref(a), int(grad)),
                  keep)
 
@@ -100,7 +105,7 @@ def moe_call(device, topk, norm, G, W1, W2, alpha, X, beta, Y):
                 E=G.n, topk=topk, norm=int(norm))
     zero = _ll()
     size = lib.dpl_moe_ws_bytes(ctypes.byref(a), ctypes.byref(zero))
-    return _Call(device, "dpl_moe", a, size, [G, W1, W2, X, Y], zero.value)
+    return _Call(device, "dpl_moe", a, size, _storages(G, W1, W2, X, Y), zero.value)
 
 
 # ----------------------------------------------------------------------------- CPU path

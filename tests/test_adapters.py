@@ -239,3 +239,31 @@ def test_extents_past_a_launch_are_refused(ctx):
     A, Bd = matrix(torch.empty(L, K, dtype=H), 1), matrix(torch.empty(L, 1, dtype=H), 1)
     with pytest.raises(ValueError, match="tiles of 256"):
         dp.gemm_lora_grad(ctx, 1.0, W, X, A, Bd, ids, None, Y, matrix(torch.empty(2, K, dtype=H)), None, None)
+
+
+def _rebind(descriptors):
+    """Another tensor in the place of every descriptor's storage."""
+    for M in descriptors:
+        M.data = torch.full_like(M.data, float("nan"))
+
+
+def test_a_taskpool_keeps_its_storages(ctx):
+    """Tensors bound to the descriptors after a taskpool was built are not its operands."""
+    c, m = Lora(D, 6, 10, 7, 3, 4), Moe(D, 4, 8, 6, 5, 2)
+    ops, y = list(c.descriptors()), torch.zeros_like(c.y)
+    dY, outs = matrix(c.dy), [torch.zeros_like(v) for v in (c.x, c.a, c.b)]
+    dX, dA, dB = matrix(outs[0]), matrix(outs[1].view(-1, c.K), c.r), matrix(outs[2].view(-1, c.r), c.N)
+    Y = matrix(y)
+    one = dp.gemm_lora_New(ctx, 1.0, *ops, c.ids, c.scale, 0.0, Y)
+    two = dp.gemm_lora_grad_New(ctx, 1.0, *ops, c.ids, c.scale, dY, dX, dA, dB)
+    G, W1, W2, X = m.descriptors()
+    out = torch.zeros_like(m.y)
+    Z = matrix(out)
+    three = dp.moe_New(ctx, 2, True, G, W1, W2, 1.0, X, 0.0, Z)
+    _rebind([*ops, dY, dX, dA, dB, Y, G, W1, W2, X, Z])
+    for tp in (one, two, three):
+        tp.execute(ctx)
+    within(y, *c.plain(), "y")
+    for got, (want, bound), what in zip(outs, c.plain_backward(), ("dx", "da", "db")):
+        within(got, want, bound, what)
+    within(out, *m.plain(), "moe")

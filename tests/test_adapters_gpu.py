@@ -557,3 +557,32 @@ def test_lora_without_room_for_short_intermediates(ctx, case, monkeypatch):
     got = c.backward(ctx)
     for one, (want, bound), what in zip((got[0][:, :c.K], *got[1:]), c.plain_backward(), ("dx", "da", "db")):
         within(one, want, bound, what)
+
+
+def test_a_taskpool_keeps_its_storages(ctx):
+    """A taskpool's operands stay in memory when the descriptors are given other tensors and nobody else holds the old ones."""
+    c, m = lora(B, 40, 512, 320, 16, 4, "tokens"), moe(B, 12, 256, 96, 8, 2)
+    want, (back, _, _), mixed = c.plain(), c.plain_backward(), m.plain()
+    ops = list(c.descriptors())
+    Y, dY, dX = (matrix(v.clone()) for v in (c.y, c.dy, c.x))
+    G, W1, W2, X = m.descriptors()
+    Z = matrix(m.y.clone())
+    one = dp.gemm_lora_New(ctx, 1.0, *ops, c.ids, c.scale, 0.0, Y)
+    two = dp.gemm_lora_grad_New(ctx, 1.0, *ops, c.ids, c.scale, dY, dX, None, None)
+    three = dp.moe_New(ctx, 2, True, G, W1, W2, 1.0, X, 0.0, Z)
+    outs = [M.data for M in (Y, dX, Z)]
+    # no tensor of the program's own: what only the descriptors held would return to the allocator here ...
+    for name in ("x", "w", "a", "b", "dy"):
+        setattr(c, name, None)
+    for name in ("x", "g", "w1", "w2"):
+        setattr(m, name, None)
+    every = [*ops, Y, dY, dX, G, W1, W2, X, Z]
+    sizes = [M.data.numel() for M in every]
+    for M in every:
+        M.data = None
+    others = [torch.full((n,), NAN, dtype=B, device="cuda:0") for n in sizes for _ in range(2)]  # ... and be theirs
+    for tp in (one, two, three):
+        tp.execute(ctx)
+    for got, (value, bound), what in zip(outs, (want, back, mixed), ("y", "dx", "moe")):
+        within(got, value, bound, what)
+    assert all(torch.isnan(o).all() for o in others)
