@@ -241,7 +241,7 @@ template <typename T> struct MoeWs {
     batches = cdiv(g.T, batch);
     tiles = cdiv(g.H, 16);
     // workgroups that share the second product of 16 rows: about 512 of 8 waves in all
-    shares = max(1, min(MAX_SHARES, 512 / max(1, tiles * batches)));
+    shares = (int)max(1ll, min((long long)MAX_SHARES, 512 / max(1ll, (long long)tiles * batches)));
     Carve c{(char*)ws};
     const size_t n = (size_t)g.T * g.topk;
     arrived = c.take<int>(g.T);  // counters first: zero before the first run, and left so by every run

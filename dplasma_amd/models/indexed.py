@@ -35,7 +35,10 @@ from ..runtime import Taskpool
 _LIMIT = 4194240      # tokens or features: 65535 tiles of 64 along one grid axis
 _FAMILY = 65535       # adapters: one grid axis
 _RANK = 262140        # 65535 groups of 4 along one grid axis
-_FACTORS = 2 ** 23    # adapters times tiles of 256 features: the workgroups of the factors' gradients
+# a launch holds less than 2^32 threads:
+_FACTORS = 2 ** 23 - 1         # adapters and windows of tokens, times tiles of 256 features: workgroups of 256 threads of
+                               # one factor's gradient, both in one launch
+_EXPERT = 16 * (2 ** 23 - 1)   # features of tokens and experts: a workgroup of 512 threads for 16 of them
 
 
 def _matrix(op, ctx, name, M, m, n, dtype):
@@ -196,8 +199,10 @@ def gemm_lora_grad_New(ctx, alpha, W, X, A, B, ids, scale, dY, dX, dA, dB) -> Ta
             if nb:
                 _family(op, name, M, nb)
     _lora_checks(op, ctx, W, X, A, B, ids, scale, N, [o[:2] for o in outputs if o[1] is not None], [("dY", dY)])
-    if A.n // r * -(-max(K, N) // 256) > _FACTORS:
-        raise ValueError(f"{op}: {A.n // r} adapters of {max(K, N)} features are more than {_FACTORS} tiles of 256")
+    windows = (T + 8 * (A.n // r) + 16) // 256 + 1
+    if (A.n // r + windows) * -(-max(K, N) // 256) > _FACTORS:
+        raise ValueError(f"{op}: {A.n // r} adapters of {max(K, N)} features and {T} tokens are more than {_FACTORS} "
+                         f"tiles of 256")
     W, X, A, B, dY, dX, dA, dB = _bound(W, X, A, B, dY, dX, dA, dB)
     return _pool(ctx, op,
                  lambda: ops.lora_call(ctx.device, float(alpha), W, X, A, B, ids, scale, dY=dY, dX=dX, dA=dA, dB=dB),
@@ -236,7 +241,9 @@ def moe_New(ctx, topk, norm, G, W1, W2, alpha, X, beta, Y) -> Taskpool:
     _matrix(op, ctx, "W2", W2, width, E * H, dtype)
     if T > 65535:
         raise ValueError(f"{op}: at most 65535 tokens, got {T}")
-    _extent(op, H=H, I=2 * width, E=E * 2 * width)
+    if max(H, width) > _EXPERT:
+        raise ValueError(f"{op}: at most {_EXPERT} features, got {H} and {width} of an expert")
+    _extent(op, E=E * 2 * width)
     _disjoint(op, [("Y", Y)], [("G", G), ("W1", W1), ("W2", W2), ("X", X)])
     G, W1, W2, X, Y = _bound(G, W1, W2, X, Y)
     return _pool(ctx, op, lambda: ops.moe_call(ctx.device, int(topk), bool(norm), G, W1, W2, float(alpha), X,

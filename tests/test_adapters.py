@@ -267,3 +267,19 @@ def test_a_taskpool_keeps_its_storages(ctx):
     for got, (want, bound), what in zip(outs, c.plain_backward(), ("dx", "da", "db")):
         within(got, want, bound, what)
     within(out, *m.plain(), "moe")
+
+
+def test_workgroups_past_a_launch_are_refused(ctx):
+    """Extents that fit a grid's axes and have more threads than a launch holds (storage that is never touched)."""
+    L, K = 65535, 32640  # 65535 x 128 tiles of 256 features are below 2^23, with the windows of the tokens they are not
+    W, X, dY = matrix(torch.empty(K, K, dtype=H)), matrix(torch.empty(2, K, dtype=H)), matrix(torch.empty(2, K, dtype=H))
+    A, Bd = matrix(torch.empty(L, K, dtype=H), 1), matrix(torch.empty(L * K, 1, dtype=H), K)
+    dA, dB = matrix(torch.empty(L, K, dtype=H), 1), matrix(torch.empty(L * K, 1, dtype=H), K)
+    with pytest.raises(ValueError, match="tiles of 256"):
+        dp.gemm_lora_grad_New(ctx, 1.0, W, X, A, Bd, torch.zeros(2, dtype=torch.int32), None, dY, None, dA, dB)
+    wide = 16 * (2 ** 23 - 1) + 1  # 2^23 workgroups of 512 threads
+    for h, i in ((wide, 1), (1, wide)):
+        x, y, g = (matrix(torch.empty(1, h, dtype=H)) for _ in range(3))
+        w1, w2 = matrix(torch.empty(2 * i, h, dtype=H), 2 * i), matrix(torch.empty(h, i, dtype=H), h)
+        with pytest.raises(ValueError, match="features"):
+            dp.moe_New(ctx, 1, True, g, w1, w2, 1.0, x, 0.0, y)
