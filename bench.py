@@ -116,6 +116,7 @@ def _choose_engine(ctx, uplo, A, A0, tp, args):
 
     import dplasma_amd as dp
     from dplasma_amd.models import potrf_dtr_dist
+    from dplasma_amd.parallel import comm
     if os.environ.get("DPLASMA_BENCH_DIST_ENGINE", "race") == "stream" or args.cpu or \
             not potrf_dtr_dist.supported(ctx, uplo, A):
         return tp, "stream"
@@ -123,7 +124,7 @@ def _choose_engine(ctx, uplo, A, A0, tp, args):
 
     def agree(v, op):
         t = torch.tensor([float(v)], dtype=torch.float64, device=dev)
-        dist.all_reduce(t, op=op)
+        comm.allreduce(t, op=op)
         return float(t.item())
 
     def timed(t, poison=False):
@@ -268,7 +269,8 @@ def main():
     info = tp.complete(ctx)
     el = torch.tensor([total], dtype=torch.float64, device=ctx.device)
     if world > 1:
-        dist.all_reduce(el, op=dist.ReduceOp.MAX)
+        from dplasma_amd.parallel import comm
+        comm.allreduce(el, op=dist.ReduceOp.MAX)
     elapsed = float(el.item())
     ms = elapsed / args.steps * 1e3
     gflops = flops * args.steps / elapsed / 1e9

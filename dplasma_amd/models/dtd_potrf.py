@@ -113,8 +113,8 @@ def _info_reducer(ctx, info):
     def _done():
         v = info.clone()
         if ctx.world > 1:
-            import torch.distributed as dist
-            dist.all_reduce(v, op=dist.ReduceOp.MAX)
+            from ..parallel import comm
+            comm.allreduce(v, op=torch.distributed.ReduceOp.MAX)
         return int(v.item())
     return _done
 

@@ -11,6 +11,7 @@ from __future__ import annotations
 from ..constants import dplasmaNoTrans
 from ..ops import tile_ops as ops
 from ..ops.batch import TileBatch
+from ..parallel import comm
 from ..parallel.exchange import ExchangePlan
 
 
@@ -61,15 +62,13 @@ def redistribute(ctx, src, dst, m=None, n=None, si=0, sj=0, di=0, dj=0):
 
 def _redistribute_elementwise(ctx, src, dst, m, n, si, sj, di, dj):
     """General (unaligned) redistribution through a dense all-gather -- small/compat use only."""
-    import torch
-    import torch.distributed as dist
     full = src.to_dense_local().to(src.device)
     if ctx.world > 1:
-        dist.all_reduce(full)
+        comm.allreduce(full)
     block = full[si:si + m, sj:sj + n]
     dense = dst.to_dense_local().to(dst.device)
     if ctx.world > 1:
-        dist.all_reduce(dense)
+        comm.allreduce(dense)
     dense[di:di + m, dj:dj + n] = block
     dst.from_dense(dense)
     return dst

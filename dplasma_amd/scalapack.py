@@ -174,9 +174,9 @@ def _make(prec):
                         if g < len(vals):
                             vals[g] = t[c % ibv, c]
             if ctx.world > 1:
-                import torch.distributed as dist
+                from .parallel import comm
                 v = vals.to(Asub.device)
-                dist.all_reduce(v)
+                comm.allreduce(v)
                 vals = v.cpu()
             tau[: len(vals)] = vals.to(tau.device)
         return 0, TS, TT, tree

@@ -834,9 +834,9 @@ def _inf(x) -> float:
 def _dense(h, X):
     d = X.to_dense_local().cpu()
     if h.ctx.world > 1:
-        import torch.distributed as dist
+        from .parallel import comm
         t = d.to(h.ctx.device)
-        dist.all_reduce(t)
+        comm.allreduce(t)
         d = t.cpu()
     return d
 
