@@ -586,3 +586,29 @@ def test_a_taskpool_keeps_its_storages(ctx):
     for got, (value, bound), what in zip(outs, (want, back, mixed), ("y", "dx", "moe")):
         within(got, value, bound, what)
     assert all(torch.isnan(o).all() for o in others)
+
+
+# x of few tokens in whole lines: every number of fragments of tokens and of features that these kernels are made for, in 16
+# and 32 bits, with waves that have no step, four, and one to four rounds of four more, and a last step that K ends inside
+LINES = [
+    (B, 1, 4096, 4200, 16, 4, "tokens", 0), (H, 1, 8192, 264, 40, 3, "one", 0), (B, 16, 4104, 264, 8, 5, "tokens", 8),
+    (H, 9, 2048, 136, 70, 3, "tokens", 0), (S, 1, 2048, 130, 33, 2, "one", 0), (S, 16, 4100, 72, 8, 3, "tokens", 4),
+    (S, 7, 1024, 264, 8, 3, "runs", 0), (B, 17, 4096, 264, 16, 4, "tokens", 0), (H, 32, 520, 136, 33, 6, "tokens", 0),
+    (S, 20, 4100, 264, 8, 3, "tokens", 0), (S, 32, 256, 72, 8, 3, "tokens", 0), (H, 32, 4104, 8200, 12, 7, "tokens", 8),
+    (B, 20, 8192, 8192, 16, 3, "runs", 0), (B, 18, 512, 8192, 8, 3, "tokens", 0), (S, 32, 2048, 8192, 8, 3, "tokens", 0),
+    (S, 17, 260, 8196, 70, 2, "tokens", 0), (H, 48, 8192, 264, 16, 5, "tokens", 0), (B, 33, 2056, 520, 64, 4, "tokens", 8),
+    (S, 40, 2048, 136, 8, 3, "tokens", 0), (B, 48, 4096, 8192, 16, 32, "tokens", 0), (H, 40, 1024, 8264, 24, 4, "tokens", 0),
+    (S, 33, 1028, 8200, 8, 3, "tokens", 0), (S, 48, 4100, 8192, 8, 3, "runs", 4), (B, 64, 8192, 520, 16, 64, "tokens", 0),
+    (H, 50, 4104, 264, 100, 3, "tokens", 8), (S, 64, 2052, 264, 8, 3, "tokens", 0), (H, 64, 4104, 8264, 16, 9, "tokens", 0),
+    (B, 50, 1024, 8192, 8, 3, "tokens", 0), (S, 64, 4100, 8192, 8, 3, "tokens", 0),
+]
+
+
+@pytest.mark.parametrize("case", LINES, ids=str)
+def test_lora_of_few_tokens_in_whole_lines(ctx, case):
+    c = lora(*case)
+    y = c.forward(ctx, -0.5, 2.0)
+    within(y[:, :c.N], *c.plain(-0.5, 2.0), "y")
+    assert torch.equal(y[:, c.N:], c.y[:, c.N:])
+    for _ in range(3):
+        assert torch.equal(y, c.forward(ctx, -0.5, 2.0))
