@@ -91,8 +91,8 @@ __global__ __launch_bounds__(1024) void k_one(const T* __restrict__ x, const T* 
 //     each wave fills for itself, straight from memory (rows laid out as in k_tile); W four steps ahead in registers.
 //   else: x in fragments from any address, in batches as large as the registers of one workgroup per CU allow.
 // (T x K x N, us without and with LINES: 48 x 4096 x 8192 30.5, 27.3; 48 x 4096 x 4096 23.0, 16.4; 48 x 1024 x 4096 12.0,
-// 10.8; 16 x 4096 x 8192 24.5, 20.5; 16 x 1024 x 4096 9.0, 9.2.)  What is left at 48 x 4096 x 8192: the way through
-// memory of the low-rank vectors, 5 us, and the beginning and end of one round of workgroups around 67 MB at 4.4 TB/s.
+// 10.8; 16 x 4096 x 8192 24.5, 20.5; 16 x 1024 x 4096 9.0, 9.2.)  What is left at 48 x 4096 x 8192: the launch of the
+// low-rank vectors, 4 us, and one round of workgroups in which W comes at 3.2 TB/s, 67 MB in 21 us.
 constexpr int S_MAX = 64;  // r up to which the low-rank vectors go through LDS
 
 template <typename T, int G, int NF, bool LINES>

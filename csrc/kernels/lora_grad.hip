@@ -347,11 +347,13 @@ template <typename T> __global__ __launch_bounds__(256) void k_join(OuterArgs a)
   }
 }
 
-// places in all, and a window's length: about 192 workgroups for both factors, which with the ends of adapters is one
-// round of the CUs (one each: the buffers take most of a CU's LDS) and leaves few parts to join, in whole steps, a window's
-// tokens in LDS; few tokens stay in one window, which needs no join.  (Both factors, us so and with 512 workgroups for
-// each: 8192 tokens, 4096 and 16384 features, r 64, 8 adapters 271, 325; 4096 tokens, 4096 features, r 16 43.0, 48; 2048
-// tokens, 2048 features, r 32 35.2, 34.8.)
+// places in all, and a window's length: both factors have (windows + adapters) workgroups for each of their tiles of columns
+// and ranks, one to a CU (the buffers take most of its LDS).  The windows alone are to make about 192 of them, in whole
+// steps, as far as WIN_MAX allows, whose tokens lie in LDS: with few adapters one round of the CUs and few parts to join
+// (4096 tokens, 4096 features, r 16, one adapter: 192 workgroups).  With many it is more: 8192 tokens, 4096 and 16384 features,
+// 8 adapters are 4 windows of 2048 and 12 items for 80 tiles, 960 workgroups in nearly four rounds.  Few tokens stay in one
+// window, which needs no join.  (us of the whole gradient so, and with 1024 in the place of 192: 8192 tokens, r 64, as above
+// 1073, 1099; 4096 tokens, 4096 features, r 16 156, 161; 2048 tokens, 2048 features, r 32, 4 adapters 61, 60.)
 long long places(const LoraArgs& g) { return cdiv(g.T, 8) * 8ll + 8ll * (g.L + 1); }
 int window(const LoraArgs& g) {
   if (places(g) <= 512) return 512;

@@ -178,8 +178,14 @@ __global__ __launch_bounds__(DMA && JF * TF >= 4 ? 256 : 512) void k_low_tile(Lo
 template <typename T> int run_low(const LowSets& sets, hipStream_t st) {
   const LowArgs& a = sets.set[0];
   // one wave per (token, j) for few tokens, and up to 512 where a tile's tokens would go through several adapters one after
-  // the other (us in all, by tiles and so: 300 x 4096 x 1024, r 32, 16 adapters 36.1, 31.0; 413 x 2040 x 5001, r 12, 9
-  // adapters 38.6, 36.0; 512 x 4096 x 4096, r 16, one adapter 37.9, 38.9; 500 x 4096 x 1024, r 64, 16 adapters 42.0, 44.0)
+  // the other.  Tokens x K x N, us of the whole product by tiles and so (bf16 unless said):
+  //   65 x 4096 x 1024, one adapter: r 8 24.8, 22.6, r 64 29.9, 25.5; 32 adapters in any order: r 16 95.6, 47.1
+  //   256 x 4096 x 1024, one adapter: r 16 25.3, 24.2, r 64 30.7, 31.4; 4 in runs, r 64: 42.1, 33.1; 32: r 16 91.9, 45.9
+  //   256 tokens, one adapter: fp16 2015 x 1001 r 16 30.6, 29.9, r 64 38.2, 41.7; fp32 2048 x 1024 r 64 59.3, 54.5
+  //   300 x 4096 x 1024, r 32, 16 adapters: in runs 41.5, 30.0, in any order 91.5, 39.4
+  //   413 x 2040 x 5001, fp16, r 12, 9 adapters in runs: 40.5, 34.2
+  //   512 x 4096 x 1024, r 32: one adapter 26.6, 29.7, 4 in runs 31.7, 30.6; 500, r 64, one adapter 30.5, 38.4
+  // (500 x 4096 x 1024, r 64, 16 adapters would be better so too: in runs 48.4, 43.2, in any order 135.5, 60.4.)
   if (a.nt <= 256 || (a.nt <= 512 && a.r <= 32 && a.L > 1)) {
     k_low_dot<T><<<dim3(a.nt, cdiv(a.r, 4), sets.sets), 256, 0, st>>>(sets);
     return (int)hipGetLastError();
@@ -209,24 +215,25 @@ template <typename T> int run_low(const LowSets& sets, hipStream_t st) {
 
 // ---------------------------------------------------------------- shared product
 // A workgroup owns B tokens x B features, WT x WN waves of (B / WT) x (B / WN).  The contraction goes in steps of 128
-// bytes of a row (whole cache lines: with 64-byte steps the same lines were asked for twice, 1.12 against 1.13 PFLOP/s at
-// 16384 x 4096 x 16384, and 1.26 against 1.38 where all of it lies in the L2) through LDS buffers, each step in two
+// bytes of a row (whole cache lines: with 64-byte steps, which ask for the same lines twice, an earlier form of this kernel
+// took 1 % longer at 16384 x 4096 x 16384, and 10 % where all of it lies in the L2) through LDS buffers, each step in two
 // halves of one fragment.  While a half is multiplied from registers the fragments of the next one are read from LDS;
 // when a step's second half is in registers its buffers take a later step.  So neither latency is waited for, and a step
 // has one barrier.  SLOTS buffers, each of one operand's part of a step, X and W in turn: 4 (a step ahead) where several
 // workgroups share a CU, 8 where few share the chip and a step's products are much shorter than the way from memory, and
-// 5, all of the LDS, with the largest tile: X then has two steps to arrive (16384 x 4096 x 16384: 1.25 PFLOP/s with 4,
-// 1.31 with 5, W's features contiguous 1.20 and 1.37; W two steps instead of X: the same).
-// What bounds the largest tile: power.  At 16384 x 4096 x 16384 (1.67 ms) the matrix pipes are busy 71 % of the time (W's
-// features contiguous: 80 %) at the 1.77 (1.72) GHz that the card's limit leaves; the library's product runs at 85 % and
-// 1.50 GHz, 1.64 to 1.70 ms.  (4 waves of 128 x 128 would read a third less from LDS, but with 256 accumulators a lane the
+// 5, all of the LDS, with the largest tile: X then has two steps to arrive (16384 x 4096 x 16384, r 64: 1899 us with 4, 1796
+// with 5; a gradient with dX of 8192 x 16384 x 4096, W's features contiguous: 1193, 1071; W two steps instead of X: the same).
+// What bounds the largest tile: power.  At 16384 x 4096 x 16384 (1.76 ms) the matrix pipes are busy 65 % of the time (8192 x
+// 16384 x 4096, W's features contiguous: 72 %) at the 1.9 GHz that the card's limit leaves; the library's product runs at
+// 85 % and 1.50 GHz, 1.64 to 1.70 ms.  (4 waves of 128 x 128 would read a third less from LDS, but with 256 accumulators a lane the
 // compiler moves them about: 1.04 PFLOP/s.)
 //   DMA: rows begin at multiples of 16 bytes and the tile's rows lie within 2^30 bytes: memory to LDS directly.
 //        A chunk past the rows' end is fetched from past the buffer descriptor's end, which reads as zero.
 //   else: through registers, 16 bytes from any address, with zeros past the rows' end, one step ahead of the buffers on a
 //     128 tile and two on a 64 tile (bf16, 184 x 4429 x 704: 38.3 us with 4, 36.5 with 2; 4097^3: 302 with 2, 292 with 1).
 // LDS rows are 8 chunks of 16 bytes; chunk c of row i lies at c ^ (i & 7), so that the rows that a fragment read takes
-// the same chunk of lie in different banks (no conflicts by the counter).  W stored with its features contiguous (NT false) is kept as it comes,
+// the same chunk of lie in different banks: the counter's 6144 cycles of conflicts a tile are the same with K = 4096 as
+// with 8192, so they are the output's and not the steps'.  W stored with its features contiguous (NT false) is kept as it comes,
 // [step][features], and read through the transposing LDS read: a group of 16 lanes takes 4 steps x 16 features; the
 // 32-byte pair of such a read is displaced by the step's place in the instruction (16 steps of one instruction: 8 pairs).
 // s and d read element by element there, a lane group q its own E steps, with the 16 features of a fragment displaced by q
@@ -245,7 +252,7 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, c16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wt = wave / WN, wn = wave % WN;
   // tiles of one XCD's workgroups: 4 tile rows of tokens at a time, tokens fastest, so that they share rows in its L2
-  // (4 / 8 / 16 rows: 1.12 / 1.03 / 1.04 PFLOP/s at 16384 x 4096 x 16384)
+  // (4 / 8 / 16 rows: 1796 / 1803 / 1835 us at 16384 x 4096 x 16384, 801 / 812 / 836 at 8192^3)
   const int tt = (a.T + B - 1) / B, tn = (a.N + B - 1) / B;
   const int id = xcd_remap(blockIdx.x, tt * tn);
   const int group = id / (4 * tn), in = id % (4 * tn), gs = min(4, tt - group * 4);
@@ -281,7 +288,7 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_tile(TileArgs a) {
   const unsigned wbytes = DMA ? (unsigned)((NT ? (rn - 1) * a.ldw + a.C : (a.C - 1) * a.ldw + rn) * (long long)sizeof(T)) : 0;
   const int steps = (a.C + BK - 1) / BK;
   // each XCD begins at another eighth of the contraction: beginning together they all ask for the same rows of W at
-  // once (1.13 -> 1.20 PFLOP/s at 16384 x 4096 x 16384, 1.26 -> 1.35 at 8192^3)
+  // once (1888 us, so 1796 at 16384 x 4096 x 16384; 850, 801 at 8192^3)
   const int turned = steps / 8 * (blockIdx.x & 7);
   auto place = [&](int s) { return (s >= steps ? s : s + turned >= steps ? s + turned - steps : s + turned) * BK; };
   auto stage_x = [&](int s, char* slot) {  // steps past the last one read as zero

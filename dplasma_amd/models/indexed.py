@@ -18,7 +18,8 @@ A taskpool runs on the stream that is current when it is run, takes the operands
 makes no allocation and no host synchronisation, and may be captured into a HIP graph (moe's is built before the
 capture).  Its operands are the storages that the descriptors have when it is built, and it holds on to them: a tensor
 that is bound to a descriptor later is another matrix's.  It owns its workspace, so one taskpool (and every graph that
-captured it) has one run in flight at a time, and it lives as long as those graphs.
+captured it) has one run in flight at a time, and it lives as long as those graphs.  Building one takes tens of
+microseconds and waits for the current stream; the number of tokens is fixed in it.
 Outputs must not overlap inputs.  An infinity or NaN in one adapter, expert, token or output's weights makes what it meets
 infinite or NaN (in h and b an infinity of a factor may come out as NaN) and nothing else.
 """
@@ -222,8 +223,8 @@ def moe_New(ctx, topk, norm, G, W1, W2, alpha, X, beta, Y) -> Taskpool:
     G: H x E, the router.  W1: H x (E 2I) in tiles of 2I columns, expert e's gate (the first I) and up projections.
     W2: I x (E H) in tiles of H columns, its down projections.  X, Y: H x T.  The logits z = G^T x_t are summed in 64
     bits and the topk largest taken, ties by the lowest index; w is the softmax over all E logits at the chosen ones,
-    divided by its sum over them where ``norm`` is true.  Meant for a few tokens: every chosen expert's weights are
-    read once for up to 64 of its tokens.
+    divided by its sum over them where ``norm`` is true.  Meant for a few tokens: they go in batches of 64 (of 512 / topk
+    with more than 8 experts a token), and every batch reads the weights of the experts that it uses.
     """
     op = "moe"
     dtype, H, T, E, width = _precision(op, X), X.m, X.n, G.n, W2.m

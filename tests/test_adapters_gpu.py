@@ -612,3 +612,36 @@ def test_lora_of_few_tokens_in_whole_lines(ctx, case):
     assert torch.equal(y[:, c.N:], c.y[:, c.N:])
     for _ in range(3):
         assert torch.equal(y, c.forward(ctx, -0.5, 2.0))
+
+
+def test_built_inside_a_capture(ctx):
+    """gemm_lora and its gradient built and run while a graph is captured, with other work between the replays."""
+    c = lora(B, 100, 256, 320, 16, 4, "tokens")
+    y, dx = torch.empty(100, 320, dtype=B, device="cuda:0"), torch.empty_like(c.x)
+    da, db = torch.empty_like(c.a), torch.empty_like(c.b)
+    W, X, A, Bd = c.descriptors()
+
+    def build():
+        return (dp.gemm_lora_New(ctx, 1.0, W, X, A, Bd, c.ids, c.scale, 0.0, matrix(y)),
+                dp.gemm_lora_grad_New(ctx, 1.0, W, X, A, Bd, c.ids, c.scale, matrix(c.dy), matrix(dx),
+                                      matrix(da.view(-1, 256), 16), matrix(db.view(-1, 16), 320)))
+    for tp in build():
+        tp.execute(ctx)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        pools = build()
+        for tp in pools:
+            tp.run(ctx)
+    gen = torch.Generator(device="cuda:0").manual_seed(5)
+    for _ in range(3):
+        c.x.copy_(torch.randn(c.x.shape, generator=gen, device="cuda:0"))
+        c.ids.copy_(torch.randint(-1, 4, c.ids.shape, generator=gen, device="cuda:0", dtype=torch.int32))
+        other = [torch.full((1 << 20,), NAN, device="cuda:0") for _ in range(4)]
+        graph.replay()
+        torch.cuda.synchronize()
+        within(y, *c.plain(), "y")
+        for got, (want, bound), what in zip((dx, da, db), c.plain_backward(), ("dx", "da", "db")):
+            within(got, want, bound, what)
+        assert all(torch.isnan(o).all() for o in other)
+    for tp in pools:
+        tp.destruct()
