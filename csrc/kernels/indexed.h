@@ -108,8 +108,7 @@ template <typename V> __device__ inline V keep(V v, bool in) {
 // A 32-bit result that is the next product's operand.  It lies in memory as it is (64 bits in d).  For h and b it goes to
 // the 16-bit matrix instructions as three bf16 numbers of 8 bits each whose sum it is, over the whole range of 32-bit
 // numbers: nothing is rounded between the two products.  The second product's own operand is exact in one bf16 (b) or two
-// (h); of the six products of an h pair the smallest, below 2^-24 of the whole and so below the rounding of a 32-bit
-// product, is left out.  s and d take it as it is.
+// (h), so three or six products of the instruction's are the exact product.  s and d take it as it is.
 //
 // Mem: a lane's intermediates as they come from memory, Op<T>::E of them.
 template <typename T> struct Mem {  // h, b
@@ -186,7 +185,7 @@ template <> struct MidOp<__bf16> {
   __device__ inline f4_t product_first(int k, const Mid<__bf16>& m, f4_t c) const { return Op<__bf16>::mma(m.part[k], f, c); }
 };
 template <> struct MidOp<_Float16> {
-  static constexpr int N = 5;
+  static constexpr int N = 6;
   b8_t f, g;
   // 11 bits: the upper 8 by truncation, the rest exactly in the second number (none beside an infinity)
   __device__ inline void set(h8_t v) {

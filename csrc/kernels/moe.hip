@@ -440,10 +440,11 @@ __global__ __launch_bounds__(512, 4) void k_moe_down(const typename Num<T>::acc*
           f.set(wv[u]);
 #pragma unroll
           for (int g = 0; g < G; ++g) {
-            Mid<T> m;
-            m.set(h[u][g]);
+            if (g && 16 * g >= m) continue;  // no slot of this unit (48 tokens, 2 of 8 experts of 2048 x 2048: 85 us without, 75)
+            Mid<T> p;
+            p.set(h[u][g]);
 #pragma unroll
-            for (int k = 0; k < MidOp<T>::N; ++k) acc[g] = f.product(k, m, acc[g]);
+            for (int k = 0; k < MidOp<T>::N; ++k) acc[g] = f.product(k, p, acc[g]);
           }
         }
         s += U;
@@ -457,10 +458,10 @@ __global__ __launch_bounds__(512, 4) void k_moe_down(const typename Num<T>::acc*
         for (int g = 0; g < G; ++g) {
           Mem<T> h;
           h.load_to(pa[g] + s * KS, left);
-          Mid<T> m;
-          m.set(h);
+          Mid<T> p;
+          p.set(h);
 #pragma unroll
-          for (int k = 0; k < MidOp<T>::N; ++k) acc[g] = f.product(k, m, acc[g]);
+          for (int k = 0; k < MidOp<T>::N; ++k) acc[g] = f.product(k, p, acc[g]);
         }
       }
 #pragma unroll

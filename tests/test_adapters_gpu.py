@@ -645,3 +645,44 @@ def test_built_inside_a_capture(ctx):
         assert all(torch.isnan(o).all() for o in other)
     for tp in pools:
         tp.destruct()
+
+
+@pytest.mark.parametrize("T", [70, 600])
+def test_products_of_half_precision_keep_every_part(ctx, T):
+    """The last 8 of a low-rank number's 24 bits against the last 3 of a half precision number's 11."""
+    last, z = 255 * 2.0 ** -23, 1 + 7 * 2.0 ** -10
+    c = lora(H, T, 24, 72, 2, 1, "one")
+    c.w.zero_()
+    first = torch.zeros(2, 72, dtype=D)  # against [1, 2^-4, 0 ..]: 1 + 2^-8 + last, and 1 + 2^-8
+    first[:, 0], first[0, 1] = 1 + 2.0 ** -8, 16 * last
+    one = torch.tensor([1, 2.0 ** -4] + [0] * 70, dtype=D)
+    c.x[:], c.a[0] = one[:24].to(c.x), first[:, :24].to(c.a)
+    c.b[0, :, 0], c.b[0, :, 1] = z, -z
+    # all but the last parts cancel, each of a product's parts has at most 16 bits: sums are exact, the result is rounded once
+    y = c.forward(ctx, 1024.0, scale=False).double()
+    want = 1024 * z * last
+    assert ((y - want).abs() <= 2.0 ** -11 * want).all(), float((y - want).abs().max() / want)
+    c.dy[:], c.b[0] = one.to(c.dy), first.t().to(c.b)
+    c.a[0, 0], c.a[0, 1] = z, -z
+    dx = c.backward(ctx, 1024.0, scale=False, want="x")[0].double()
+    assert ((dx - want).abs() <= 2.0 ** -11 * want).all(), float((dx - want).abs().max() / want)
+    # even tokens have the last bits; T / 2 of these terms are summed, in 32 bits
+    c.dy[1::2, 1] = 0
+    c.x[:] = torch.where(torch.arange(T) % 2 == 0, z, -z)[:, None].to(c.x)
+    da = c.backward(ctx, 1024.0, scale=False, want="a")[1][0, 0].double()
+    want *= T // 2
+    assert ((da - want).abs() <= (2.0 ** -11 + T * 2.0 ** -24) * want).all(), float((da - want).abs().max() / want)
+
+
+@pytest.mark.parametrize("T", [3, 20, 60])
+def test_experts_of_half_precision_keep_every_part(ctx, T):
+    last, z = 255 * 2.0 ** -23, 1 + 7 * 2.0 ** -10
+    c = moe(H, T, 40, 16, 1, 1)
+    c.x.zero_(), c.w1.zero_(), c.w2.zero_()
+    c.x[:, 0], c.x[:, 1] = 1, 2.0 ** -4
+    c.w1[0, :16, 0] = 32  # silu(32) is 32 in 32 bits
+    c.w1[0, 16:18, 0], c.w1[0, 16, 1] = 1 + 2.0 ** -8, 16 * last
+    c.w2[0, :, 0], c.w2[0, :, 1] = z, -z
+    y = c.forward(ctx, True, 1024.0).double()
+    want = 1024 * 32 * z * last
+    assert ((y - want).abs() <= 2.0 ** -11 * want).all(), float((y - want).abs().max() / want)
