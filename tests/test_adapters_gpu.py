@@ -489,7 +489,7 @@ def test_low_rank_vectors_keep_32_bits(ctx, T, dtype, b):
     c.x[:], c.a[0] = one.to(c.x), rows.to(c.a)
     c.b[0, :, 0], c.b[0, :, 1] = b, -b
     # S is exact.  Its product with B is a sum of at most 12 numbers whose partial sums stay below 1.01, each rounded by
-    # 2^-24 at most, and what is left out of an fp16 pair is below 2^-24: 13 2^-24 1.01, times alpha, below 2^-10
+    # 2^-24 at most: 12 2^-24 1.01, times alpha, below 2^-10
     y = c.forward(ctx, 1024.0, scale=False).double()
     want = b * 2.0 ** -7
     assert ((y - want).abs() <= 2.0 ** -10 + 2.0 ** -8 * want).all(), float((y - want).abs().max())
@@ -509,8 +509,8 @@ def test_gradients_of_the_factors_keep_32_bits(ctx, T, dtype, z, r):
     c = lora(dtype, T, 24, 72, r, 1, "one")
     sign = torch.where(torch.arange(T) % 2 == 0, z, -z)[:, None]
     # Every product of parts is a multiple of 2^-19, and no more than 16 tokens of one sign come one after the other (an
-    # instruction adds 32), so partial sums below 2^4.1 are exact in 32 bits in any order.  What is left out of an fp16
-    # pair is 2^-10 of 2^-17 each; the result is rounded once.  Ranks past the first are not looked at
+    # instruction adds 32), so partial sums below 2^4.1 are exact in 32 bits in any order, but for the products of the last
+    # parts, 2^-10 of 2^-17 each; the result is rounded once.  Ranks past the first are not looked at
     room = 2.0 ** -8 + 2.0 ** -10
     for n, what in ((72, "a"), (24, "b")):
         rows, one = _third(n)
@@ -540,7 +540,7 @@ def test_moe_activations_keep_32_bits(ctx, T, I, dtype, b):
     c.w1[0, I:I + 2] = rows.to(c.w1)
     c.w2.zero_()
     c.w2[0, :, 0], c.w2[0, :, 1] = b, -b
-    # as for the low-rank vectors, with partial sums below 33: 13 2^-24 33 1024 < 2^-5
+    # as for the low-rank vectors, with partial sums below 33: 12 2^-24 33 1024 < 2^-5
     y = c.forward(ctx, True, 1024.0).double()
     want = b * 2.0 ** -2
     assert ((y - want).abs() <= 2.0 ** -5 + 2.0 ** -8 * want).all(), float((y - want).abs().max())
